@@ -18,6 +18,9 @@ CSRC = os.path.join(HERE, "csrc")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
+# scalar fp32 VALU forms only: some packed fp32 forms that -O3 makes from ordinary float code have given wrong results
+# now and then on this hardware.  (The host pass warns that it does not know the feature; harmless.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
@@ -50,7 +53,7 @@ def build(verbose: bool = False, force: bool = False, jobs: int = 0) -> str:
     inc = ["-I" + pybind11.get_include(), "-I" + sysconfig.get_paths()["include"], "-I" + CSRC,
            "-I" + os.path.join(ROCM, "include")]
     common = [HIPCC, "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
-              "-Wno-unused-result"] + inc + os.environ.get("DPA_BUILD_DEFS", "").split()
+              "-Wno-unused-result"] + NO_PACKED_FP32 + inc + os.environ.get("DPA_BUILD_DEFS", "").split()
     hmt = _headers_mtime()
     todo, objs = [], []
     for src in _sources():

@@ -73,9 +73,9 @@ template <typename T> struct Vec16 {
 
 // ---- relu(scale * x + shift) on one 16-byte chunk (BatchNorm + ReLU applied while an operand tile is staged) -----
 // Bit-identical to the stand-alone bn_apply pass: fp32 fma, one rounding to T, ReLU.  The bf16 version is written
-// for the VALU budget of the GEMM loops that host it: packed fp32 fma (v_pk_fma_f32), packed convert
+// for the VALU budget of the GEMM loops that host it: two scalar fp32 fma (the build keeps packed fp32 off), packed convert
 // (v_cvt_pk_bf16_f32) and the ReLU as a packed signed-16-bit max with zero on the ROUNDED pair (a negative bf16 has
-// its sign bit set, i.e. is a negative int16; -0.0 becomes +0.0 like fmaxf(x, 0) does) -- 5 VALU ops per two elements.
+// its sign bit set, i.e. is a negative int16; -0.0 becomes +0.0 like fmaxf(x, 0) does) -- 6 VALU ops per two elements.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short s16x2_t __attribute__((ext_vector_type(2)));
@@ -95,7 +95,7 @@ __device__ __forceinline__ uint32_t bn_relu_pair_bf16(uint32_t w, f32x2_t sc, f3
   return r;
 }
 
-// ---- packed bf16 pair arithmetic for the streaming epilogues (v_pk_add_f32 / v_pk_fma_f32 / v_cvt_pk_bf16_f32): the
+// ---- packed bf16 pair arithmetic for the streaming epilogues (scalar fp32 math on pairs, v_cvt_pk_bf16_f32): the
 // epilogue of a fused accumulate + BN-backward launch was VALU bound at ~22 instructions per element when every element
 // went through scalar get / select / set (bench/experiments/lean_racc_ablate.py); pairs take ~8.
 __device__ __forceinline__ f32x2_t unpack_bf16x2(uint32_t w) {
