@@ -3,11 +3,12 @@
 ``python -m distributed_pytorch_amd.build`` compiles every ``csrc/kernels/*.hip`` for gfx950 with
 hipcc (cross-compiles without a GPU), the C++ runtime / binding, and links one pybind11 module that
 sits next to the package so it travels to the GPU box with the tree.  Objects are cached under
-``build/`` and rebuilt only when a source (or any header) is newer.
+``build/`` and rebuilt only when a source (or a header that it includes) is newer.
 """
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -32,13 +33,19 @@ def _sources():
     return out
 
 
-def _headers_mtime() -> float:
-    m = 0.0
-    for root, _, files in os.walk(CSRC):
-        for f in files:
-            if f.endswith(".h"):
-                m = max(m, os.path.getmtime(os.path.join(root, f)))
-    return m
+def _mtime_with_headers(path: str, seen=None) -> float:
+    """Newest modification time of a source and of the package's own headers that it includes."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path in seen or not os.path.isfile(path):
+        return 0.0
+    seen.add(path)
+    newest = os.path.getmtime(path)
+    with open(path) as f:
+        for name in re.findall(r'^\s*#include\s+"([^"]+)"', f.read(), re.M):
+            for base in (os.path.dirname(path), CSRC):
+                newest = max(newest, _mtime_with_headers(os.path.join(base, name), seen))
+    return newest
 
 
 def target_path() -> str:
@@ -54,12 +61,11 @@ def build(verbose: bool = False, force: bool = False, jobs: int = 0) -> str:
            "-I" + os.path.join(ROCM, "include")]
     common = [HIPCC, "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
               "-Wno-unused-result"] + NO_PACKED_FP32 + inc + os.environ.get("DPA_BUILD_DEFS", "").split()
-    hmt = _headers_mtime()
     todo, objs = [], []
     for src in _sources():
         obj = os.path.join(objdir, os.path.relpath(src, CSRC).replace(os.sep, "_") + ".o")
         objs.append(obj)
-        if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), hmt):
+        if force or not os.path.exists(obj) or os.path.getmtime(obj) < _mtime_with_headers(src):
             todo.append((src, obj))
 
     def compile_one(job):

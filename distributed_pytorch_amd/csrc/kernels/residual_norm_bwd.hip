@@ -1,0 +1,401 @@
+// Backward of residual_norm (gfx950).  With sh = (s - mean) / dev and yh likewise:
+//
+//     gs = ds + dpre,  dpre = (g - [layer] mean(g) - sh * mean(g sh)) / dev,  g = dh * w_pre
+//     dx = gs,  dz = scale * gate * gs,  dgate = sum scale * gs * z,  dw_pre = sum dh * sh,  db_pre = sum dh
+//     dy = dz, or the same formula of `post` applied to it;  dw_post = sum dz * yh,  db_post = sum dz
+//
+// One pass: ds, dh, x, y are read once, dx and dy written once.  s is formed again from x and y in 32 bits: the s of
+// the forward pass is rounded to T, and 1 / deviation and the sums over rows magnify that (dw_pre of bf16 rows is off by
+// 2e-3 from it, by 2e-7 from this), for one more tensor to read where there is no `post` (5 in place of 4).  The per-channel sums stay with the lane across all rows
+// that it visits (its channels never change), meet across the row groups of a wave with shuffles and across waves in
+// LDS, and every workgroup writes one partial row; residual_norm_fold_kernel adds those in a fixed order, straight into
+// the gradients' buffers.  A per-sample gate's sums are flushed at the end of every unit, a part of one sample's rows.
+#include "residual_norm_common.h"
+
+namespace dpa {
+namespace {
+using namespace rn;
+
+constexpr int kMaxParts = 768;      // workgroups of the pass = partial rows of the fold
+constexpr int kMaxUnits = 4096;     // parts of samples, where the gate is per sample
+
+// what a kernel is made for: s = x + y, s = x + scale * post(y) without `pre`, or everything
+enum Mode : int { kPreOnly = 0, kPostOnly = 1, kAll = 2 };
+
+// v[k][j] of every wave (row group) of the workgroup added up and written to out[C]; the lanes of the first group write
+template <typename T, int MAXCH, bool WIDE, bool VEC>
+__device__ __forceinline__ void merge_out(float (&v)[MAXCH][kV<T>], float* out, float* lds, int gl, int G, int C) {
+  constexpr int V = kV<T>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int k = 0; k < MAXCH; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        for (int off = 32; off >= G; off >>= 1) v[k][j] += __shfl_xor(v[k][j], off, 64);
+    __syncthreads();                                   // the buffer's last readers are done
+    if (lane < G)
+#pragma unroll
+      for (int k = 0; k < MAXCH; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) lds[(wave * MAXCH * 64 + gl + k * G) * V + j] = v[k][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += 256) {
+      float a = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) a += lds[w * MAXCH * 64 * V + c];
+      out[c] = a;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < MAXCH; ++k) {
+      const int c0 = (gl + k * G) * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c0 + j < C) out[c0 + j] = v[k][j];
+    }
+  }
+}
+
+template <typename T, int MAXCH, bool WIDE, bool VEC, int MODE>
+__global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNormBwd p, const int G, const long units,
+                                                                const long unit_rows, const int splits,
+                                                                const FastDiv by_sample) {
+  constexpr int V = kV<T>;
+  constexpr bool PRE = MODE != kPostOnly, POST = MODE != kPreOnly;
+  __shared__ float red[WIDE ? 16 : 1];
+  __shared__ float lds[WIDE ? 1 : 4 * MAXCH * 64 * V];
+  GroupSum<WIDE, 2> gsum{red};
+  const int lane = threadIdx.x & 63;
+  const int gl = WIDE ? threadIdx.x : (lane & (G - 1));
+  const int rpw = WIDE ? 1 : 64 / G;
+  const int groups = WIDE ? 1 : 4;
+  const int grp = WIDE ? 0 : threadIdx.x >> 6;
+  const int C = p.C;
+  const float invC = 1.f / (float)C;
+  const T* ds_in = reinterpret_cast<const T*>(p.ds);
+  const T* dh_in = reinterpret_cast<const T*>(p.dh);
+  const T* x_in = reinterpret_cast<const T*>(p.x);
+  const T* y_in = reinterpret_cast<const T*>(p.y);
+  T* dx = reinterpret_cast<T*>(p.dx);
+  T* dy = reinterpret_cast<T*>(p.dy);
+  const bool has_pre = PRE && p.pre != kNormNone && dh_in != nullptr;
+  const bool has_post = POST && p.post != kNormNone;
+  const bool has_gate = MODE == kAll && p.gate_kind != kGateNone;
+
+  float a_prew[PRE ? MAXCH : 1][V], a_preb[PRE ? MAXCH : 1][V], a_postw[POST ? MAXCH : 1][V], a_postb[POST ? MAXCH : 1][V],
+      a_gate[MODE == kAll ? MAXCH : 1][V];
+  auto clear = [&](auto& a) {
+    for (auto& ak : a)
+#pragma unroll
+      for (int j = 0; j < V; ++j) ak[j] = 0.f;
+  };
+  clear(a_prew); clear(a_preb); clear(a_postw); clear(a_postb); clear(a_gate);
+
+  for (long u = blockIdx.x; u < units; u += gridDim.x) {
+    // rows of this unit: a part of one sample where the gate is per sample, else a part of all rows
+    long lo, hi;
+    if (MODE == kAll && p.gate_kind == kGateSample) {
+      const long n = u / splits, part = u - n * splits;
+      lo = n * p.per_sample + part * unit_rows;
+      hi = min(lo + unit_rows, (n + 1) * p.per_sample);
+    } else {
+      lo = u * unit_rows;
+      hi = min(lo + unit_rows, p.rows);
+    }
+    for (long base = lo + grp * rpw; base < hi; base += groups * rpw) {
+      const long row = base + (WIDE ? 0 : lane / G);
+      const bool live = row < hi;
+      const int Cr = live ? C : 0;
+      const long at = live ? row * C : 0;
+      Vec16<T> dsv[MAXCH], dhv[PRE ? MAXCH : 1], xv[PRE ? MAXCH : 1], yv[MAXCH];
+#pragma unroll
+      for (int k = 0; k < MAXCH; ++k) {
+        if (ds_in != nullptr) dsv[k] = load_chunk<T, VEC>(ds_in + at, gl + k * G, Cr);
+        else dsv[k].raw = make_uint4(0u, 0u, 0u, 0u);
+        if (has_pre) {
+          dhv[k] = load_chunk<T, VEC>(dh_in + at, gl + k * G, Cr);
+          xv[k] = load_chunk<T, VEC>(x_in + at, gl + k * G, Cr);
+        }
+        if (y_in != nullptr) yv[k] = load_chunk<T, VEC>(y_in + at, gl + k * G, Cr);
+        else yv[k].raw = make_uint4(0u, 0u, 0u, 0u);
+      }
+      const long n = MODE != kPreOnly && (p.scale != nullptr || p.gate_kind == kGateSample)
+                         ? fdiv((uint32_t)(live ? row : 0), by_sample) : 0;
+      const float sc = MODE != kPreOnly && p.scale != nullptr ? p.scale[n] : 1.f;
+      const float* gate = p.gate_kind == kGateSample ? p.gate + n * C : p.gate;
+      float ymean = 0.f, yrstd = 0.f;
+      if (has_post) {
+        ymean = live ? p.post_stat[row] : 0.f;
+        yrstd = live ? p.post_stat[p.rows + row] : 0.f;
+      }
+      float g[MAXCH][V];
+#pragma unroll
+      for (int k = 0; k < MAXCH; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[k][j] = dsv[k].get(j);
+      if (has_pre) {
+        const float mean = live ? p.pre_stat[row] : 0.f, rstd = live ? p.pre_stat[p.rows + row] : 0.f;
+        float m[2] = {0.f, 0.f};
+        float sh[PRE ? MAXCH : 1][V];
+#pragma unroll
+        for (int k = 0; k < MAXCH; ++k) {
+          float w[V], f[V], pw[V], pb[V];
+          load_vec<V, VEC>(p.pre_w, gl + k * G, C, 1.f, w);
+          if (MODE == kAll) {
+            load_vec<V, VEC>(gate, gl + k * G, C, 1.f, f);
+            if (has_post) {
+              load_vec<V, VEC>(p.post_w, gl + k * G, C, 1.f, pw);
+              load_vec<V, VEC>(p.post_b, gl + k * G, C, 0.f, pb);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            float z = yv[k].get(j);
+            if (MODE == kAll) {
+              if (has_post) z = (z - ymean) * yrstd * pw[j] + pb[j];
+              z *= sc * f[j];
+            }
+            const float d = dhv[k].get(j), gw = d * w[j];      // absent: d = 0
+            sh[k][j] = (xv[k].get(j) + z - mean) * rstd;
+            m[0] += gw;
+            m[1] += gw * sh[k][j];
+            if constexpr (PRE) {
+              a_prew[k][j] += d * sh[k][j];
+              a_preb[k][j] += d;
+            }
+          }
+        }
+        gsum.run(m, G);
+        const float m0 = p.pre == kNormLayer ? m[0] * invC : 0.f, m1 = m[1] * invC;
+#pragma unroll
+        for (int k = 0; k < MAXCH; ++k) {
+          float w[V];
+          load_vec<V, VEC>(p.pre_w, gl + k * G, C, 1.f, w);
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[k][j] += rstd * (dhv[k].get(j) * w[j] - m0 - sh[k][j] * m1);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < MAXCH; ++k) {
+        Vec16<T> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.set(j, g[k][j]);
+        if (live && dx != nullptr) store_chunk<T, VEC>(o, dx + row * C, gl + k * G, C);
+      }
+      if (dy != nullptr) {
+        float m[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < MAXCH; ++k) {
+          const int c0 = (gl + k * G) * V;
+          float gt[V], w[V], b[V];
+          if (MODE == kAll) load_vec<V, VEC>(gate, gl + k * G, C, 1.f, gt);
+          if (has_post) {
+            load_vec<V, VEC>(p.post_w, gl + k * G, C, 1.f, w);
+            if (has_gate) load_vec<V, VEC>(p.post_b, gl + k * G, C, 0.f, b);
+          }
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const bool ok = live && (VEC ? c0 < C : c0 + j < C);
+            const float dzs = ok ? sc * g[k][j] : 0.f;
+            const float yj = yv[k].get(j);
+            const float yh = has_post ? (yj - ymean) * yrstd : yj;
+            if constexpr (MODE == kAll)
+              if (has_gate && ok) a_gate[k][j] += dzs * (has_post ? yh * w[j] + b[j] : yh);
+            float dz = MODE == kAll && has_gate ? dzs * gt[j] : dzs;
+            if constexpr (POST)
+              if (has_post) {
+                if (ok) {
+                  a_postw[k][j] += dz * yh;
+                  a_postb[k][j] += dz;
+                }
+                dz *= w[j];
+                m[0] += dz;
+                m[1] += dz * yh;
+              }
+            g[k][j] = dz;
+          }
+        }
+        if (has_post) {
+          gsum.run(m, G);
+          const float m0 = p.post == kNormLayer ? m[0] * invC : 0.f, m1 = m[1] * invC;
+#pragma unroll
+          for (int k = 0; k < MAXCH; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+              g[k][j] = yrstd * (g[k][j] - m0 - (yv[k].get(j) - ymean) * yrstd * m1);
+        }
+#pragma unroll
+        for (int k = 0; k < MAXCH; ++k) {
+          Vec16<T> o;
+#pragma unroll
+          for (int j = 0; j < V; ++j) o.set(j, g[k][j]);
+          if (live) store_chunk<T, VEC>(o, dy + row * C, gl + k * G, C);
+        }
+      }
+    }
+    if constexpr (MODE == kAll)
+      if (p.gate_kind == kGateSample && p.gate_partial != nullptr) {
+        merge_out<T, MAXCH, WIDE, VEC>(a_gate, p.gate_partial + u * C, lds, gl, G, C);
+        clear(a_gate);
+      }
+  }
+  if (p.partial == nullptr) return;
+  float* part = p.partial + (long)blockIdx.x * 5 * C;
+  if constexpr (PRE) {
+    if (p.out[0] != nullptr) merge_out<T, MAXCH, WIDE, VEC>(a_prew, part, lds, gl, G, C);
+    if (p.out[1] != nullptr) merge_out<T, MAXCH, WIDE, VEC>(a_preb, part + C, lds, gl, G, C);
+  }
+  if constexpr (POST) {
+    if (p.out[2] != nullptr) merge_out<T, MAXCH, WIDE, VEC>(a_postw, part + 2 * C, lds, gl, G, C);
+    if (p.out[3] != nullptr) merge_out<T, MAXCH, WIDE, VEC>(a_postb, part + 3 * C, lds, gl, G, C);
+  }
+  if constexpr (MODE == kAll)
+    if (p.out[4] != nullptr) merge_out<T, MAXCH, WIDE, VEC>(a_gate, part + 4 * C, lds, gl, G, C);
+}
+
+// out[v][c] = beta * out + sum over the partial rows, in a fixed order: 16 columns x 16 part lanes a workgroup
+struct FoldArgs {
+  const float* partial; long nparts, part_stride;
+  float* out[5]; float beta[5];
+  int C;
+};
+__global__ __launch_bounds__(256) void residual_norm_fold_kernel(const FoldArgs a) {
+  __shared__ float red[16][17];
+  const int v = blockIdx.y;
+  if (a.out[v] == nullptr) return;
+  const int cl = threadIdx.x & 15, pl = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + cl;
+  float t = 0.f;
+  if (c < a.C) {
+    const float* src = a.partial + (long)v * a.C + c;
+    long q = pl;
+    for (; q + 7 * 16 < a.nparts; q += 8 * 16) {
+      float r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = src[(q + i * 16) * a.part_stride];
+      t += ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+    }
+    for (; q < a.nparts; q += 16) t += src[q * a.part_stride];
+  }
+  red[pl][cl] = t;
+  __syncthreads();
+  if (pl == 0 && c < a.C) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += red[i][cl];
+    a.out[v][c] = a.beta[v] == 0.f ? sum : sum + a.beta[v] * a.out[v][c];
+  }
+}
+
+// dgate[n][c] = sum over the splits of sample n
+__global__ __launch_bounds__(256) void residual_norm_fold_gate_kernel(const float* __restrict__ partial, int splits, long total,
+                                                                      int C, float* __restrict__ out) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const long n = i / C, c = i - n * C;
+  float t = 0.f;
+  for (int q = 0; q < splits; ++q) t += partial[(n * splits + q) * C + c];
+  out[i] = t;
+}
+
+struct Units {
+  long units, unit_rows;
+  int splits;
+  unsigned blocks;
+};
+Units units_of(long rows, long per_sample, int C, int dtype, int gate_kind) {
+  const Plan pl = plan(C, dtype == kF32 ? 4 : 8);
+  Units u;
+  const long trip = pl.rows_per_trip;
+  if (gate_kind == kGateSample) {
+    const long samples = rows / per_sample;
+    long splits = (kMaxParts + samples - 1) / samples;
+    const long most = (per_sample + trip - 1) / trip;
+    if (splits > most) splits = most;
+    u.unit_rows = (per_sample + splits - 1) / splits;
+    u.unit_rows = (u.unit_rows + trip - 1) / trip * trip;
+    u.splits = (int)((per_sample + u.unit_rows - 1) / u.unit_rows);
+    u.units = samples * u.splits;
+    u.blocks = (unsigned)(u.units < kMaxParts ? u.units : kMaxParts);
+  } else {
+    long blocks = (rows + trip - 1) / trip;
+    if (blocks > kMaxParts) blocks = kMaxParts;
+    u.unit_rows = (rows + blocks - 1) / blocks;
+    u.unit_rows = (u.unit_rows + trip - 1) / trip * trip;
+    u.units = (rows + u.unit_rows - 1) / u.unit_rows;
+    u.splits = 1;
+    u.blocks = (unsigned)u.units;
+  }
+  return u;
+}
+
+template <typename T, int MAXCH, bool WIDE>
+void launch(const ResidualNormBwd& p, const Plan& pl, const Units& u, bool vec, int mode, hipStream_t s) {
+  const FastDiv by_sample = make_fastdiv((uint32_t)p.per_sample);
+#define DPA_RN_BWD(VECB, MODEC)                                                                                       \
+  hipLaunchKernelGGL((residual_norm_bwd_kernel<T, MAXCH, WIDE, VECB, MODEC>), dim3(u.blocks), dim3(256), 0, s, p, pl.G, \
+                     u.units, u.unit_rows, u.splits, by_sample)
+  if (!vec) DPA_RN_BWD(false, kAll);
+  else if (mode == kPreOnly) DPA_RN_BWD(true, kPreOnly);
+  else if (mode == kPostOnly) DPA_RN_BWD(true, kPostOnly);
+  else DPA_RN_BWD(true, kAll);
+#undef DPA_RN_BWD
+}
+
+}  // namespace
+
+long residual_norm_parts(long rows, long per_sample, int C, int dtype, int gate_kind, long* splits) {
+  if (rows <= 0 || per_sample <= 0 || C <= 0) throw std::invalid_argument("residual_norm: empty shape");
+  const Units u = units_of(rows, per_sample, C, dtype, gate_kind);
+  *splits = u.splits;
+  return u.blocks;
+}
+
+void residual_norm_bwd_launch(const ResidualNormBwd& p, int dtype, hipStream_t s) {
+  if (p.rows <= 0) return;
+  if (p.rows >= (1l << 31)) throw std::invalid_argument("residual_norm: at most 2^31 - 1 rows");
+  const int vecn = dtype == kF32 ? 4 : 8;
+  if (p.C <= 0 || (p.C + vecn - 1) / vecn > kResidualNormMaxChunks)
+    throw std::invalid_argument("residual_norm: C must be 1 .. 2048 16-byte chunks");
+  const Plan pl = plan(p.C, vecn);
+  const Units u = units_of(p.rows, p.per_sample, p.C, dtype, p.gate_kind);
+  auto off16 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0; };
+  const bool vec = p.C % vecn == 0 && !(off16(p.ds) || off16(p.dh) || off16(p.x) || off16(p.y) || off16(p.dx) || off16(p.dy) ||
+                                        off16(p.post_w) || off16(p.post_b) || off16(p.pre_w) || off16(p.gate));
+  const bool plain = p.post == kNormNone && p.gate_kind == kGateNone && p.scale == nullptr;
+  const int mode = plain ? kPreOnly : (p.pre == kNormNone && p.gate_kind == kGateNone && p.post != kNormNone ? kPostOnly : kAll);
+  if (plain && p.dy != nullptr) throw std::invalid_argument("residual_norm: without a branch of its own dy is dx");
+  DPA_DISPATCH_DTYPE(dtype, {
+    if (!pl.wide && pl.maxch == 1) launch<T, 1, false>(p, pl, u, vec, mode, s);
+    else if (!pl.wide) launch<T, 2, false>(p, pl, u, vec, mode, s);
+    else if (pl.maxch == 1) launch<T, 1, true>(p, pl, u, vec, mode, s);
+    else if (pl.maxch == 2) launch<T, 2, true>(p, pl, u, vec, mode, s);
+    else if (pl.maxch == 4) launch<T, 4, true>(p, pl, u, vec, mode, s);
+    else launch<T, 8, true>(p, pl, u, vec, mode, s);
+  });
+  DPA_CHECK_HIP(hipGetLastError());
+  FoldArgs f{};
+  f.partial = p.partial;
+  f.nparts = u.blocks;
+  f.part_stride = 5l * p.C;
+  f.C = p.C;
+  bool any = false;
+  for (int v = 0; v < 5; ++v) {
+    f.out[v] = p.out[v];
+    f.beta[v] = p.beta[v];
+    any = any || p.out[v] != nullptr;
+  }
+  if (any) {
+    hipLaunchKernelGGL(residual_norm_fold_kernel, dim3((unsigned)((p.C + 15) / 16), 5), dim3(256), 0, s, f);
+    DPA_CHECK_HIP(hipGetLastError());
+  }
+  if (p.gate_kind == kGateSample && p.dgate_sample != nullptr) {
+    const long total = p.rows / p.per_sample * p.C;
+    hipLaunchKernelGGL(residual_norm_fold_gate_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, p.gate_partial,
+                       u.splits, total, p.C, p.dgate_sample);
+    DPA_CHECK_HIP(hipGetLastError());
+  }
+}
+
+}  // namespace dpa

@@ -10,7 +10,9 @@ scripts: what cuDNN / cuBLAS / ATen / Apex ran fo
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence, Tuple
+import functools
+import math
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as TF
@@ -26,6 +28,12 @@ def _hip():
     from . import hip_ops
 
     return hip_ops
+
+
+def _tops():
+    from . import transformer_ops
+
+    return transformer_ops
 
 
 def _pair(v) -> Tuple[int, int]:
@@ -319,6 +327,154 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: f
     return TF.layer_norm(x.float(), (x.shape[-1],), weight.float(), bias.float(), eps).to(x.dtype)
 
 
+class Norm(NamedTuple):
+    """A norm over the last axis as ``residual_norm`` takes it: ``kind`` "layer" (``weight``, ``bias`` or None) or "rms"
+    (``weight``).  ``nn.LayerNorm`` and ``nn.RMSNorm`` modules give theirs with ``.spec()``."""
+    weight: torch.Tensor
+    bias: Optional[torch.Tensor] = None
+    eps: float = 1e-5
+    kind: str = "layer"
+
+
+def _check_norm(name: str, norm: Norm, x: torch.Tensor) -> None:
+    C = x.shape[-1]
+    if norm.kind not in ("layer", "rms"):
+        raise ValueError("%s: unknown kind %r" % (name, norm.kind))
+    if norm.weight.shape != (C,) or (norm.bias is not None and norm.bias.shape != (C,)):
+        raise ValueError("%s: weight / bias must be [C]" % name)
+    if norm.kind == "rms" and norm.bias is not None:
+        raise ValueError("%s: an RMSNorm has no bias" % name)
+    if not norm.eps >= 0.0:
+        raise ValueError("%s: eps must not be negative" % name)
+    if any(t is not None and t.device != x.device for t in norm[:2]):
+        raise ValueError("%s: weight / bias must be on the input's device" % name)
+
+
+_NORM_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _check_rows(name: str, x: torch.Tensor) -> None:
+    if x.dtype not in _NORM_DTYPES:
+        raise TypeError("%s: float32, bfloat16 or float16 expected, got %s" % (name, x.dtype))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("%s: rows of at least one channel expected" % name)
+    most = 2048 * 16 // x.element_size()
+    if x.shape[-1] > most:
+        raise ValueError("%s: at most %d channels in %s" % (name, most, x.dtype))
+
+
+def _norm_reference(v: torch.Tensor, norm: Norm) -> torch.Tensor:
+    if norm.kind == "layer":
+        return TF.layer_norm(v, (v.shape[-1],), norm.weight.float(), None if norm.bias is None else norm.bias.float(), norm.eps)
+    return v * torch.rsqrt(v.square().mean(-1, keepdim=True) + norm.eps) * norm.weight.float()
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post: Optional[Norm] = None, gate: Optional[torch.Tensor] = None,
+                  scale: Optional[torch.Tensor] = None, pre: Optional[Norm] = None):
+    """The residual sum of a transformer block with the norms around it:
+
+        ``s = x + scale[n] * gate * post(y)``,   ``h = pre(s)``
+
+    ``x`` (the residual stream) and ``y`` (the block's output) are ``[N, ..., C]`` of one shape and type.  ``post``: the
+    norm behind the block (Swin V2), ``pre``: the norm in front of the next one (ViT, Swin); each a ``Norm`` or None.
+    ``gate``: learnable, ``[C]`` (layer scale) or ``[N, C]`` (a conditioned block).  ``scale``: ``[N]``, a constant for
+    each sample (stochastic depth: 0 or 1 / keep; a dropped sample's branch still has to be finite).  Returns ``s``, or
+    ``(s, h)`` with ``pre``.  Everything between the inputs and the results is 32-bit arithmetic, rounded once: ``h`` is
+    the norm of the unrounded sum.  On the GPU one pass per direction (``csrc/kernels/residual_norm*.hip``), any ``C`` up
+    to 16384 (16-bit types; 8192 in float32)."""
+    _check_rows("residual_norm", x)
+    if x.dim() < 2 or y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
+        raise ValueError("residual_norm: x and y must be [N, ..., C] of the same shape, dtype and device")
+    if post is not None:
+        _check_norm("residual_norm: post", post, x)
+    if pre is not None:
+        _check_norm("residual_norm: pre", pre, x)
+    N, C = x.shape[0], x.shape[-1]
+    if gate is not None and (tuple(gate.shape) not in ((C,), (N, C)) or gate.device != x.device):
+        raise ValueError("residual_norm: gate must be [C] or [N, C] on the input's device")
+    if scale is not None:
+        if tuple(scale.shape) != (N,) or scale.device != x.device:
+            raise ValueError("residual_norm: scale must be [N] on the input's device")
+        if scale.requires_grad:
+            raise ValueError("residual_norm: scale is a constant (use a gate for a learnable factor)")
+    if _on_gpu(x):
+        return _tops().residual_norm(x, y, post, gate, scale, pre)
+    z = y.float()
+    if post is not None:
+        z = _norm_reference(z, post)
+    if gate is not None:
+        z = z * (gate.float() if gate.dim() == 1 else gate.float().reshape((N,) + (1,) * (x.dim() - 2) + (C,)))
+    if scale is not None:
+        z = z * scale.float().reshape((N,) + (1,) * (x.dim() - 1))
+    s = x.float() + z
+    if pre is None:
+        return s.to(x.dtype)
+    return s.to(x.dtype), _norm_reference(s, pre).to(x.dtype)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    """RMSNorm over the last axis: ``x / sqrt(mean(x^2) + eps) * weight``."""
+    _check_rows("rms_norm", x)
+    norm = Norm(weight, None, eps, "rms")
+    _check_norm("rms_norm", norm, x)
+    if _on_gpu(x):
+        return _tops().rms_norm(x, weight, eps)
+    return _norm_reference(x.float(), norm).to(x.dtype)
+
+
+def rotary(qkv: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axis: torch.Tensor, num_heads: int, *,
+           interleaved: bool = False, inplace: bool = False) -> torch.Tensor:
+    """Rotary positions of several axes (row and column of an image patch; time, row and column of a video's) on the
+    packed projection that ``attention`` takes: ``qkv`` is ``[B, S, 3 * H * D]``, laid out ``[3][H][D]`` per token.  Pair
+    ``j`` of every query and key head is turned by the angle ``positions[..., axis[j]] * freqs[j]``; the values are
+    unchanged.  Pairs are ``(j, j + P)``, or ``(2j, 2j + 1)`` with ``interleaved``; what lies behind the ``P`` pairs of a
+    head stays as it is.  ``positions``: ``[S, A]`` or ``[B, S, A]``, whole numbers or floats; ``freqs``: ``[P]`` float32
+    or float64; ``axis``: ``[P]`` whole numbers in ``[0, A)`` (an entry outside turns its pair into NaN).  Angles are
+    formed in 64 bits.  ``inplace`` (without gradients) overwrites ``qkv``.  ``nn.AxialRotary`` holds ``freqs`` and
+    ``axis`` for the usual splits of a head."""
+    if qkv.dtype not in _NORM_DTYPES:
+        raise TypeError("rotary: float32, bfloat16 or float16 expected, got %s" % (qkv.dtype,))
+    if qkv.dim() != 3 or num_heads < 1 or qkv.shape[-1] % (3 * num_heads) or qkv.shape[-1] == 0:
+        raise ValueError("rotary: qkv must be [B, S, 3 * heads * D]")
+    B, S, D = qkv.shape[0], qkv.shape[1], qkv.shape[-1] // (3 * num_heads)
+    if positions.dim() not in (2, 3) or tuple(positions.shape[:-1]) != ((S,) if positions.dim() == 2 else (B, S)) \
+            or positions.shape[-1] < 1:
+        raise ValueError("rotary: positions must be [S, A] or [B, S, A]")
+    if positions.dtype not in (torch.int64, torch.int32, torch.float32, torch.float64):
+        raise TypeError("rotary: positions must be int64, int32, float32 or float64, got %s" % (positions.dtype,))
+    if freqs.dtype not in (torch.float32, torch.float64):
+        raise TypeError("rotary: freqs must be float32 or float64, got %s" % (freqs.dtype,))
+    if axis.dtype not in (torch.int32, torch.int64):
+        raise TypeError("rotary: axis must be int32 or int64, got %s" % (axis.dtype,))
+    if freqs.dim() != 1 or axis.shape != freqs.shape or 2 * freqs.numel() > D or freqs.numel() > 4096:
+        raise ValueError("rotary: freqs and axis must be [P] with 2 P <= D (and P <= 4096)")
+    if any(t.device != qkv.device for t in (positions, freqs, axis)):
+        raise ValueError("rotary: positions, freqs and axis must be on the input's device")
+    if positions.requires_grad or freqs.requires_grad:
+        raise ValueError("rotary: positions and freqs are constants")
+    if inplace:
+        if torch.is_grad_enabled() and qkv.requires_grad:
+            raise ValueError("rotary: inplace is for calls without gradients")
+        if qkv.stride(-1) != 1 or (B > 1 and S > 0 and abs(qkv.stride(0)) < qkv.shape[-1]) \
+                or (S > 1 and abs(qkv.stride(1)) < qkv.shape[-1]):
+            raise ValueError("rotary: inplace needs tokens that are dense and do not overlap")
+    if _on_gpu(qkv):
+        return _tops().rotary(qkv, positions, freqs, axis, num_heads, interleaved, inplace)
+    P = freqs.numel()
+    ok = (axis >= 0) & (axis < positions.shape[-1])
+    angle = positions.double()[..., axis.long().clamp(0, positions.shape[-1] - 1)] * freqs.double()
+    angle = torch.where(ok, angle, math.nan)
+    angle = angle.reshape((B if positions.dim() == 3 else 1, S, 1, 1, P))
+    cos, sin = angle.cos().float(), angle.sin().float()
+    v = qkv.reshape(B, S, 3, num_heads, D)
+    qk = v[:, :, :2].float()
+    a, b = (qk[..., 0:2 * P:2], qk[..., 1:2 * P:2]) if interleaved else (qk[..., :P], qk[..., P:2 * P])
+    first, second = a * cos - b * sin, a * sin + b * cos
+    turned = torch.stack([first, second], -1).flatten(-2) if interleaved else torch.cat([first, second], -1)
+    out = torch.cat([torch.cat([turned, qk[..., 2 * P:]], -1).to(qkv.dtype), v[:, :, 2:]], 2).reshape(qkv.shape)
+    return qkv.copy_(out) if inplace else out
+
+
 def se_scale(x: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
     """``x[n, h, w, c] * s[n, c]``: the squeeze-excitation gate.  ``s`` is fp32 ``[N, C]``."""
     if _on_gpu(x):
@@ -406,6 +562,91 @@ def loss_and_metrics(logits: torch.Tensor, target: torch.Tensor):
         rec = torch.stack([loss.detach().float() * n, c[0], c[1],
                            torch.tensor(n, device=logits.device)])
     return loss, rec
+
+
+def token_logprobs(logits: torch.Tensor, target: torch.Tensor, k: int = 0):
+    """-> ``(logprob, entropy, top_logprob, top_index)`` of every row of ``logits`` ``[..., V]``: the log probability of
+    ``target`` ``[...]`` under the row's softmax, the entropy of that softmax, and its ``k`` most probable classes
+    ``[..., k]`` in descending order (``k <= 64``; ties go to the lowest index).  float32 (indices int64) whatever the
+    logits' type; the first three carry gradients.
+
+    A logit of -inf (a masked class) has probability zero and adds nothing.  A row that is masked altogether has entropy
+    0, log probabilities -inf and no gradient.  A ``target`` outside ``[0, V)`` is ignored: its log probability is 0 and
+    carries no gradient, the row's other results are as usual.  A row with a NaN or a +inf gives NaN."""
+    if logits.dtype not in _NORM_DTYPES:
+        raise TypeError("token_logprobs: float32, bfloat16 or float16 expected, got %s" % (logits.dtype,))
+    if logits.dim() < 1 or logits.shape[-1] < 1 or logits.shape[:-1] != target.shape:
+        raise ValueError("token_logprobs: logits [..., V] and target [...] expected")
+    if target.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
+        raise TypeError("token_logprobs: target must hold whole numbers, got %s" % (target.dtype,))
+    if target.device != logits.device:
+        raise ValueError("token_logprobs: target must be on the logits' device")
+    V = logits.shape[-1]
+    if not 0 <= k <= min(64, V):
+        raise ValueError("token_logprobs: k must be 0 .. min(64, V), got %r" % (k,))
+    lead = target.shape
+    z, t = logits.reshape(-1, V) if logits.dim() != 2 else logits, target.reshape(-1)
+    if _on_gpu(z):
+        lp, ent, top, idx = _tops().token_logprobs(z, t, int(k))
+    else:
+        zf, t = z.float(), t.long()
+        empty = (zf == -math.inf).all(1)
+        zs = torch.where(empty[:, None], 0.0, zf)                 # such a row is answered apart, without a gradient
+        m = zs.detach().amax(1, keepdim=True)
+        logp = (zs - m) - (zs - m).exp().sum(1, keepdim=True).log()
+        valid = (t >= 0) & (t < V)
+        lp = torch.where(valid, logp.gather(1, t.clamp(0, V - 1)[:, None])[:, 0], 0.0)
+        lp = torch.where(empty & valid, -math.inf, lp)
+        ent = -(logp.exp() * torch.where(logp == -math.inf, 0.0, logp)).sum(1)
+        ent = torch.where(empty, 0.0, ent)
+        idx = torch.sort(zf.detach(), dim=1, descending=True, stable=True).indices[:, :k]
+        top = torch.where(empty[:, None], -math.inf, logp.gather(1, idx))
+    return lp.reshape(lead), ent.reshape(lead), top.reshape(lead + (k,)), idx.reshape(lead + (k,))
+
+
+def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7) -> torch.Tensor:
+    """Orthogonalises the last two axes of ``g`` (``[..., m, n]``) approximately, as ``optim.FusedMuon`` does with its
+    updates: ``X = g / (|g|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` (on the
+    transposed matrix where ``m > n``).  With the default ``coefficients`` ``(a, b, c)`` five steps move the singular
+    values into about [0.7, 1.2].  Products have about 22 significant bits and are summed in 32; the result has ``g``'s
+    type.  No gradient.  A matrix with an infinity or a NaN gives NaN.
+
+    The GPU holds matrices as fp16 pairs, so the singular values may not grow: coefficients that move any value of
+    [0, 1] beyond 4 within ``steps`` steps are refused."""
+    if g.dtype not in _NORM_DTYPES:
+        raise TypeError("newton_schulz: float32, bfloat16 or float16 expected, got %s" % (g.dtype,))
+    if g.dim() < 2 or g.numel() == 0:
+        raise ValueError("newton_schulz: matrices [..., m, n] expected")
+    if steps < 1 or not eps > 0.0:
+        raise ValueError("newton_schulz: steps must be at least 1 and eps positive")
+    _check_schulz(tuple(float(v) for v in coefficients), int(steps))
+    if torch.is_grad_enabled() and g.requires_grad:
+        raise ValueError("newton_schulz: has no gradient (detach the update)")
+    if _on_gpu(g):
+        return _tops().newton_schulz(g, steps, coefficients, eps)
+    a, b, c = coefficients
+    x = g.float()
+    turned = x.shape[-2] > x.shape[-1]
+    x = x / (torch.linalg.vector_norm(x.double(), dim=(-2, -1), keepdim=True) + eps).float()
+    x = x.mT if turned else x
+    for _ in range(steps):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return (x.mT if turned else x).to(g.dtype).contiguous()
+
+
+@functools.lru_cache(maxsize=64)
+def _check_schulz(coefficients, steps: int) -> None:
+    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+        raise ValueError("newton_schulz: three finite coefficients expected")
+    a, b, c = coefficients
+    v = [i / 4096.0 for i in range(4097)]
+    for _ in range(steps):          # what every singular value of [0, 1] becomes; fp16 pairs hold entries up to 63
+        if max(abs(b * x * x + c * x ** 4) for x in v) > 32.0:
+            raise ValueError("newton_schulz: coefficients %r let singular values grow" % (coefficients,))
+        v = [x * (a + b * x * x + c * x ** 4) for x in v]
+        if max(abs(x) for x in v) > 4.0:
+            raise ValueError("newton_schulz: coefficients %r let singular values grow" % (coefficients,))
 
 
 # ----------------------------------------------------------------------------- input pipeline

@@ -3220,6 +3220,8 @@ class SgdPlan:
         self.groups = []
         self.params_with_copies = []
         for group in opt.param_groups:
+            if group.get("orthogonal"):         # updated by transformer_ops.MuonPlan
+                continue
             entries, keep, plist, nchunks = [], [], [], 0
             g_dtype = lp_dtype = None
             device = None

@@ -202,3 +202,137 @@ class FusedSGD(Optimizer):
             if buf is not None and p.dim() == 4 and not buf.is_contiguous(
                     memory_format=torch.channels_last):
                 st["momentum_buffer"] = buf.contiguous(memory_format=torch.channels_last)
+
+
+def muon_groups(model) -> list:
+    """Parameter groups for ``FusedMuon``: the matrices inside the network are orthogonalised (Linear weights,
+    attention projections, dense convolution filters as ``[K, C * R * S]``); the first convolution, the classifier,
+    embeddings, depthwise filters, biases and norms take plain SGD."""
+    from .nn.modules import Conv2d, Linear
+
+    convs = [m for m in model.modules() if isinstance(m, Conv2d)]
+    linears = [m for m in model.modules() if isinstance(m, Linear)]
+    first = convs[0].weight if convs else None
+    last = linears[-1].weight if linears else (convs[-1].weight if convs else None)
+    grouped = {id(m.weight) for m in convs if m.groups > 1}
+    matrices, rest = [], []
+    for p in model.parameters():
+        if not p.requires_grad:
+            continue
+        inside = p.dim() in (2, 4) and p is not first and p is not last and id(p) not in grouped \
+            and min(p.shape[0], p.numel() // p.shape[0]) > 1
+        (matrices if inside else rest).append(p)
+    return [g for g in (dict(params=matrices, orthogonal=True), dict(params=rest, orthogonal=False)) if g["params"]]
+
+
+class FusedMuon(FusedSGD):
+    """Muon beside ``FusedSGD``: the matrices of groups with ``orthogonal=True`` are updated with the orthogonalised
+    momentum, all other parameters by SGD with momentum in the same step.
+
+        ``buf = momentum * buf + g``,  ``u = g + momentum * buf`` (nesterov) or ``buf``
+        ``p = p * (1 - lr * weight_decay) - lr * matrix_scale * sqrt(max(1, rows / columns)) * newton_schulz(u)``
+
+    ``g`` is the unscaled gradient; the decay is decoupled (it does not enter the momentum).  A group without
+    ``orthogonal`` behaves exactly like one of ``FusedSGD`` (coupled decay, no nesterov).  ``params``: groups as
+    ``muon_groups(model)`` makes them, or parameters, of which those of two dimensions are orthogonalised.
+
+    On the GPU a step is two launches over a device-resident table per group plus ``newton_schulz`` once per matrix shape
+    (matrices of one shape are a batch); loss scaling, the overflow skip, low-precision copies, gradient arenas and
+    hipGraph capture work as in ``FusedSGD``.  ``state_dict`` holds ``momentum_buffer`` per parameter."""
+
+    def __init__(self, params, lr: float = 0.1, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True,
+                 matrix_scale: float = 0.2, ns_steps: int = 5, ns_coefficients=(3.4445, -4.7750, 2.0315),
+                 ns_eps: float = 1e-7):
+        from .ops.functional import _check_schulz
+
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("Invalid momentum: {}".format(momentum))
+        if weight_decay < 0.0 or matrix_scale <= 0.0:
+            raise ValueError("weight_decay must not be negative and matrix_scale positive")
+        if ns_steps < 1 or not ns_eps > 0.0:
+            raise ValueError("ns_steps must be at least 1 and ns_eps positive")
+        _check_schulz(tuple(float(v) for v in ns_coefficients), int(ns_steps))
+        groups = list(params)
+        if groups and not isinstance(groups[0], dict):
+            groups = [g for g in (dict(params=[p for p in groups if p.dim() == 2], orthogonal=True),
+                                  dict(params=[p for p in groups if p.dim() != 2], orthogonal=False)) if g["params"]]
+        super().__init__(groups, lr=lr, momentum=momentum, weight_decay=weight_decay)
+        self._matrix_defaults = dict(orthogonal=False, matrix_scale=float(matrix_scale), ns_steps=int(ns_steps),
+                                     ns_coefficients=tuple(float(v) for v in ns_coefficients), ns_eps=float(ns_eps))
+        self._nesterov = bool(nesterov)
+        self._muon = None
+        self._fill_groups()
+
+    def _fill_groups(self) -> None:
+        for group in self.param_groups:
+            for k, v in self._matrix_defaults.items():
+                group.setdefault(k, v)
+            if group["orthogonal"]:
+                group["nesterov"] = self._nesterov
+                for p in group["params"]:
+                    if p.dim() < 2:
+                        raise ValueError("FusedMuon: an orthogonal group holds matrices (2 or more dimensions)")
+
+    def add_param_group(self, group) -> None:
+        super().add_param_group(group)
+        if hasattr(self, "_matrix_defaults"):        # (the base constructor adds its groups through here)
+            self._fill_groups()
+            self._plan = self._muon = None
+
+    def _step_reference(self, scaler) -> None:
+        from .ops import functional as F
+
+        if scaler is not None and float(scaler.found_inf.item()) > 0:
+            return
+        plain, mine = [], []
+        for g in self.param_groups:
+            (mine if g["orthogonal"] else plain).append(g)
+        every, self.param_groups = self.param_groups, plain
+        try:
+            super()._step_reference(scaler)
+        finally:
+            self.param_groups = every
+        inv = None if scaler is None else scaler.inv_scale
+        for group in mine:
+            lr, mu = group["lr"], group["momentum"]
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                g = p.grad.to(p.dtype)
+                if inv is not None:
+                    g = g * inv.to(g.dtype).squeeze(0)
+                buf = self._momentum_buffer(p)
+                buf.mul_(mu).add_(g)
+                u = g.add(buf, alpha=mu) if group["nesterov"] else buf
+                rows, cols = p.shape[0], p.numel() // p.shape[0]
+                o = F.newton_schulz(u.reshape(rows, cols), group["ns_steps"], group["ns_coefficients"], group["ns_eps"])
+                p.mul_(1.0 - lr * group["weight_decay"])
+                p.add_(o.reshape(p.shape), alpha=-lr * group["matrix_scale"] * max(1.0, rows / cols) ** 0.5)
+
+    def _step_hip(self, scaler) -> None:
+        from .ops.transformer_ops import MuonPlan
+
+        if self._muon is None or not self._muon.matches(self):
+            self._muon = MuonPlan(self)
+        self._muon.launch(self, scaler)
+        super()._step_hip(scaler)                    # the other groups; then every derived copy is stale ...
+        self._muon.stamp_copies()                    # ... but those that this step wrote
+        _amp.mark_copies_written([p for gt in self._muon.groups for p, lp in gt["plist"] if lp is not None])
+
+    def set_amp(self, amp_state) -> None:
+        super().set_amp(amp_state)
+        self._muon = None
+
+    def rebind(self) -> None:
+        super().rebind()
+        self._muon = None
+
+    def sync_hyper(self) -> None:
+        super().sync_hyper()
+        if self._muon is not None:
+            self._muon.sync_hyper(self)
+
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict(state_dict)
+        self._muon = None
+        self._fill_groups()
