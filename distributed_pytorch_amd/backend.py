@@ -46,6 +46,17 @@ def require():
     return ext
 
 
+def require_transformer():
+    """The module ``_T`` (transformer-block operators, ``csrc/transformer``)."""
+    require()
+    try:
+        return importlib.import_module("distributed_pytorch_amd._T")
+    except ImportError as exc:
+        raise RuntimeError(
+            "distributed_pytorch_amd._T is not built/loadable (%r). Run `python -m distributed_pytorch_amd.build`. "
+            "GPU tensors never fall back to PyTorch ops." % (exc,))
+
+
 def stream_handle() -> int:
     """Raw ``hipStream_t`` of torch's current stream, as an integer."""
     return torch.cuda.current_stream().cuda_stream

@@ -1,8 +1,9 @@
-"""In-tree build of the native extension ``distributed_pytorch_amd/_C*.so``.
+"""In-tree build of the native extensions ``distributed_pytorch_amd/_C*.so`` and ``_T*.so``.
 
-``python -m distributed_pytorch_amd.build`` compiles every ``csrc/kernels/*.hip`` for gfx950 with
-hipcc (cross-compiles without a GPU), the C++ runtime / binding, and links one pybind11 module that
-sits next to the package so it travels to the GPU box with the tree.  Objects are cached under
+``python -m distributed_pytorch_amd.build`` compiles every ``csrc/**/*.hip`` for gfx950 with
+hipcc (cross-compiles without a GPU), the C++ runtime / bindings, and links two pybind11 modules that
+sit next to the package so they travel to the GPU box with the tree: ``_C``, and ``_T`` (``csrc/transformer``:
+operators with autograd nodes in C++, the only part built against torch's headers).  Objects are cached under
 ``build/`` and rebuilt only when a source (or a header that it includes) is newer.
 """
 from __future__ import annotations
@@ -25,11 +26,12 @@ NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
-    out = []
+    """{module: sources}: ``_C`` (no torch headers) and ``_T`` (``csrc/transformer``, built against torch's)."""
+    out = {"_C": [], "_T": []}
     for root, _, files in os.walk(CSRC):
         for f in sorted(files):
             if f.endswith((".hip", ".cpp")):
-                out.append(os.path.join(root, f))
+                out["_T" if os.path.basename(root) == "transformer" else "_C"].append(os.path.join(root, f))
     return out
 
 
@@ -48,8 +50,18 @@ def _mtime_with_headers(path: str, seen=None) -> float:
     return newest
 
 
-def target_path() -> str:
-    return os.path.join(HERE, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
+def target_path(module: str = "_C") -> str:
+    return os.path.join(HERE, module + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _torch_flags():
+    """(compiler flags, linker flags) of a host source that includes torch's headers."""
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    inc = ["-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include")]
+    libs = ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
+    return ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"] + inc, libs
 
 
 def build(verbose: bool = False, force: bool = False, jobs: int = 0) -> str:
@@ -61,16 +73,20 @@ def build(verbose: bool = False, force: bool = False, jobs: int = 0) -> str:
            "-I" + os.path.join(ROCM, "include")]
     common = [HIPCC, "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
               "-Wno-unused-result"] + NO_PACKED_FP32 + inc + os.environ.get("DPA_BUILD_DEFS", "").split()
-    todo, objs = [], []
-    for src in _sources():
-        obj = os.path.join(objdir, os.path.relpath(src, CSRC).replace(os.sep, "_") + ".o")
-        objs.append(obj)
-        if force or not os.path.exists(obj) or os.path.getmtime(obj) < _mtime_with_headers(src):
-            todo.append((src, obj))
+    torch_cc, torch_ld = _torch_flags()
+    host = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden"] + torch_cc + inc[1:]
+    todo, objs = [], {}
+    for module, sources in _sources().items():
+        objs[module] = []
+        for src in sources:
+            obj = os.path.join(objdir, os.path.relpath(src, CSRC).replace(os.sep, "_") + ".o")
+            objs[module].append(obj)
+            if force or not os.path.exists(obj) or os.path.getmtime(obj) < _mtime_with_headers(src):
+                todo.append((module, src, obj))
 
     def compile_one(job):
-        src, obj = job
-        cmd = common + ["-c", src, "-o", obj]
+        module, src, obj = job
+        cmd = (host if module == "_T" and src.endswith(".cpp") else common) + ["-c", src, "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -82,16 +98,18 @@ def build(verbose: bool = False, force: bool = False, jobs: int = 0) -> str:
     if todo:
         with ThreadPoolExecutor(max_workers=jobs) as ex:
             list(ex.map(compile_one, todo))
-    tgt = target_path()
-    if todo or not os.path.exists(tgt):
-        # no rpath: at run time libamdhip64.so.7 resolves to the copy torch loaded first
-        cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", tgt] + objs + ["-ldl"]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed:\n%s" % r.stderr[-4000:])
-    return tgt
+    changed = {module for module, _, _ in todo}
+    for module, files in objs.items():
+        tgt = target_path(module)
+        if module in changed or not os.path.exists(tgt):
+            # no rpath: at run time libamdhip64.so.7 (and torch's libraries) resolve to the copies torch loaded first
+            cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", tgt] + files + ["-ldl"] + (torch_ld if module == "_T" else [])
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError("link failed:\n%s" % r.stderr[-4000:])
+    return target_path()
 
 
 if __name__ == "__main__":

@@ -10,10 +10,6 @@
 namespace py = pybind11;
 using namespace dpa;
 
-namespace dpa {
-void bind_transformer(py::module_& m);      // bind_transformer.cpp
-}
-
 namespace {
 template <typename T> T* ptr(uintptr_t p) { return reinterpret_cast<T*>(p); }
 hipStream_t st(uintptr_t s) { return reinterpret_cast<hipStream_t>(s); }
@@ -26,8 +22,6 @@ PYBIND11_MODULE(_C, m) {
   m.attr("F16") = (int)kF16;
   m.attr("IGEMM_RELU") = (int)kIgemmRelu;
   m.attr("IGEMM_SCATTER") = (int)kIgemmScatter;
-
-  bind_transformer(m);
 
   m.def("igemm",
         [](uintptr_t A, uintptr_t B, uintptr_t C, uintptr_t R, uintptr_t bias, uintptr_t stats, uintptr_t taps, int M,

@@ -6,9 +6,9 @@
 #include <stdexcept>
 #include <string>
 
-namespace dpa {
+#include "dtype.h"
 
-enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+namespace dpa {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;

@@ -1,0 +1,435 @@
+// The transformer-block operators as torch sees them: allocation, launch and autograd nodes in C++.
+//
+// A training step of a small batch is bound by the host: as Python autograd functions a forward and backward call of one
+// of these operators took 120 - 200 us of host time around 25 - 60 us of kernels.  So this module, unlike _C, is built
+// against torch's headers.  Arguments are checked in ops/functional.py.
+//
+// Outputs and workspaces come from torch's allocator per call and launches go to torch's current stream of the tensors'
+// device: nothing is shared between two calls or two graphs, and nothing synchronises with the host.
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <ATen/ops/zeros_like.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include "transformer.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+namespace dpa {
+namespace {
+
+int code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return kF32;
+    case at::kBFloat16: return kBF16;
+    case at::kHalf: return kF16;
+    default: TORCH_CHECK_TYPE(false, "unsupported dtype ", t.scalar_type(), " for HIP kernels");
+  }
+}
+hipStream_t stream_of(const Tensor& t) {
+  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
+}
+Tensor given(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+template <typename T> T* data(const Tensor& t) { return t.defined() ? reinterpret_cast<T*>(t.data_ptr()) : nullptr; }
+// a parameter vector as the kernels read it
+Tensor vec32(const Tensor& t) {
+  if (!t.defined()) return t;
+  return (t.scalar_type() == at::kFloat ? t.detach() : t.detach().to(at::kFloat)).contiguous();
+}
+Tensor floats(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options().dtype(at::kFloat)); }
+bool tracked(std::initializer_list<Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+// ------------------------------------------------------------------------------------------ residual norm
+struct NormCfg {
+  int64_t post, pre;                     // NormKind
+  double post_eps, pre_eps;
+  bool sinks;                            // parameters may have gradient sinks (ops/grad_sink.py)
+};
+struct RowShape {
+  long rows, per_sample;
+  int C;
+};
+RowShape row_shape(const Tensor& x) {
+  RowShape r;
+  r.C = (int)x.size(-1);
+  r.rows = x.numel() / r.C;
+  r.per_sample = x.size(0) > 0 && r.rows > 0 ? r.rows / x.size(0) : 1;
+  return r;
+}
+// fp32 copies of post_w, post_b, pre_w, pre_b, gate, scale
+using Vecs = std::array<Tensor, 6>;
+
+struct RnOut {
+  Tensor s, h, post_stat, pre_stat;
+};
+RnOut rn_forward(const Tensor& x, const Tensor& y, const Vecs& v, const NormCfg& c, bool want_stats) {
+  const c10::DeviceGuard guard(x.device());
+  const RowShape r = row_shape(x);
+  RnOut o;
+  if (y.defined()) o.s = at::empty_like(x);
+  if (c.pre != kNormNone) o.h = at::empty_like(x);
+  if (want_stats && c.post != kNormNone) o.post_stat = floats({2, r.rows}, x);
+  if (want_stats && c.pre != kNormNone) o.pre_stat = floats({2, r.rows}, x);
+  ResidualNormFwd p;
+  p.x = data<void>(x); p.y = data<void>(y); p.s = data<void>(o.s); p.h = data<void>(o.h);
+  p.post_w = data<float>(v[0]); p.post_b = data<float>(v[1]); p.pre_w = data<float>(v[2]); p.pre_b = data<float>(v[3]);
+  p.gate = data<float>(v[4]); p.scale = data<float>(v[5]);
+  p.post_stat = data<float>(o.post_stat); p.pre_stat = data<float>(o.pre_stat);
+  p.rows = r.rows; p.per_sample = r.per_sample; p.C = r.C;
+  p.post = (int)c.post; p.pre = (int)c.pre; p.gate_kind = v[4].defined() ? (int)v[4].dim() : kGateNone;
+  p.post_eps = (float)c.post_eps; p.pre_eps = (float)c.pre_eps;
+  residual_norm_fwd_launch(p, code(x), stream_of(x));
+  return o;
+}
+
+// A parameter's gradient sink (ops/grad_sink.py), where it has one now: the kernel writes into its view.
+struct Sink {
+  py::object sink;           // set: the kernel writes here
+  Tensor view;
+  float beta = 0.f;
+  bool late = false;         // the gradient goes through deliver() after the kernel
+};
+// needs the GIL
+void find_sink(const Tensor& param, Sink& out) {
+  if (!param.is_leaf()) return;
+  py::object p = py::reinterpret_steal<py::object>(THPVariable_Wrap(param));
+  if (!py::hasattr(p, "_dpa_sink")) return;
+  out.late = true;
+  py::object s = py::module_::import("distributed_pytorch_amd.ops.grad_sink").attr("sink_of")(p);
+  if (s.is_none()) return;
+  out.view = s.attr("view").cast<Tensor>();
+  if (!out.view.is_contiguous()) return;
+  out.beta = s.attr("beta")().cast<float>();
+  out.sink = std::move(s);
+}
+// through the framework's own delivery (accumulates into a sink, or hands the gradient to autograd); needs the GIL
+Tensor deliver(const Tensor& param, const Tensor& grad) {
+  py::object p = py::reinterpret_steal<py::object>(THPVariable_Wrap(param));
+  py::object g = py::module_::import("distributed_pytorch_amd.ops.hip_ops").attr("_deliver")(p, grad);
+  return g.is_none() ? Tensor() : g.cast<Tensor>();
+}
+
+struct ResidualNormFn : Function<ResidualNormFn> {
+  // y undefined: h = pre(x) alone
+  static variable_list forward(AutogradContext* ctx, const Tensor& x0, const OptTensor& y0, const OptTensor& post_w0,
+                               const OptTensor& post_b0, const OptTensor& pre_w0, const OptTensor& pre_b0,
+                               const OptTensor& gate0, const OptTensor& scale, const NormCfg& c) {
+    const Tensor x = x0.contiguous(), y = dense(given(y0)), post_w = given(post_w0), post_b = given(post_b0),
+                 pre_w = given(pre_w0), pre_b = given(pre_b0), gate = given(gate0);
+    const Vecs v{vec32(post_w), vec32(post_b), vec32(pre_w), vec32(pre_b), vec32(gate), vec32(given(scale))};
+    RnOut o = rn_forward(x, y, v, c, true);
+    const bool pre = c.pre != kNormNone, keep_y = pre || c.post != kNormNone || gate.defined();
+    ctx->save_for_backward({pre ? x : Tensor(), keep_y ? y : Tensor(), o.post_stat, o.pre_stat, post_w, post_b, pre_w, pre_b,
+                            gate, v[5]});
+    ctx->saved_data["cfg"] = std::vector<int64_t>{c.post, c.pre, y.defined(), c.sinks};
+    ctx->set_materialize_grads(false);
+    variable_list out;
+    if (o.s.defined()) out.push_back(o.s);
+    if (o.h.defined()) out.push_back(o.h);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const std::vector<int64_t> cfg = ctx->saved_data["cfg"].toIntVector();
+    const bool has_y = cfg[2] != 0;
+    variable_list got(9);
+    Tensor ds = has_y ? grads[0] : Tensor(), dh = has_y ? (grads.size() > 1 ? grads[1] : Tensor()) : grads[0];
+    if (!ds.defined() && !dh.defined()) return got;
+    ds = dense(ds);
+    dh = dense(dh);
+    const Tensor& ref = ds.defined() ? ds : dh;
+    const c10::DeviceGuard guard(ref.device());
+    const Tensor &x = sv[0], &y = sv[1];
+    // the caller's parameters in the order of the kernel's sums, and where their gradients go
+    const std::array<Tensor, 5> params{sv[6], sv[7], sv[4], sv[5], sv[8]};
+    constexpr int place[5] = {4, 5, 2, 3, 6};
+    const Vecs v{vec32(sv[4]), vec32(sv[5]), vec32(sv[6]), vec32(sv[7]), vec32(sv[8]), sv[9]};
+    const RowShape r = row_shape(ref);
+    const int gate_kind = v[4].defined() ? (int)v[4].dim() : kGateNone;
+    // autograd counts the arguments that were given
+    const bool here[7] = {true, has_y, sv[4].defined(), sv[5].defined(), sv[6].defined(), sv[7].defined(), sv[8].defined()};
+    bool needs[7];
+    for (int i = 0, edge = 0; i < 7; ++i) needs[i] = here[i] && ctx->needs_input_grad(edge++);
+    const bool need_x = needs[0], need_y = needs[1];
+    bool need[5], any_leaf = false;
+    for (int i = 0; i < 5; ++i) {
+      need[i] = needs[place[i]];
+      any_leaf = any_leaf || (cfg[3] != 0 && need[i] && params[i].is_leaf());
+    }
+    // without a norm, gate or scale of its own the block's gradient is that of the sum
+    const bool plain = cfg[0] == kNormNone && gate_kind == kGateNone && !v[5].defined();
+    const bool branch = !plain && (need_y || need[2] || need[3] || need[4]);
+    Tensor dx, dy;
+    if (need_x || (need_y && plain)) dx = at::empty_like(ref);
+    if (branch) dy = at::empty_like(ref);
+
+    ResidualNormBwd p;
+    Tensor own[5];
+    std::array<Sink, 5> sinks;
+    if (any_leaf) {
+      const py::gil_scoped_acquire gil;
+      for (int i = 0; i < 5; ++i) {
+        if (!need[i] || (i == 4 && gate_kind == kGateSample)) continue;
+        find_sink(params[i], sinks[i]);
+        for (int j = 0; j < i; ++j)             // a parameter used twice in this call: its second sum has a buffer of its own
+          if (sinks[j].sink && sinks[i].sink && sinks[j].sink.is(sinks[i].sink)) sinks[i].sink = py::object();
+      }
+    }
+    bool sums = false;
+    for (int i = 0; i < 5; ++i) {
+      if (!need[i] || (i == 4 && gate_kind == kGateSample)) continue;
+      sums = true;
+      if (sinks[i].sink) {
+        p.out[i] = sinks[i].view.data_ptr<float>();
+        p.beta[i] = sinks[i].beta;
+      } else {
+        own[i] = floats({r.C}, ref);
+        p.out[i] = own[i].data_ptr<float>();
+      }
+    }
+    Tensor partial, gate_partial, dgate;
+    const bool gate_sums = gate_kind == kGateSample && need[4];
+    if (gate_sums) dgate = floats({ref.size(0), r.C}, ref);
+    if (r.rows > 0) {
+      long splits = 1;
+      const long parts = residual_norm_parts(r.rows, r.per_sample, r.C, code(ref), gate_kind, &splits);
+      if (sums) partial = floats({parts, 5, r.C}, ref);
+      if (gate_sums) gate_partial = floats({ref.size(0) * splits, r.C}, ref);
+      p.ds = data<void>(ds); p.dh = data<void>(dh); p.x = data<void>(x); p.y = data<void>(y);
+      p.dx = data<void>(dx); p.dy = data<void>(dy);
+      p.post_w = data<float>(v[0]); p.post_b = data<float>(v[1]); p.pre_w = data<float>(v[2]);
+      p.gate = data<float>(v[4]); p.scale = data<float>(v[5]);
+      p.post_stat = data<float>(sv[2]); p.pre_stat = data<float>(sv[3]);
+      p.partial = data<float>(partial); p.gate_partial = data<float>(gate_partial); p.dgate_sample = data<float>(dgate);
+      p.rows = r.rows; p.per_sample = r.per_sample; p.C = r.C;
+      p.post = (int)cfg[0]; p.pre = (int)cfg[1]; p.gate_kind = gate_kind;
+      residual_norm_bwd_launch(p, code(ref), stream_of(ref));
+    } else {                                    // no rows: every sum is zero
+      for (int i = 0; i < 5; ++i) {
+        if (own[i].defined()) own[i].zero_();
+        if (sinks[i].sink && sinks[i].beta == 0.f) sinks[i].view.zero_();
+      }
+      if (dgate.defined()) dgate.zero_();
+    }
+    if (need_x) got[0] = dx;
+    if (need_y) got[1] = plain ? dx : dy;
+    for (int i = 0; i < 5; ++i) {
+      if (!need[i] || sinks[i].sink) continue;
+      const Tensor g = i == 4 && gate_kind == kGateSample ? dgate : own[i];
+      got[place[i]] = g.scalar_type() == params[i].scalar_type() ? g : g.to(params[i].scalar_type());
+    }
+    if (any_leaf) {
+      const py::gil_scoped_acquire gil;
+      for (Sink& s : sinks)
+        if (s.sink) {
+          s.sink.attr("delivered")();
+          s.sink = py::object();                // (dropped under the GIL)
+        }
+      for (int i = 0; i < 5; ++i)
+        if (sinks[i].late && got[place[i]].defined()) got[place[i]] = deliver(params[i], got[place[i]]);
+    }
+    return got;
+  }
+};
+
+// -> (s, h), None where there is none
+std::pair<OptTensor, OptTensor> residual_norm(const Tensor& x, const OptTensor& y, const OptTensor& post_w,
+                                              const OptTensor& post_b, int64_t post, double post_eps, const OptTensor& pre_w,
+                                              const OptTensor& pre_b, int64_t pre, double pre_eps, const OptTensor& gate,
+                                              const OptTensor& scale, bool sinks) {
+  const Tensor Y = given(y), pw = given(post_w), pb = given(post_b), qw = given(pre_w), qb = given(pre_b), g = given(gate),
+               sc = given(scale);
+  const NormCfg c{post, pre, post_eps, pre_eps, sinks};
+  const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+  if (!tracked({x, Y, pw, pb, qw, qb, g})) {
+    const RnOut o = rn_forward(x.contiguous(), dense(Y), {vec32(pw), vec32(pb), vec32(qw), vec32(qb), vec32(g), vec32(sc)}, c,
+                               false);
+    return {opt(o.s), opt(o.h)};
+  }
+  variable_list out = ResidualNormFn::apply(x, y, post_w, post_b, pre_w, pre_b, gate, scale, c);
+  if (!Y.defined()) return {OptTensor(), out[0]};
+  return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
+}
+
+// ------------------------------------------------------------------------------------------ rotary
+void rotary_run(const Tensor& src, const Tensor& out, const Tensor& pos, const Tensor& freqs, const Tensor& axis, int64_t heads,
+                bool interleaved, bool negate) {
+  const c10::DeviceGuard guard(src.device());
+  RotaryParams p;
+  p.in = src.data_ptr(); p.out = out.data_ptr(); p.pos = pos.data_ptr(); p.freq = freqs.data_ptr();
+  p.axis = axis.data_ptr<int>();
+  p.S = std::max<int64_t>(src.size(1), 1);
+  p.tokens = src.size(0) * src.size(1);
+  p.in_batch = src.stride(0); p.in_token = src.stride(1); p.out_batch = out.stride(0); p.out_token = out.stride(1);
+  p.H = (int)heads; p.D = (int)(src.size(2) / (3 * heads)); p.pairs = (int)freqs.numel(); p.axes = (int)pos.size(-1);
+  p.pos_kind = pos.scalar_type() == at::kLong ? kPosI64
+               : pos.scalar_type() == at::kInt ? kPosI32 : pos.scalar_type() == at::kFloat ? kPosF32 : kPosF64;
+  p.pos_batched = pos.dim() == 3; p.freq_f64 = freqs.scalar_type() == at::kDouble;
+  p.interleaved = interleaved; p.negate = negate;
+  rotary_launch(p, code(src), stream_of(src));
+}
+Tensor token_dense(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor rotary_new(const Tensor& t, const Tensor& pos, const Tensor& freqs, const Tensor& axis, int64_t heads, bool interleaved,
+                  bool negate) {
+  const Tensor src = token_dense(t);
+  const Tensor out = at::empty(src.sizes(), src.options());
+  rotary_run(src, out, pos, freqs, axis, heads, interleaved, negate);
+  return out;
+}
+
+struct RotaryFn : Function<RotaryFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& pos, const Tensor& freqs, const Tensor& axis,
+                        int64_t heads, bool interleaved) {
+    ctx->save_for_backward({pos, freqs, axis});
+    ctx->saved_data["heads"] = heads;
+    ctx->saved_data["interleaved"] = interleaved;
+    return rotary_new(qkv, pos, freqs, axis, heads, interleaved, false);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    variable_list got(6);
+    got[0] = rotary_new(grads[0], sv[0], sv[1], sv[2], ctx->saved_data["heads"].toInt(), ctx->saved_data["interleaved"].toBool(),
+                        true);
+    return got;
+  }
+};
+
+Tensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs, const Tensor& axis, int64_t heads,
+              bool interleaved, bool inplace) {
+  const Tensor pos = positions.contiguous(), f = freqs.contiguous(), a = axis.to(at::kInt).contiguous();
+  if (inplace) {
+    rotary_run(qkv, qkv, pos, f, a, heads, interleaved, false);
+    qkv.unsafeGetTensorImpl()->bump_version();
+    return qkv;
+  }
+  if (!tracked({qkv})) return rotary_new(qkv, pos, f, a, heads, interleaved, false);
+  return RotaryFn::apply(qkv, pos, f, a, heads, interleaved);
+}
+
+// ------------------------------------------------------------------------------------------ log probabilities
+struct LpOut {
+  Tensor lp, ent, top, idx, norm;
+};
+LpOut lp_forward(const Tensor& z, const Tensor& t, int64_t k) {
+  const c10::DeviceGuard guard(z.device());
+  const int64_t N = z.size(0), V = z.size(1);
+  LpOut o{floats({N}, z), floats({N}, z), floats({N, k}, z), at::empty({N, k}, t.options()), floats({N, 2}, z)};
+  TokenLogprobs p;
+  p.logits = z.data_ptr(); p.target = t.data_ptr<int64_t>();
+  p.N = N; p.C = V; p.ld = z.stride(0); p.k = (int)k;
+  p.splits = token_logprobs_splits(N, V, code(z));
+  Tensor stat, keys;
+  if (p.splits > 1) {
+    stat = floats({N, p.splits, 3}, z);
+    keys = at::empty({N, p.splits, k}, t.options());
+  }
+  p.logprob = o.lp.data_ptr<float>(); p.entropy = o.ent.data_ptr<float>(); p.norm = o.norm.data_ptr<float>();
+  p.top = o.top.data_ptr<float>(); p.index = o.idx.data_ptr<int64_t>();
+  p.stat = data<float>(stat); p.keys = data<uint64_t>(keys);
+  token_logprobs_launch(p, code(z), stream_of(z));
+  return o;
+}
+
+struct TokenLogprobsFn : Function<TokenLogprobsFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& target, int64_t k) {
+    const Tensor z = logits.stride(1) == 1 ? logits : logits.contiguous();
+    LpOut o = lp_forward(z, target, k);
+    ctx->save_for_backward({z, target, o.norm, o.ent, o.idx});
+    ctx->saved_data["k"] = k;
+    ctx->mark_non_differentiable({o.idx});
+    ctx->set_materialize_grads(false);
+    return {o.lp, o.ent, o.top, o.idx};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list got(3);
+    Tensor g[3];
+    bool any = false;
+    for (int i = 0; i < 3; ++i) {
+      if (grads[i].defined()) g[i] = vec32(grads[i]);
+      any = any || g[i].defined();
+    }
+    if (!any) return got;
+    const variable_list sv = ctx->get_saved_variables();
+    const Tensor& z = sv[0];
+    const c10::DeviceGuard guard(z.device());
+    const Tensor dz = at::empty(z.sizes(), z.options());
+    TokenLogprobsBwd p;
+    p.logits = z.data_ptr(); p.target = sv[1].data_ptr<int64_t>(); p.norm = sv[2].data_ptr<float>();
+    p.entropy = sv[3].data_ptr<float>(); p.index = sv[4].data_ptr<int64_t>();
+    p.d_logprob = data<float>(g[0]); p.d_entropy = data<float>(g[1]); p.d_top = data<float>(g[2]);
+    p.dlogits = dz.data_ptr();
+    p.N = z.size(0); p.C = z.size(1); p.ld = z.stride(0); p.k = (int)ctx->saved_data["k"].toInt();
+    token_logprobs_bwd_launch(p, code(z), stream_of(z));
+    got[0] = dz;
+    return got;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& target, int64_t k) {
+  const Tensor t = target.to(at::kLong).contiguous();
+  if (!tracked({logits})) {
+    const LpOut o = lp_forward(logits.stride(1) == 1 ? logits : logits.contiguous(), t, k);
+    return {o.lp, o.ent, o.top, o.idx};
+  }
+  variable_list o = TokenLogprobsFn::apply(logits, t, k);
+  return {o[0], o[1], o[2], o[3]};
+}
+
+// ------------------------------------------------------------------------------------------ Newton-Schulz and Muon
+// out may be g itself (contiguous then)
+Tensor newton_schulz(const Tensor& g0, const OptTensor& into, int64_t steps, double a, double b, double c, double eps) {
+  const Tensor g = g0.contiguous();
+  const c10::DeviceGuard guard(g.device());
+  const Tensor out = into.has_value() ? *into : at::empty_like(g);
+  NewtonSchulz p;
+  p.rows = g.size(-2); p.cols = g.size(-1); p.batch = g.numel() / (p.rows * p.cols);
+  const Tensor work = at::empty({(int64_t)newton_schulz_workspace(p.batch, p.rows, p.cols)}, g.options().dtype(at::kByte));
+  p.g = g.data_ptr(); p.out = out.data_ptr(); p.work = work.data_ptr();
+  p.steps = (int)steps; p.a = (float)a; p.b = (float)b; p.c = (float)c; p.eps = eps;
+  newton_schulz_launch(p, code(g), stream_of(g));
+  return out;
+}
+
+void muon_begin(const Tensor& table, int n, long chunks, int g_dtype, const Tensor& hyper, const OptTensor& inv_scale,
+                const OptTensor& found_inf, const Tensor& update) {
+  const c10::DeviceGuard guard(update.device());
+  muon_begin_launch(reinterpret_cast<const MuonTensor*>(table.data_ptr()), n, chunks, g_dtype, hyper.data_ptr<float>(),
+                    data<float>(given(inv_scale)), data<float>(given(found_inf)), update.data_ptr<float>(), stream_of(update));
+}
+void muon_end(const Tensor& table, int n, long chunks, int lp_dtype, const Tensor& hyper, const OptTensor& found_inf,
+              const Tensor& update) {
+  const c10::DeviceGuard guard(update.device());
+  muon_end_launch(reinterpret_cast<const MuonTensor*>(table.data_ptr()), n, chunks, lp_dtype, hyper.data_ptr<float>(),
+                  data<float>(given(found_inf)), update.data_ptr<float>(), stream_of(update));
+}
+
+}  // namespace
+}  // namespace dpa
+
+PYBIND11_MODULE(_T, m) {
+  m.doc() = "distributed_pytorch_amd transformer-block operators (gfx950 / MI355X)";
+  m.def("residual_norm", &dpa::residual_norm);
+  m.def("rotary", &dpa::rotary);
+  m.def("token_logprobs", &dpa::token_logprobs);
+  m.def("newton_schulz", &dpa::newton_schulz);
+  m.def("muon_chunk_elems", &dpa::muon_chunk_elems);
+  m.def("muon_table_entry_bytes", []() { return sizeof(dpa::MuonTensor); });
+  m.def("muon_begin", &dpa::muon_begin);
+  m.def("muon_end", &dpa::muon_end);
+}

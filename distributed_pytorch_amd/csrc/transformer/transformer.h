@@ -1,8 +1,11 @@
 // Host entry points of the transformer-block kernels: residual_norm*.hip, rotary.hip, token_logprobs.hip,
-// newton_schulz.hip.
+// newton_schulz.hip, muon.hip.
 #pragma once
-#include <hip/hip_runtime.h>
+#include <hip/hip_runtime_api.h>
+#include <stddef.h>
 #include <stdint.h>
+
+#include "../dtype.h"
 
 namespace dpa {
 

@@ -16,11 +16,16 @@ from typing import Callable, Optional
 import torch
 
 
+any_sinks = False             # set with the first sink of the process: until then nobody has to look for one
+
+
 class GradSink:
     __slots__ = ("param", "view", "index", "on_ready", "stamp", "zeroed", "arena", "uses")
 
     def __init__(self, param, view: torch.Tensor, index: int, on_ready: Optional[Callable] = None,
                  arena=None):
+        global any_sinks
+        any_sinks = True
         self.param, self.view, self.index, self.on_ready = param, view, index, on_ready
         self.arena = arena
         self.stamp = -1           # arena epoch of the last delivery ("written this iteration")
