@@ -3,14 +3,26 @@
 //
 //     A = X X^T,   B = b A + c A A,   X = a X + B X
 //
-// 32-bit products on the 16-bit matrix cores.  Every matrix is held as two fp16 planes, x * 2^10 = hi + lo with 22
-// significant bits (singular values stay below ~4, so nothing leaves the fp16 range, and the scale keeps `lo` clear of the
-// subnormals), and a product is hi hi + hi lo + lo hi in fp32 accumulators: three MFMAs in place of one fp32 product at
-// a sixteenth of the rate, with an error near that of fp32 (one fp16 or bf16 plane loses 3 to 6 bits over five steps,
-// more than the rounding of a bf16 result).  Planes are interleaved by 8 elements ([row][k / 8][hi 8][lo 8]), so a
-// K slice of 32 is one 128-byte row piece.  All dimensions are padded to whole tiles with zeros, which every product
-// preserves; A and B are symmetric, and only their tiles on and below the diagonal are computed.
-// X is also kept transposed, because B X needs it with m contiguous.
+// on the fp16 matrix cores.  Values are held times 2^10 (singular values stay below ~4, so nothing leaves the fp16 range,
+// and the scale keeps small entries clear of the subnormals) in fp16 planes: `hi`, and `lo` with what hi leaves, together
+// 22 significant bits.
+//
+//  * PAIR (fp32 and fp16 results): every operand is hi + lo and a product is hi hi + hi lo + lo hi in fp32 accumulators,
+//    32-bit products at three times the cost of one fp16 product; fp32's own matrix rate is 1 / 16 of fp16's.
+//  * single (bf16 results): products take the hi planes alone, a third of the cost.  What keeps the error (2e-4 .. 7e-4,
+//    2e-3 where a few directions are 100 times the rest) below the rounding of the result (1.7e-3): X itself stays hi + lo
+//    (with one plane: 5e-3 to 2e-2 there), and the diagonals of A and B, which are near 1 and -2.7 and would be rounded
+//    as such (1.4e-3 to 1.8e-3 by themselves), are kept apart in fp32; with A = Ao + Da,
+//        A A = Ao Ao + (Da_i + Da_j) Ao_ij + Da^2,   a X + B X = (a + Db_i) X_ij + Bo X.
+//
+// A and B are symmetric: only tiles on and below the diagonal are computed.  X is also kept transposed, because B X needs
+// it with m contiguous.  Dimensions are padded to whole tiles with zeros, which every product preserves.
+//
+// Two product kernels (ns_use_large has the rule and its measurements):
+//  * 256 x 256 tiles, 8 waves: the half-tile ring of the framework's large GEMM (gemm8.hip has the ordering argument),
+//    bound by the matrix cores; the epilogue moves whole 128-byte row pieces through the free ring.
+//  * 64 x 64 tiles, 4 waves: for matrices too small or too few to fill the card with the large ones; bound by latency
+//    and by the L2's rate.
 #include "../common.h"
 #include "transformer.h"
 #include <type_traits>
@@ -21,7 +33,6 @@ namespace {
 typedef __attribute__((address_space(3))) void* lds_void_ptr;
 typedef const __attribute__((address_space(1))) void* gbl_void_ptr;
 
-constexpr int kTile = 128;
 constexpr float kScale = 1024.f, kInvScale = 1.f / 1024.f;
 constexpr int kNormParts = 64;
 
@@ -32,8 +43,12 @@ __device__ __forceinline__ Half2 split(float x) {
   h.lo = (_Float16)(x - (float)h.hi);
   return h;
 }
-// element (r, k) of a plane pair
-__device__ __forceinline__ long at(long r, long k, long ld) { return r * ld + ((k >> 3) << 4) + (k & 7); }
+__device__ __forceinline__ uint32_t pack(_Float16 a, _Float16 b) {
+  uint16_t x, y;
+  __builtin_memcpy(&x, &a, 2);
+  __builtin_memcpy(&y, &b, 2);
+  return (uint32_t)x | ((uint32_t)y << 16);
+}
 
 // ---- |G|_F^2 in 64 bits: kNormParts partial sums a matrix
 template <typename T>
@@ -53,11 +68,16 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const T* __restrict__ g, l
   if (threadIdx.x == 0) parts[(long)blockIdx.y * kNormParts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// ---- X and X^T planes of 64 x 64 elements of the normalised matrix (zeros in the padding)
+// a matrix of fp16 planes: rows of ld elements, `next` elements from one matrix of the batch to the next
+struct Planes {
+  _Float16* hi; _Float16* lo;
+  long ld, next;
+};
+
+// ---- planes of X and X^T, 64 x 64 elements of the normalised matrix (zeros in the padding)
 template <typename T>
 __global__ __launch_bounds__(256) void ns_split_kernel(const T* __restrict__ g, long rows, long cols, int turned, double eps,
-                                                       const double* __restrict__ parts, _Float16* __restrict__ x,
-                                                       _Float16* __restrict__ xt, long mp, long np) {
+                                                       const double* __restrict__ parts, const Planes x, const Planes xt) {
   __shared__ float tile[64][65];
   __shared__ float inv_s;
   const long b = blockIdx.z;
@@ -78,230 +98,632 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const T* __restrict__ g, 
     else tile[r][c] = v;
   }
   __syncthreads();
-  _Float16* xb = x + b * mp * np * 2;
-  _Float16* xtb = xt + b * mp * np * 2;
   for (int e = threadIdx.x; e < 512; e += 256) {
-    const int r = e >> 3, u = e & 7;
+    const int r = e >> 3, u = (e & 7) * 8;
     f16x8_t h, l;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const Half2 v = split(tile[r][u * 8 + q]);
+      const Half2 v = split(tile[r][u + q]);
       h[q] = v.hi; l[q] = v.lo;
     }
-    f16x8_t* d = reinterpret_cast<f16x8_t*>(xb + at(i0 + r, j0 + u * 8, 2 * np));
-    d[0] = h; d[1] = l;
+    long o = b * x.next + (i0 + r) * x.ld + j0 + u;
+    *reinterpret_cast<f16x8_t*>(x.hi + o) = h;
+    *reinterpret_cast<f16x8_t*>(x.lo + o) = l;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const Half2 v = split(tile[u * 8 + q][r]);
+      const Half2 v = split(tile[u + q][r]);
       h[q] = v.hi; l[q] = v.lo;
     }
-    d = reinterpret_cast<f16x8_t*>(xtb + at(j0 + r, i0 + u * 8, 2 * mp));
-    d[0] = h; d[1] = l;
+    o = b * xt.next + (j0 + r) * xt.ld + i0 + u;
+    *reinterpret_cast<f16x8_t*>(xt.hi + o) = h;
+    if (xt.lo != nullptr) *reinterpret_cast<f16x8_t*>(xt.lo + o) = l;
   }
 }
 
-// ---- out = alpha * R + beta * P Q^T on plane pairs
+// ---- products: P Q^T on planes with the contraction contiguous, and what becomes of it
+enum Op : int { kGram = 0, kPoly = 1, kApply = 2, kFinal = 3 };
 struct Product {
-  const _Float16* P; const _Float16* Q; const _Float16* R;
-  _Float16* out; _Float16* out_t;            // planes of the result and of its transpose (each may be null)
-  void* fin;                                 // the last step: the result in the caller's type and orientation
-  long ldp, ldq, ldr, ldo, ldt;              // in fp16 elements: twice the padded row length
-  long bp, bq, br, bo, bt, bfin;             // from one matrix of the batch to the next
-  int mt, nt, ksteps, sym, turned;
-  long rows, cols;                           // of the caller's matrix
-  float alpha, beta, fin_scale;
+  Planes P, Q, R, out, out_t;               // R: added term; out: result, out_t: its transpose (lo may be null)
+  float* diag;                              // kGram: Da (written), kPoly and kApply: read (Da, Db)
+  float* diag_out;                          // kPoly: Db
+  void* fin;                                // kFinal: the result in the caller's type and orientation
+  long diag_next, fin_next;
+  int mt, nt, ktiles, turned;               // tiles; slices of 128 bytes of a row
+  long rows, cols;                          // of the caller's matrix
+  float c0, c1;                             // kPoly: b, c; kApply, kFinal: a, -
 };
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void ns_product_kernel(const Product p, const uint32_t per_matrix) {
-  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * kTile * 128];     // two stages of P and Q slices
+// which tile of which matrix
+struct Place { long b; int ti, tj; };
+template <int OP> __device__ __forceinline__ Place place_of(const Product& p, uint32_t per_matrix) {
+  const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);      // a matrix's tiles share an XCD's L2
+  Place q;
+  q.b = lid / per_matrix;
+  const uint32_t t = lid - (uint32_t)q.b * per_matrix;
+  if constexpr (OP == kGram || OP == kPoly) {                 // on and below the diagonal
+    q.ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((uint32_t)(q.ti + 1) * (q.ti + 2) / 2 <= t) ++q.ti;
+    while ((uint32_t)q.ti * (q.ti + 1) / 2 > t) --q.ti;
+    q.tj = (int)(t - (uint32_t)q.ti * (q.ti + 1) / 2);
+  } else {
+    q.ti = (int)(t % (uint32_t)p.mt);
+    q.tj = (int)(t / (uint32_t)p.mt);
+  }
+  return q;
+}
+
+// element (i, j) of the result from the accumulated product, in the scale of the planes; r = R(i, j)
+template <int OP> __device__ __forceinline__ float combine(float acc, float r, float di, float dj, float c0, float c1) {
+  if constexpr (OP == kGram) return acc * kInvScale;
+  else if constexpr (OP == kPoly) return c0 * r + c1 * (acc * kInvScale + (di + dj) * r);
+  else return (c0 + di) * r + acc * kInvScale;
+}
+// the diagonal element's true value
+template <int OP> __device__ __forceinline__ float on_diagonal(float acc, float di, float c0, float c1) {
+  if constexpr (OP == kGram) return acc * kInvScale * kInvScale;
+  else return c0 * di + c1 * (acc * kInvScale * kInvScale + di * di);
+}
+
+// ================================================================================ 64 x 64 tiles
+constexpr int kSmall = 64;
+constexpr int kRingSmall = 4;               // slices in LDS: 3 in flight ahead of the one that is read
+
+template <bool PAIR, int OP, typename T>
+__global__ __launch_bounds__(256, 2) void ns_small_kernel(const Product p, const uint32_t per_matrix) {
+  __shared__ __attribute__((aligned(16))) unsigned char smem[kRingSmall * 2 * kSmall * 128];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave >> 1, wc = wave & 1, l31 = lane & 31, lh = lane >> 5;
-  const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
-  const long b = lid / per_matrix;
-  uint32_t t = lid - (uint32_t)b * per_matrix;
-  int ti, tj;
-  if (p.sym) {                               // tiles on and below the diagonal
-    ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((uint32_t)(ti + 1) * (ti + 2) / 2 <= t) ++ti;
-    while ((uint32_t)ti * (ti + 1) / 2 > t) --ti;
-    tj = (int)(t - (uint32_t)ti * (ti + 1) / 2);
-  } else {
-    ti = (int)(t % (uint32_t)p.mt);
-    tj = (int)(t / (uint32_t)p.mt);
-  }
-  const long i0 = (long)ti * kTile, j0 = (long)tj * kTile;
-  // staging: instruction q of a wave covers rows (wave * 4 + q) * 8 + lane / 8; LDS chunk lane % 8 holds source chunk
-  // (lane % 8) ^ ((row >> 1) & 7), so that 16 rows of a fragment read touch 16 different 16-byte columns
-  const _Float16* srcp[4];
-  const _Float16* srcq[4];
+  const Place at = place_of<OP>(p, per_matrix);
+  const long b = at.b, i0 = (long)at.ti * kSmall, j0 = (long)at.tj * kSmall;
+  // staging: instruction q of a wave covers rows (wave * 2 + q) * 8 + lane / 8; LDS chunk lane % 8 holds source chunk
+  // (lane % 8) ^ ((row >> 1) & 7), so that 16 rows of a fragment read touch 16 different 16-byte columns.  PAIR: chunks
+  // 0 .. 3 are 32 elements of hi, 4 .. 7 the same of lo
+  const _Float16* src[2][2];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int row = (wave * 4 + q) * 8 + (lane >> 3);
+  for (int q = 0; q < 2; ++q) {
+    const int row = (wave * 2 + q) * 8 + (lane >> 3);
     const int ch = (lane & 7) ^ ((row >> 1) & 7);
-    srcp[q] = p.P + b * p.bp + (i0 + row) * p.ldp + ch * 8;
-    srcq[q] = p.Q + b * p.bq + (j0 + row) * p.ldq + ch * 8;
+    const _Float16* hp = PAIR && ch >= 4 ? p.P.lo : p.P.hi;
+    const _Float16* hq = PAIR && ch >= 4 ? p.Q.lo : p.Q.hi;
+    const int k = (PAIR ? ch & 3 : ch) * 8;
+    src[0][q] = hp + b * p.P.next + (i0 + row) * p.P.ld + k;
+    src[1][q] = hq + b * p.Q.next + (j0 + row) * p.Q.ld + k;
   }
   auto stage = [&](int k) {
-    unsigned char* dst = smem + (k & 1) * (2 * kTile * 128) + wave * 4096;
+    unsigned char* dst = smem + (k % kRingSmall) * (2 * kSmall * 128) + wave * 2048;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(srcp[q] + (long)k * 64), (lds_void_ptr)(dst + q * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(srcq[q] + (long)k * 64), (lds_void_ptr)(dst + kTile * 128 + q * 1024), 16,
+    for (int q = 0; q < 2; ++q) {
+      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[0][q] + (long)k * (PAIR ? 32 : 64)), (lds_void_ptr)(dst + q * 1024), 16,
                                        0, 0);
+      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[1][q] + (long)k * (PAIR ? 32 : 64)),
+                                       (lds_void_ptr)(dst + kSmall * 128 + q * 1024), 16, 0, 0);
     }
   };
-  f32x16_t acc[2][2];
+  f32x16_t acc;
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[a][c][r] = 0.f;
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  const int nk = p.ktiles;
+  // four loads a slice and wave: with slices k .. k + 2 requested, vmcnt(8) means that slice k has landed
   stage(0);
-  for (int k = 0; k < p.ksteps; ++k) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                         // slice k has landed for every wave, and slice k - 1 has been read
-    if (k + 1 < p.ksteps) stage(k + 1);
-    const unsigned char* base = smem + (k & 1) * (2 * kTile * 128);
-    f16x8_t fp[2][2][2], fq[2][2][2];        // [32-row block][k16][hi, lo]
+  if (nk > 1) stage(1);
+  if (nk > 2) stage(2);
+  for (int k = 0; k < nk; ++k) {
+    if (k + 2 < nk) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else if (k + 1 < nk) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                        // slice k has landed for every wave; slice k - 1 has been read by all
+    if (k + 3 < nk) stage(k + 3);           // ... and its slot is free
+    const unsigned char* base = smem + (k % kRingSmall) * (2 * kSmall * 128);
+    f16x8_t fp[4], fq[4];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int c = 0; c < 4; ++c) {
+      // PAIR: c = k16 step * 2 + plane, else the k16 step
+      const int ch = (PAIR ? (c & 1) * 4 + (c >> 1) * 2 + lh : c * 2 + lh) ^ ((l31 >> 1) & 7);
+      fp[c] = *reinterpret_cast<const f16x8_t*>(base + (wr * 32 + l31) * 128 + ch * 16);
+      fq[c] = *reinterpret_cast<const f16x8_t*>(base + kSmall * 128 + (wc * 32 + l31) * 128 + ch * 16);
+    }
+    if constexpr (PAIR) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 4; s += 2) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s], fp[s], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s + 1], fp[s], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s], fp[s + 1], acc, 0, 0, 0);
+      }
+    } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int ch = ((s * 2 + lh) * 2 + h) ^ ((l31 >> 1) & 7);
-          fp[m][s][h] = *reinterpret_cast<const f16x8_t*>(base + (wr * 64 + m * 32 + l31) * 128 + ch * 16);
-          fq[m][s][h] = *reinterpret_cast<const f16x8_t*>(base + kTile * 128 + (wc * 64 + m * 32 + l31) * 128 + ch * 16);
-        }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int x = 0; x < 3; ++x)            // hi hi, hi lo, lo hi
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-            acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[n][s][x == 1], fp[m][s][x == 2], acc[m][n], 0, 0, 0);
+      for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s], fp[s], acc, 0, 0, 0);
+    }
   }
-  // acc[m][n][r] is element (i0 + wr * 64 + m * 32 + l31, j0 + wc * 64 + n * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh)
-  const bool mirror = p.out_t != nullptr && !(p.sym && ti == tj);
+  // acc[r] is element (i0 + wr * 32 + l31, j0 + wc * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh)
+  constexpr bool SYM = OP == kGram || OP == kPoly;
+  const long i = i0 + wr * 32 + l31;
+  const float* diag = p.diag + b * p.diag_next;
+  const float di = OP == kGram ? 0.f : diag[i];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const long i = i0 + wr * 64 + m * 32 + l31;
+  for (int g = 0; g < 4; ++g) {
+    const long j = j0 + wc * 32 + 8 * g + 4 * lh;
+    float v[4];
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (OP != kGram) {
+      const long o = b * p.R.next + i * p.R.ld + j;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int q = 0; q < 4; ++q) r[q] = (float)p.R.hi[o + q] + (p.R.lo != nullptr ? (float)p.R.lo[o + q] : 0.f);
+    }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const long j = j0 + wc * 64 + n * 32 + 8 * g + 4 * lh;
-        float v[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = p.beta * acc[m][n][g * 4 + q];
-        if (p.R != nullptr) {
-          const _Float16* r = p.R + b * p.br + at(i, j, p.ldr);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] += p.alpha * ((float)r[q] + (float)r[q + 8]);
+    for (int q = 0; q < 4; ++q) {
+      const float dj = OP == kPoly ? diag[j + q] : 0.f;
+      v[q] = combine<OP>(acc[g * 4 + q], r[q], di, dj, p.c0, p.c1);
+      if constexpr (SYM)
+        if (i == j + q) {
+          (OP == kGram ? p.diag : p.diag_out)[b * p.diag_next + i] = on_diagonal<OP>(acc[g * 4 + q], di, p.c0, p.c1);
+          v[q] = 0.f;
         }
-        if (p.fin != nullptr) {
-          T* f = reinterpret_cast<T*>(p.fin) + b * p.bfin;
+    }
+    if constexpr (OP == kFinal) {
+      T* f = reinterpret_cast<T*>(p.fin) + b * p.fin_next;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const long r = p.turned ? j + q : i, c = p.turned ? i : j + q;
-            if (r < p.rows && c < p.cols) f[r * p.cols + c] = from_float<T>(v[q] * p.fin_scale);
-          }
-        }
-        if (p.out != nullptr || mirror) {
-          Half2 h[4];
+      for (int q = 0; q < 4; ++q) {
+        const long row = p.turned ? j + q : i, col = p.turned ? i : j + q;
+        if (row < p.rows && col < p.cols) f[row * p.cols + col] = from_float<T>(v[q] * kInvScale);
+      }
+    } else {
+      Half2 h[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) h[q] = split(v[q]);
-          if (p.out != nullptr) {
-            _Float16* o = p.out + b * p.bo + at(i, j, p.ldo);
+      for (int q = 0; q < 4; ++q) h[q] = split(v[q]);
+      const long o = b * p.out.next + i * p.out.ld + j;
+      *reinterpret_cast<uint2*>(p.out.hi + o) = make_uint2(pack(h[0].hi, h[1].hi), pack(h[2].hi, h[3].hi));
+      if (p.out.lo != nullptr) *reinterpret_cast<uint2*>(p.out.lo + o) = make_uint2(pack(h[0].lo, h[1].lo), pack(h[2].lo, h[3].lo));
+      if (!SYM || at.ti != at.tj) {
+        const long t = b * p.out_t.next + j * p.out_t.ld + i;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) { o[q] = h[q].hi; o[q + 8] = h[q].lo; }
-          }
-          if (mirror)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              _Float16* o = p.out_t + b * p.bt + at(j + q, i, p.ldt);
-              o[0] = h[q].hi;
-              o[8] = h[q].lo;
-            }
+        for (int q = 0; q < 4; ++q) {
+          p.out_t.hi[t + q * p.out_t.ld] = h[q].hi;
+          if (p.out_t.lo != nullptr) p.out_t.lo[t + q * p.out_t.ld] = h[q].lo;
         }
       }
+    }
   }
 }
 
-template <typename T>
-void product(const Product& p, long batch, hipStream_t s) {
-  const uint32_t per = p.sym ? (uint32_t)p.mt * (p.mt + 1) / 2 : (uint32_t)p.mt * p.nt;
+// ================================================================================ 256 x 256 tiles
+constexpr int kLarge = 256;
+constexpr int kHalf = 128 * 128;            // bytes of a half-tile: 128 rows of a 128-byte slice
+constexpr int kRing = 8 * kHalf;            // two K slices of P and Q
+
+template <int OFF> __device__ __forceinline__ f16x8_t lds_read16(uint32_t addr) {
+  uint4 r;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(OFF));
+  f16x8_t v;
+  __builtin_memcpy(&v, &r, 16);
+  return v;
+}
+// Makes the accumulators new values to the compiler: it would otherwise keep what one pass of the epilogue derived from
+// them for the next one, and spill thousands of registers.
+__device__ __forceinline__ void forget(f32x16_t (&acc)[2][2][2]) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) asm volatile("" : "+v"(acc[x >> 2][(x >> 1) & 1][x & 1]));
+}
+// products of one 32 x 32 block over one K slice
+template <bool PAIR> __device__ __forceinline__ void block_mma(f32x16_t& acc, const f16x8_t (&q)[4], const f16x8_t (&f)[4]) {
+  if constexpr (PAIR) {                     // [k16 step * 2 + plane]
+#pragma unroll
+    for (int s = 0; s < 4; s += 2) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[s], f[s], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[s + 1], f[s], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[s], f[s + 1], acc, 0, 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[s], f[s], acc, 0, 0, 0);
+  }
+}
+
+template <bool PAIR, int OP, typename T>
+__global__ __launch_bounds__(512, 1) void ns_large_kernel(const Product p, const uint32_t per_matrix) {
+  __shared__ __attribute__((aligned(16))) unsigned char smem[kRing];
+  constexpr bool SYM = OP == kGram || OP == kPoly;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave >> 2, wc = wave & 3;
+  const int l31 = lane & 31, lh = lane >> 5;
+  const Place at = place_of<OP>(p, per_matrix);
+  const long b = at.b, m0 = (long)at.ti * kLarge, n0 = (long)at.tj * kLarge;
+  const int nk = p.ktiles, nhalf = 4 * nk;
+
+  // staging: wave-instruction i of this wave covers rows (wave * 2 + i) * 8 + lane / 8 of a half-tile; chunks swizzled as
+  // in the small kernel.  Half-tile kinds: Q rows 0 .. 127, 128 .. 255, P rows 0 .. 127, 128 .. 255
+  const _Float16* src[4][2];
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = (wave * 2 + i) * 8 + (lane >> 3);
+      const int ch = (lane & 7) ^ ((row >> 1) & 7);
+      const Planes& m = h >= 2 ? p.P : p.Q;
+      const _Float16* base = PAIR && ch >= 4 ? m.lo : m.hi;
+      src[h][i] = base + b * m.next + ((h >= 2 ? m0 : n0) + (h & 1) * 128 + row) * m.ld + (PAIR ? ch & 3 : ch) * 8;
+    }
+  auto stage = [&](int g, auto kind_c) {
+    constexpr int h = decltype(kind_c)::value;
+    unsigned char* dst = smem + (g & 7) * kHalf + wave * 2048;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      __builtin_amdgcn_global_load_lds((gbl_void_ptr)src[h][i], (lds_void_ptr)(dst + i * 1024), 16, 0, 0);
+      src[h][i] += PAIR ? 32 : 64;
+    }
+  };
+  constexpr std::integral_constant<int, 0> kB0{};
+  constexpr std::integral_constant<int, 1> kB1{};
+  constexpr std::integral_constant<int, 2> kA0{};
+  constexpr std::integral_constant<int, 3> kA1{};
+
+  const uint32_t lds0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) unsigned char*)smem);
+  uint32_t cA[4], cB[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int ch = PAIR ? (c & 1) * 4 + (c >> 1) * 2 + lh : c * 2 + lh;
+    const uint32_t o = (uint32_t)((ch ^ ((l31 >> 1) & 7)) * 16) + (uint32_t)l31 * 128;
+    cA[c] = lds0 + (2 + wr) * kHalf + o;
+    cB[c] = lds0 + (wc >> 1) * kHalf + (wc & 1) * 8192 + o;
+  }
+  f32x16_t acc[2][2][2];                    // [mq][mt][nq]
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[x][y][z][r] = 0.f;
+
+  // prologue: half-tiles 0 .. 4, K slice 0 complete (one half-tile may stay in flight)
+  stage(0, kB0);
+  stage(1, kB1);
+  stage(2, kA0);
+  stage(3, kA1);
+  if (4 < nhalf) {
+    stage(4, kB0);
+    asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  __builtin_amdgcn_s_barrier();
+  if (wr == 1) __builtin_amdgcn_s_barrier();          // this group runs one barrier behind
+
+  f16x8_t fa[2][4], fb[2][4];               // P fragments of the current mq [mt], Q fragments [nq]
+  for (int t = 0; t < nk; ++t) {
+    const uint32_t tb = (uint32_t)(t & 1) * (4 * kHalf);
+    const int g = 4 * t + 5;                // half-tile requested in phase 0 of this K slice
+    // ---- phase 0: quadrant (m 0, n 0)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) fb[0][c] = lds_read16<0>(cB[c] + tb);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      fa[0][c] = lds_read16<0>(cA[c] + tb);
+      fa[1][c] = lds_read16<4096>(cA[c] + tb);
+    }
+    if (g < nhalf) stage(g, kB1);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    block_mma<PAIR>(acc[0][0][0], fb[0], fa[0]);
+    block_mma<PAIR>(acc[0][1][0], fb[0], fa[1]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_barrier();
+    // ---- phase 1: quadrant (m 0, n 1)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) fb[1][c] = lds_read16<4096>(cB[c] + tb);
+    if (g + 1 < nhalf) stage(g + 1, kA0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    block_mma<PAIR>(acc[0][0][1], fb[1], fa[0]);
+    block_mma<PAIR>(acc[0][1][1], fb[1], fa[1]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_barrier();
+    // ---- phase 2: quadrant (m 1, n 1)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      fa[0][c] = lds_read16<8192>(cA[c] + tb);
+      fa[1][c] = lds_read16<12288>(cA[c] + tb);
+    }
+    if (g + 2 < nhalf) stage(g + 2, kA1);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    block_mma<PAIR>(acc[1][0][1], fb[1], fa[0]);
+    block_mma<PAIR>(acc[1][1][1], fb[1], fa[1]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_barrier();
+    // ---- phase 3: quadrant (m 1, n 0): operands are in registers; K slice t + 1 must have landed
+    if (g + 3 < nhalf) {
+      stage(g + 3, kB0);
+      asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    block_mma<PAIR>(acc[1][0][0], fb[0], fa[0]);
+    block_mma<PAIR>(acc[1][1][0], fb[0], fa[1]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_barrier();
+  }
+  if (wr == 0) __builtin_amdgcn_s_barrier();          // balance the stagger
+
+  // ---- epilogue.  acc[mq][mt][nq][r] is element (m0 + wr*128 + mq*64 + mt*32 + l31,
+  // n0 + wc*64 + nq*32 + (r & 3) + 8 * (r >> 2) + 4 * lh).  Every wave is past its last read of the ring, and owns 16 KiB
+  // of it: 128 rows of 64 elements ([row][8 chunks of 16 bytes], chunk ^ (row & 7)), or 64 rows of 128 for the transpose.
+  // Only the wave itself touches them, so a wait for its own LDS traffic orders everything.
+  unsigned char* my = smem + wave * 16384;
+  const long mw = m0 + wr * 128, nw = n0 + wc * 64;
+  const float* diag = p.diag + b * p.diag_next;
+  float di[2][2];
+#pragma unroll
+  for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) di[mq][mt] = OP == kGram ? 0.f : diag[mw + mq * 64 + mt * 32 + l31];
+
+  if constexpr (SYM) {                      // the diagonal, before the off-diagonal terms are added
+    if (at.ti == at.tj)
+#pragma unroll
+      for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nq = 0; nq < 2; ++nq)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const long i = mw + mq * 64 + mt * 32 + l31, j = nw + nq * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh;
+              if (i == j)
+                (OP == kGram ? p.diag : p.diag_out)[b * p.diag_next + i] =
+                    on_diagonal<OP>(acc[mq][mt][nq][r], di[mq][mt], p.c0, p.c1);
+            }
+  }
+  // acc <- result: one plane of R at a time through LDS (lo alone first, so that r = hi + lo is added up term by term)
+  if constexpr (OP == kGram) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x >> 2][(x >> 1) & 1][x & 1][r] *= kInvScale;
+  } else {
+    const float scale = OP == kPoly ? p.c1 * kInvScale : kInvScale;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x >> 2][(x >> 1) & 1][x & 1][r] *= scale;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      const _Float16* R = plane ? p.R.lo : p.R.hi;
+      if (R == nullptr) continue;
+      forget(acc);
+      R += b * p.R.next + mw * p.R.ld + nw;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int row = i * 8 + (lane >> 3);
+        __builtin_amdgcn_global_load_lds((gbl_void_ptr)(R + row * p.R.ld + ((lane & 7) ^ (row & 7)) * 8),
+                                         (lds_void_ptr)(my + i * 1024), 16, 0, 0);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nq = 0; nq < 2; ++nq)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int row = mq * 64 + mt * 32 + l31, col = nq * 32 + 8 * g + 4 * lh;
+              const uint2 raw = *reinterpret_cast<const uint2*>(my + row * 128 + (((col >> 3) ^ (row & 7)) * 16) + (col & 7) * 2);
+              _Float16 h[4];
+              __builtin_memcpy(h, &raw, 8);
+              float4 dj = make_float4(0.f, 0.f, 0.f, 0.f);
+              if constexpr (OP == kPoly) dj = *reinterpret_cast<const float4*>(diag + nw + col);
+              const float djs[4] = {dj.x, dj.y, dj.z, dj.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float f = OP == kPoly ? p.c0 + p.c1 * (di[mq][mt] + djs[q]) : p.c0 + di[mq][mt];
+                acc[mq][mt][nq][g * 4 + q] += f * (float)h[q];
+              }
+              __builtin_amdgcn_sched_barrier(0);      // (left to itself the compiler reads ahead until it spills)
+            }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  }
+  if constexpr (SYM) {
+    if (at.ti == at.tj)
+#pragma unroll
+      for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nq = 0; nq < 2; ++nq)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (mw + mq * 64 + mt * 32 + l31 == nw + nq * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh) acc[mq][mt][nq][r] = 0.f;
+  }
+
+  if constexpr (OP == kFinal) {
+    // the caller's rows may start anywhere: its type and orientation straight from registers
+    T* f = reinterpret_cast<T*>(p.fin) + b * p.fin_next;
+#pragma unroll
+    for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int nq = 0; nq < 2; ++nq)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const long i = mw + mq * 64 + mt * 32 + l31, j = nw + nq * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh;
+            const long row = p.turned ? j : i, col = p.turned ? i : j;
+            if (row < p.rows && col < p.cols) f[row * p.cols + col] = from_float<T>(acc[mq][mt][nq][r] * kInvScale);
+          }
+    return;
+  } else {
+    // rows of the result: hi, then lo
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      _Float16* out = plane ? p.out.lo : p.out.hi;
+      if (out == nullptr) continue;
+      forget(acc);
+      out += b * p.out.next + mw * p.out.ld + nw;
+#pragma unroll
+      for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nq = 0; nq < 2; ++nq)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int row = mq * 64 + mt * 32 + l31, col = nq * 32 + 8 * g + 4 * lh;
+              _Float16 h[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const Half2 s = split(acc[mq][mt][nq][g * 4 + q]);
+                h[q] = plane ? s.lo : s.hi;
+              }
+              *reinterpret_cast<uint2*>(my + row * 128 + (((col >> 3) ^ (row & 7)) * 16) + (col & 7) * 2) =
+                  make_uint2(pack(h[0], h[1]), pack(h[2], h[3]));
+              __builtin_amdgcn_sched_barrier(0);
+            }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int row = i * 8 + (lane >> 3), ck = lane & 7;
+        const uint4 v = *reinterpret_cast<const uint4*>(my + row * 128 + ((ck ^ (row & 7)) * 16));
+        *reinterpret_cast<uint4*>(out + row * p.out.ld + ck * 8) = v;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    // rows of the transpose: neighbouring lanes hold neighbouring columns of it; they trade so that each has two columns
+    // of one row (a lane of even number the row of register r, its neighbour that of r + 1)
+    if (SYM && at.ti == at.tj) return;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      _Float16* out = plane ? p.out_t.lo : p.out_t.hi;
+      if (out == nullptr) continue;
+      forget(acc);
+      out += b * p.out_t.next + nw * p.out_t.ld + mw;
+#pragma unroll
+      for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nq = 0; nq < 2; ++nq)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              const Half2 s0 = split(acc[mq][mt][nq][r]), s1 = split(acc[mq][mt][nq][r + 1]);
+              const uint32_t both = plane ? pack(s0.lo, s1.lo) : pack(s0.hi, s1.hi);
+              const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)both, 0xB1, 0xf, 0xf, true);   // lanes 1 0 3 2
+              const bool odd = lane & 1;
+              const uint32_t v = odd ? (other >> 16) | (both & 0xffff0000u) : (both & 0xffffu) | (other << 16);
+              const int n = nq * 32 + ((r + (odd ? 1 : 0)) & 3) + 8 * (r >> 2) + 4 * lh;
+              const int m = mq * 64 + mt * 32 + (l31 & ~1);
+              *reinterpret_cast<uint32_t*>(my + n * 256 + (((m >> 3) ^ (n & 15)) * 16) + (m & 7) * 2) = v;
+              if ((r & 3) == 2) __builtin_amdgcn_sched_barrier(0);
+            }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int n = i * 4 + (lane >> 4), ck = lane & 15;
+        const uint4 v = *reinterpret_cast<const uint4*>(my + n * 256 + ((ck ^ (n & 15)) * 16));
+        *reinterpret_cast<uint4*>(out + n * p.out_t.ld + ck * 8) = v;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  }
+}
+
+// Tile of the products, and with it the padding.
+bool ns_use_large(long batch, long m, long n) {
+  const long mt = (m + kLarge - 1) / kLarge;
+  (void)n;
+  return batch * mt * (mt + 1) / 2 >= 96;
+}
+
+template <bool PAIR, int OP, typename T>
+void product(const Product& p, long batch, bool large, hipStream_t s) {
+  const uint32_t per = OP == kGram || OP == kPoly ? (uint32_t)p.mt * (p.mt + 1) / 2 : (uint32_t)p.mt * p.nt;
   const long blocks = (long)per * batch;
   if (blocks >= (1l << 31)) throw std::invalid_argument("newton_schulz: batch too large");
-  hipLaunchKernelGGL(ns_product_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, p, per);
+  if (large) hipLaunchKernelGGL((ns_large_kernel<PAIR, OP, T>), dim3((unsigned)blocks), dim3(512), 0, s, p, per);
+  else hipLaunchKernelGGL((ns_small_kernel<PAIR, OP, T>), dim3((unsigned)blocks), dim3(256), 0, s, p, per);
 }
 
 struct Sizes {
-  long m, n, mp, np;                         // X: m <= n, padded
-  size_t x, sq, norm;                        // bytes of the X planes, of A and of the partial norms
+  long m, n, mp, np;                        // X: m <= n, padded
+  bool large;
+  size_t x, sq, diag, norm;                 // bytes of one plane of X, of A, of a diagonal, of the partial norms
 };
 Sizes sizes(long batch, long rows, long cols) {
   Sizes z;
   z.m = rows < cols ? rows : cols;
   z.n = rows < cols ? cols : rows;
-  z.mp = (z.m + kTile - 1) / kTile * kTile;
-  z.np = (z.n + kTile - 1) / kTile * kTile;
-  z.x = (size_t)batch * z.mp * z.np * 4;
-  z.sq = (size_t)batch * z.mp * z.mp * 4;
+  z.large = ns_use_large(batch, z.m, z.n);
+  const long tile = z.large ? kLarge : kSmall;
+  z.mp = (z.m + tile - 1) / tile * tile;
+  z.np = (z.n + tile - 1) / tile * tile;
+  z.x = (size_t)batch * z.mp * z.np * 2;
+  z.sq = (size_t)batch * z.mp * z.mp * 2;
+  z.diag = (size_t)batch * z.mp * 4;
   z.norm = (size_t)batch * kNormParts * 8;
   return z;
 }
 
-template <typename T>
+template <bool PAIR, typename T>
 void run(const NewtonSchulz& q, hipStream_t s) {
   const Sizes z = sizes(q.batch, q.rows, q.cols);
   const int turned = q.rows > q.cols;
   char* w = reinterpret_cast<char*>(q.work);
   auto take = [&](size_t bytes) { char* r = w; w += bytes; return r; };
-  _Float16* X = reinterpret_cast<_Float16*>(take(z.x));
-  _Float16* XT[2];
-  XT[0] = reinterpret_cast<_Float16*>(take(z.x));
-  XT[1] = reinterpret_cast<_Float16*>(take(z.x));
-  _Float16* A = reinterpret_cast<_Float16*>(take(z.sq));
-  _Float16* B = reinterpret_cast<_Float16*>(take(z.sq));
+  auto planes = [&](size_t bytes, long ld, long next, bool lo) {
+    Planes p{reinterpret_cast<_Float16*>(take(bytes)), nullptr, ld, next};
+    if (lo) p.lo = reinterpret_cast<_Float16*>(take(bytes));
+    return p;
+  };
+  const long bx = z.mp * z.np, ba = z.mp * z.mp;
+  const Planes X = planes(z.x, z.np, bx, true);
+  const Planes XT[2] = {planes(z.x, z.mp, bx, PAIR), planes(z.x, z.mp, bx, PAIR)};
+  const Planes A = planes(z.sq, z.mp, ba, PAIR), B = planes(z.sq, z.mp, ba, PAIR);
+  float* Da = reinterpret_cast<float*>(take(z.diag));
+  float* Db = reinterpret_cast<float*>(take(z.diag));
   double* norm = reinterpret_cast<double*>(take(z.norm));
   const T* g = reinterpret_cast<const T*>(q.g);
   hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(kNormParts, (unsigned)q.batch), dim3(256), 0, s, g, q.rows * q.cols, norm);
   hipLaunchKernelGGL(ns_split_kernel<T>, dim3((unsigned)(z.np / 64), (unsigned)(z.mp / 64), (unsigned)q.batch), dim3(256), 0, s,
-                     g, q.rows, q.cols, turned, q.eps, norm, X, XT[0], z.mp, z.np);
-  const long bx = z.mp * z.np * 2, ba = z.mp * z.mp * 2;
+                     g, q.rows, q.cols, turned, q.eps, norm, X, XT[0]);
+  const long tile = z.large ? kLarge : kSmall, slice = PAIR ? 32 : 64;
   for (int it = 0; it < q.steps; ++it) {
-    const bool last = it + 1 == q.steps;
-    Product a{};                             // A = X X^T
-    a.P = a.Q = X; a.ldp = a.ldq = 2 * z.np; a.bp = a.bq = bx;
-    a.out = a.out_t = A; a.ldo = a.ldt = 2 * z.mp; a.bo = a.bt = ba;
-    a.mt = a.nt = (int)(z.mp / kTile); a.ksteps = (int)(z.np / 32); a.sym = 1;
-    a.beta = kInvScale;
-    product<T>(a, q.batch, s);
-    Product b{};                             // B = b A + c A A
-    b.P = b.Q = b.R = A; b.ldp = b.ldq = b.ldr = 2 * z.mp; b.bp = b.bq = b.br = ba;
-    b.out = b.out_t = B; b.ldo = b.ldt = 2 * z.mp; b.bo = b.bt = ba;
-    b.mt = b.nt = (int)(z.mp / kTile); b.ksteps = (int)(z.mp / 32); b.sym = 1;
-    b.alpha = q.b; b.beta = q.c * kInvScale;
-    product<T>(b, q.batch, s);
-    Product c{};                             // X = a X + B X
-    c.P = B; c.ldp = 2 * z.mp; c.bp = ba;
-    c.Q = XT[it & 1]; c.ldq = 2 * z.mp; c.bq = bx;
-    c.R = X; c.ldr = 2 * z.np; c.br = bx;
-    if (last) {
-      c.fin = q.out; c.bfin = q.rows * q.cols; c.rows = q.rows; c.cols = q.cols; c.turned = turned; c.fin_scale = kInvScale;
+    Product a{};                            // A = X X^T
+    a.P = a.Q = X;
+    a.out = a.out_t = A;
+    a.diag = Da; a.diag_next = z.mp;
+    a.mt = a.nt = (int)(z.mp / tile); a.ktiles = (int)(z.np / slice);
+    product<PAIR, kGram, T>(a, q.batch, z.large, s);
+    Product b{};                            // B = b A + c A A
+    b.P = b.Q = b.R = A;
+    b.out = b.out_t = B;
+    b.diag = Da; b.diag_out = Db; b.diag_next = z.mp;
+    b.mt = b.nt = (int)(z.mp / tile); b.ktiles = (int)(z.mp / slice);
+    b.c0 = q.b; b.c1 = q.c;
+    product<PAIR, kPoly, T>(b, q.batch, z.large, s);
+    Product c{};                            // X = a X + B X
+    c.P = B; c.Q = XT[it & 1]; c.R = X;
+    c.diag = Db; c.diag_next = z.mp;
+    c.mt = (int)(z.mp / tile); c.nt = (int)(z.np / tile); c.ktiles = (int)(z.mp / slice);
+    c.c0 = q.a;
+    if (it + 1 == q.steps) {
+      c.fin = q.out; c.fin_next = q.rows * q.cols; c.rows = q.rows; c.cols = q.cols; c.turned = turned;
+      product<PAIR, kFinal, T>(c, q.batch, z.large, s);
     } else {
-      c.out = X; c.ldo = 2 * z.np; c.bo = bx;
-      c.out_t = XT[(it + 1) & 1]; c.ldt = 2 * z.mp; c.bt = bx;
+      c.out = X; c.out_t = XT[(it + 1) & 1];
+      product<PAIR, kApply, T>(c, q.batch, z.large, s);
     }
-    c.mt = (int)(z.mp / kTile); c.nt = (int)(z.np / kTile); c.ksteps = (int)(z.mp / 32);
-    c.alpha = q.a; c.beta = kInvScale;
-    product<T>(c, q.batch, s);
   }
 }
 
@@ -310,14 +732,19 @@ void run(const NewtonSchulz& q, hipStream_t s) {
 size_t newton_schulz_workspace(long batch, long rows, long cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) throw std::invalid_argument("newton_schulz: empty shape");
   const Sizes z = sizes(batch, rows, cols);
-  return 3 * z.x + 2 * z.sq + z.norm;
+  return 6 * z.x + 4 * z.sq + 2 * z.diag + z.norm;
 }
 
 void newton_schulz_launch(const NewtonSchulz& q, int dtype, hipStream_t s) {
   if (q.batch <= 0 || q.rows <= 0 || q.cols <= 0 || q.steps <= 0) throw std::invalid_argument("newton_schulz: empty shape or no steps");
   const Sizes z = sizes(q.batch, q.rows, q.cols);
   if (q.batch > 65535 || z.mp / 64 > 65535) throw std::invalid_argument("newton_schulz: too many matrices");
-  DPA_DISPATCH_DTYPE(dtype, run<T>(q, s));
+  switch (dtype) {
+    case kF32: run<true, float>(q, s); break;
+    case kF16: run<true, f16_t>(q, s); break;
+    case kBF16: run<false, bf16_t>(q, s); break;
+    default: throw std::invalid_argument("unsupported dtype");
+  }
   DPA_CHECK_HIP(hipGetLastError());
 }
 

@@ -442,6 +442,24 @@ def test_newton_schulz(shape, dtype):
     _ns_check(normal(gen(sum(shape)), shape, dtype))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(96, 40, 72), (97, 256, 130), (33, 300, 513), (10, 1024, 1030)])
+def test_newton_schulz_many_matrices(shape, dtype):
+    """Enough tiles for the large product kernel."""
+    _ns_check(normal(gen(sum(shape)), shape, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,m,n", [(1, 64, 200), (2, 200, 64), (40, 260, 300)])
+def test_newton_schulz_strong_directions(batch, m, n, dtype):
+    """A few directions 100 times the rest: the rest's singular values start near 10^-3 of the norm.  A result rounded
+    to bf16 is off by 2^-8 / sqrt(3) in the quadratic mean at most, so the bound leaves 2^-8 * sqrt(2 / 3) = 3e-3 to the
+    single-plane products, whose X keeps 22 bits."""
+    g = gen(batch)
+    u, v = normal(g, (batch, m, 4)), normal(g, (batch, 4, n))
+    _ns_check((normal(g, (batch, m, n)) + 50.0 * torch.matmul(u, v)).to(dtype))
+
+
 @pytest.mark.parametrize("steps", [1, 2, 5, 7])
 def test_newton_schulz_steps_and_coefficients(steps):
     g = normal(gen(steps), (2, 96, 160))
