@@ -131,12 +131,12 @@ struct Product {
   int mt, nt, ktiles, turned;               // tiles; slices of 128 bytes of a row
   long rows, cols;                          // of the caller's matrix
   float c0, c1;                             // kPoly: b, c; kApply, kFinal: a, -
-};
+  int splits; float* partial;               // kGram on 64 x 64 tiles: the contraction split over workgroups,
+};                                          // [tile][split][4096] sums
 
 // which tile of which matrix
 struct Place { long b; int ti, tj; };
-template <int OP> __device__ __forceinline__ Place place_of(const Product& p, uint32_t per_matrix) {
-  const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);      // a matrix's tiles share an XCD's L2
+template <int OP> __device__ __forceinline__ Place place_of(const Product& p, uint32_t per_matrix, uint32_t lid) {
   Place q;
   q.b = lid / per_matrix;
   const uint32_t t = lid - (uint32_t)q.b * per_matrix;
@@ -166,97 +166,59 @@ template <int OP> __device__ __forceinline__ float on_diagonal(float acc, float 
 
 // ================================================================================ 64 x 64 tiles
 constexpr int kSmall = 64;
-constexpr int kRingSmall = 4;               // slices in LDS: 3 in flight ahead of the one that is read
 
-template <bool PAIR, int OP, typename T>
-__global__ __launch_bounds__(256, 2) void ns_small_kernel(const Product p, const uint32_t per_matrix) {
-  __shared__ __attribute__((aligned(16))) unsigned char smem[kRingSmall * 2 * kSmall * 128];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = wave >> 1, wc = wave & 1, l31 = lane & 31, lh = lane >> 5;
-  const Place at = place_of<OP>(p, per_matrix);
+// products of one 32 x 32 block over one K slice.  The terms go to accumulators of their own: a chain on one of them
+// would wait for each product's full latency, and few waves are there to fill in
+template <bool PAIR> __device__ __forceinline__ void slice_mma(f32x16_t (&acc)[2], const f16x8_t (&q)[4], const f16x8_t (&f)[4]) {
+  if constexpr (PAIR) {                     // [k16 step * 2 + plane]
+    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[0], f[0], acc[0], 0, 0, 0);
+    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[1], f[0], acc[1], 0, 0, 0);
+    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[2], f[2], acc[0], 0, 0, 0);
+    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[0], f[1], acc[1], 0, 0, 0);
+    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[3], f[2], acc[0], 0, 0, 0);
+    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[2], f[3], acc[1], 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc[s & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q[s], f[s], acc[s & 1], 0, 0, 0);
+  }
+}
+
+// what becomes of a wave's sums on a 64 x 64 tile: half of the registers of its 32 x 32 quarter
+template <int OP, typename T>
+__device__ __forceinline__ void small_epilogue(const Product& p, const Place& at, int wave, int lane, const float (&sum)[8]) {
+  const int kg = wave >> 2, wr = (wave >> 1) & 1, wc = wave & 1, l31 = lane & 31, lh = lane >> 5;
   const long b = at.b, i0 = (long)at.ti * kSmall, j0 = (long)at.tj * kSmall;
-  // staging: instruction q of a wave covers rows (wave * 2 + q) * 8 + lane / 8; LDS chunk lane % 8 holds source chunk
-  // (lane % 8) ^ ((row >> 1) & 7), so that 16 rows of a fragment read touch 16 different 16-byte columns.  PAIR: chunks
-  // 0 .. 3 are 32 elements of hi, 4 .. 7 the same of lo
-  const _Float16* src[2][2];
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int row = (wave * 2 + q) * 8 + (lane >> 3);
-    const int ch = (lane & 7) ^ ((row >> 1) & 7);
-    const _Float16* hp = PAIR && ch >= 4 ? p.P.lo : p.P.hi;
-    const _Float16* hq = PAIR && ch >= 4 ? p.Q.lo : p.Q.hi;
-    const int k = (PAIR ? ch & 3 : ch) * 8;
-    src[0][q] = hp + b * p.P.next + (i0 + row) * p.P.ld + k;
-    src[1][q] = hq + b * p.Q.next + (j0 + row) * p.Q.ld + k;
-  }
-  auto stage = [&](int k) {
-    unsigned char* dst = smem + (k % kRingSmall) * (2 * kSmall * 128) + wave * 2048;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[0][q] + (long)k * (PAIR ? 32 : 64)), (lds_void_ptr)(dst + q * 1024), 16,
-                                       0, 0);
-      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[1][q] + (long)k * (PAIR ? 32 : 64)),
-                                       (lds_void_ptr)(dst + kSmall * 128 + q * 1024), 16, 0, 0);
-    }
-  };
-  f32x16_t acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-  const int nk = p.ktiles;
-  // four loads a slice and wave: with slices k .. k + 2 requested, vmcnt(8) means that slice k has landed
-  stage(0);
-  if (nk > 1) stage(1);
-  if (nk > 2) stage(2);
-  for (int k = 0; k < nk; ++k) {
-    if (k + 2 < nk) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    else if (k + 1 < nk) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                        // slice k has landed for every wave; slice k - 1 has been read by all
-    if (k + 3 < nk) stage(k + 3);           // ... and its slot is free
-    const unsigned char* base = smem + (k % kRingSmall) * (2 * kSmall * 128);
-    f16x8_t fp[4], fq[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      // PAIR: c = k16 step * 2 + plane, else the k16 step
-      const int ch = (PAIR ? (c & 1) * 4 + (c >> 1) * 2 + lh : c * 2 + lh) ^ ((l31 >> 1) & 7);
-      fp[c] = *reinterpret_cast<const f16x8_t*>(base + (wr * 32 + l31) * 128 + ch * 16);
-      fq[c] = *reinterpret_cast<const f16x8_t*>(base + kSmall * 128 + (wc * 32 + l31) * 128 + ch * 16);
-    }
-    if constexpr (PAIR) {
-#pragma unroll
-      for (int s = 0; s < 4; s += 2) {
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s], fp[s], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s + 1], fp[s], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s], fp[s + 1], acc, 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s], fp[s], acc, 0, 0, 0);
-    }
-  }
-  // acc[r] is element (i0 + wr * 32 + l31, j0 + wc * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh)
+  // sum[r] is element (i0 + wr * 32 + l31, j0 + wc * 32 + 16 * kg + (r & 3) + 8 * (r >> 2) + 4 * lh)
   constexpr bool SYM = OP == kGram || OP == kPoly;
   const long i = i0 + wr * 32 + l31;
   const float* diag = p.diag + b * p.diag_next;
   const float di = OP == kGram ? 0.f : diag[i];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const long j = j0 + wc * 32 + 8 * g + 4 * lh;
+  for (int g = 0; g < 2; ++g) {
+    const long j = j0 + wc * 32 + 16 * kg + 8 * g + 4 * lh;
     float v[4];
     float r[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (OP != kGram) {
       const long o = b * p.R.next + i * p.R.ld + j;
+      _Float16 h[4];
+      uint2 raw = *reinterpret_cast<const uint2*>(p.R.hi + o);
+      __builtin_memcpy(h, &raw, 8);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) r[q] = (float)p.R.hi[o + q] + (p.R.lo != nullptr ? (float)p.R.lo[o + q] : 0.f);
+      for (int q = 0; q < 4; ++q) r[q] = (float)h[q];
+      if (p.R.lo != nullptr) {
+        raw = *reinterpret_cast<const uint2*>(p.R.lo + o);
+        __builtin_memcpy(h, &raw, 8);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r[q] += (float)h[q];
+      }
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float dj = OP == kPoly ? diag[j + q] : 0.f;
-      v[q] = combine<OP>(acc[g * 4 + q], r[q], di, dj, p.c0, p.c1);
+      v[q] = combine<OP>(sum[g * 4 + q], r[q], di, dj, p.c0, p.c1);
       if constexpr (SYM)
         if (i == j + q) {
-          (OP == kGram ? p.diag : p.diag_out)[b * p.diag_next + i] = on_diagonal<OP>(acc[g * 4 + q], di, p.c0, p.c1);
+          (OP == kGram ? p.diag : p.diag_out)[b * p.diag_next + i] = on_diagonal<OP>(sum[g * 4 + q], di, p.c0, p.c1);
           v[q] = 0.f;
         }
     }
@@ -284,6 +246,119 @@ __global__ __launch_bounds__(256, 2) void ns_small_kernel(const Product p, const
       }
     }
   }
+}
+
+// 8 waves: two groups of four take turns at the K slices (a wave's reads, waits and products follow each other; the other
+// group's fill in), each wave a 32 x 32 quarter of the tile.  RING slices of LDS, RING - 2 in flight.
+template <bool PAIR, int OP, typename T, int RING>
+__global__ __launch_bounds__(512) void ns_small_kernel(const Product p, const uint32_t per_matrix) {
+  constexpr int kSlice = 2 * kSmall * 128;  // bytes
+  __shared__ __attribute__((aligned(16))) unsigned char smem[RING * kSlice];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = wave >> 2, wr = (wave >> 1) & 1, wc = wave & 1, l31 = lane & 31, lh = lane >> 5;
+  uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);           // a matrix's tiles share an XCD's L2
+  int first = 0, nk = p.ktiles, part = 0;
+  if constexpr (OP == kGram)
+    if (p.splits > 1) {
+      part = (int)(lid % (uint32_t)p.splits);
+      lid /= (uint32_t)p.splits;
+      const int each = (p.ktiles + p.splits - 1) / p.splits;
+      first = min(part * each, p.ktiles);
+      nk = min(first + each, p.ktiles) - first;
+    }
+  const Place at = place_of<OP>(p, per_matrix, lid);
+  const long b = at.b, i0 = (long)at.ti * kSmall, j0 = (long)at.tj * kSmall;
+  // staging, two slices a round: instruction q of wave w of a group covers rows (w * 2 + q) * 8 + lane / 8 of the group's
+  // slice; LDS chunk lane % 8 holds source chunk (lane % 8) ^ ((row >> 1) & 7), so that 16 rows of a fragment read touch 16
+  // different 16-byte columns.  PAIR: chunks 0 .. 3 are 32 elements of hi, 4 .. 7 the same of lo
+  const _Float16* src[2][2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int row = ((wave & 3) * 2 + q) * 8 + (lane >> 3);
+    const int ch = (lane & 7) ^ ((row >> 1) & 7);
+    const _Float16* hp = PAIR && ch >= 4 ? p.P.lo : p.P.hi;
+    const _Float16* hq = PAIR && ch >= 4 ? p.Q.lo : p.Q.hi;
+    const int k = (PAIR ? ch & 3 : ch) * 8 + first * (PAIR ? 32 : 64);
+    src[0][q] = hp + b * p.P.next + (i0 + row) * p.P.ld + k;
+    src[1][q] = hq + b * p.Q.next + (j0 + row) * p.Q.ld + k;
+  }
+  auto stage = [&](int k) {                 // this group's slice; always four loads, behind the last slice of the last one
+    unsigned char* dst = smem + (k % RING) * kSlice + (wave & 3) * 2048;
+    const long o = (long)max(min(k, nk - 1), 0) * (PAIR ? 32 : 64);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[0][q] + o), (lds_void_ptr)(dst + q * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[1][q] + o), (lds_void_ptr)(dst + kSmall * 128 + q * 1024), 16, 0, 0);
+    }
+  };
+  f32x16_t acc[2];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[0][r] = acc[1][r] = 0.f;
+  // a wave requests RING / 2 - 1 of its group's slices ahead, four loads each, and one more per round: when round k is
+  // waited for, the newer ones may stay in flight
+  const int rounds = (nk + 1) / 2;
+#pragma unroll
+  for (int r = 0; r < RING / 2 - 1; ++r) stage(2 * r + kg);
+  for (int r = 0; r < rounds; ++r) {
+    if constexpr (RING == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();           // round r has landed for every wave; round r - 1 has been read by all ...
+    asm volatile("" ::: "memory");
+    stage(2 * (r + RING / 2 - 1) + kg);     // ... and its slots are free
+    const int k = 2 * r + kg;
+    const unsigned char* base = smem + (k % RING) * kSlice;
+    if (k < nk) {
+      f16x8_t fp[4], fq[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        // PAIR: c = k16 step * 2 + plane, else the k16 step
+        const int ch = (PAIR ? (c & 1) * 4 + (c >> 1) * 2 + lh : c * 2 + lh) ^ ((l31 >> 1) & 7);
+        fp[c] = *reinterpret_cast<const f16x8_t*>(base + (wr * 32 + l31) * 128 + ch * 16);
+        fq[c] = *reinterpret_cast<const f16x8_t*>(base + kSmall * 128 + (wc * 32 + l31) * 128 + ch * 16);
+      }
+      slice_mma<PAIR>(acc, fq, fp);
+    }
+  }
+  // the groups' sums meet: each finishes half of the registers (8 of 16) of its quarter
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // (the requests behind the last slice, too)
+  __syncthreads();
+  float* swap = reinterpret_cast<float*>(smem);                     // [wave][8][64]
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    swap[(wave * 8 + r) * 64 + lane] = kg == 0 ? acc[0][8 + r] + acc[1][8 + r] : acc[0][r] + acc[1][r];
+  }
+  __syncthreads();
+  float sum[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float mine = kg == 0 ? acc[0][r] + acc[1][r] : acc[0][8 + r] + acc[1][8 + r];
+    const float other = swap[((wave ^ 4) * 8 + r) * 64 + lane];
+    sum[r] = kg == 0 ? mine + other : other + mine;
+  }
+  if constexpr (OP == kGram)
+    if (p.splits > 1) {                     // ns_join_kernel goes on from here
+      float* to = p.partial + ((long)lid * p.splits + part) * 4096 + wave * 512 + lane;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) to[r * 64] = sum[r];
+      return;
+    }
+  small_epilogue<OP, T>(p, at, wave, lane, sum);
+}
+
+// adds the parts of a tile in their order
+template <typename T>
+__global__ __launch_bounds__(512) void ns_join_kernel(const Product p, const uint32_t per_matrix) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place at = place_of<kGram>(p, per_matrix, blockIdx.x);
+  const float* from = p.partial + (long)blockIdx.x * p.splits * 4096 + wave * 512 + lane;
+  float sum[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sum[r] = from[r * 64];
+  for (int q = 1; q < p.splits; ++q)
+#pragma unroll
+    for (int r = 0; r < 8; ++r) sum[r] += from[(long)q * 4096 + r * 64];
+  small_epilogue<kGram, T>(p, at, wave, lane, sum);
 }
 
 // ================================================================================ 256 x 256 tiles
@@ -327,7 +402,7 @@ __global__ __launch_bounds__(512, 1) void ns_large_kernel(const Product p, const
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave >> 2, wc = wave & 3;
   const int l31 = lane & 31, lh = lane >> 5;
-  const Place at = place_of<OP>(p, per_matrix);
+  const Place at = place_of<OP>(p, per_matrix, xcd_remap(blockIdx.x, gridDim.x));
   const long b = at.b, m0 = (long)at.ti * kLarge, n0 = (long)at.tj * kLarge;
   const int nk = p.ktiles, nhalf = 4 * nk;
 
@@ -649,16 +724,21 @@ bool ns_use_large(long batch, long m, long n) {
 template <bool PAIR, int OP, typename T>
 void product(const Product& p, long batch, bool large, hipStream_t s) {
   const uint32_t per = OP == kGram || OP == kPoly ? (uint32_t)p.mt * (p.mt + 1) / 2 : (uint32_t)p.mt * p.nt;
-  const long blocks = (long)per * batch;
+  const long blocks = (long)per * batch * (OP == kGram && !large ? p.splits : 1);
   if (blocks >= (1l << 31)) throw std::invalid_argument("newton_schulz: batch too large");
   if (large) hipLaunchKernelGGL((ns_large_kernel<PAIR, OP, T>), dim3((unsigned)blocks), dim3(512), 0, s, p, per);
-  else hipLaunchKernelGGL((ns_small_kernel<PAIR, OP, T>), dim3((unsigned)blocks), dim3(256), 0, s, p, per);
+  else hipLaunchKernelGGL((ns_small_kernel<PAIR, OP, T, OP == kGram || OP == kPoly ? 8 : 4>), dim3((unsigned)blocks), dim3(512), 0, s,
+                          p, per);
+  if constexpr (OP == kGram)
+    if (!large && p.splits > 1) hipLaunchKernelGGL(ns_join_kernel<T>, dim3((unsigned)(per * batch)), dim3(512), 0, s, p, per);
 }
 
 struct Sizes {
   long m, n, mp, np;                        // X: m <= n, padded
   bool large;
+  int splits;                               // of the contraction over n
   size_t x, sq, diag, norm;                 // bytes of one plane of X, of A, of a diagonal, of the partial norms
+  size_t partial;                           // ... of the split sums
 };
 Sizes sizes(long batch, long rows, long cols) {
   Sizes z;
@@ -672,6 +752,13 @@ Sizes sizes(long batch, long rows, long cols) {
   z.sq = (size_t)batch * z.mp * z.mp * 2;
   z.diag = (size_t)batch * z.mp * 4;
   z.norm = (size_t)batch * kNormParts * 8;
+  // a few dozen tiles of a long contraction see one memory latency after the other (60 tiles, 2304 elements: 22 us):
+  // split it until the card has a workgroup per compute unit, 8 slices each at least
+  const long tiles = batch * (z.mp / kSmall) * (z.mp / kSmall + 1) / 2, slices = z.np / 32;
+  z.splits = 1;
+  if (!z.large)
+    while (z.splits < 8 && tiles * (z.splits + 1) <= 256 && slices / (z.splits + 1) >= 8) ++z.splits;
+  z.partial = z.splits > 1 ? (size_t)tiles * z.splits * 4096 * 4 : 0;
   return z;
 }
 
@@ -693,6 +780,7 @@ void run(const NewtonSchulz& q, hipStream_t s) {
   float* Da = reinterpret_cast<float*>(take(z.diag));
   float* Db = reinterpret_cast<float*>(take(z.diag));
   double* norm = reinterpret_cast<double*>(take(z.norm));
+  float* partial = reinterpret_cast<float*>(take(z.partial));
   const T* g = reinterpret_cast<const T*>(q.g);
   hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(kNormParts, (unsigned)q.batch), dim3(256), 0, s, g, q.rows * q.cols, norm);
   hipLaunchKernelGGL(ns_split_kernel<T>, dim3((unsigned)(z.np / 64), (unsigned)(z.mp / 64), (unsigned)q.batch), dim3(256), 0, s,
@@ -704,6 +792,7 @@ void run(const NewtonSchulz& q, hipStream_t s) {
     a.out = a.out_t = A;
     a.diag = Da; a.diag_next = z.mp;
     a.mt = a.nt = (int)(z.mp / tile); a.ktiles = (int)(z.np / slice);
+    a.splits = z.splits; a.partial = partial;
     product<PAIR, kGram, T>(a, q.batch, z.large, s);
     Product b{};                            // B = b A + c A A
     b.P = b.Q = b.R = A;
@@ -732,7 +821,7 @@ void run(const NewtonSchulz& q, hipStream_t s) {
 size_t newton_schulz_workspace(long batch, long rows, long cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) throw std::invalid_argument("newton_schulz: empty shape");
   const Sizes z = sizes(batch, rows, cols);
-  return 6 * z.x + 4 * z.sq + 2 * z.diag + z.norm;
+  return 6 * z.x + 4 * z.sq + 2 * z.diag + z.norm + z.partial;
 }
 
 void newton_schulz_launch(const NewtonSchulz& q, int dtype, hipStream_t s) {
