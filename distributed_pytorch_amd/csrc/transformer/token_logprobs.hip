@@ -20,6 +20,9 @@ namespace {
 
 constexpr int kCap = 1024;         // candidates of one look
 
+// elements of one part of a row, whole chunks
+__host__ __device__ __forceinline__ long part_of(long C, int splits) { return ((C + splits - 1) / splits + 7) & ~7l; }
+
 // order-preserving bits of a float as unsigned (-0 as +0); > 0 for everything but a NaN with the sign bit
 __device__ __forceinline__ uint32_t order_bits(float z) {
   const uint32_t b = __float_as_uint(z + 0.f);
@@ -34,14 +37,19 @@ __device__ __forceinline__ uint64_t make_key(float z, long i) {
 }
 __device__ __forceinline__ long key_index(uint64_t k) { return (long)(0xffffffffu - (uint32_t)k); }
 
-struct RunSums {                    // running maximum m, S and U relative to it
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// running maximum m, S and U relative to it.  m starts at the lowest finite value: a masked class is then exp(-inf) = 0
+// without a case of its own
+constexpr float kLowest = -3.402823466e38f;
+struct RunSums {
   float m, s, u;
-  __device__ __forceinline__ void clear() { m = -INFINITY; s = u = 0.f; }
+  __device__ __forceinline__ void clear() { m = kLowest; s = u = 0.f; }
   __device__ __forceinline__ void raise(float to) {
     if (to > m) {
-      const float d = m - to;
       if (s != 0.f) {               // also where s is NaN
-        const float f = __expf(d);
+        const float d = m - to, f = exp_of(d);
         u = f == 0.f ? 0.f : (u + d * s) * f;        // (d * s may have left the range where f is 0)
         s *= f;
       }
@@ -49,16 +57,24 @@ struct RunSums {                    // running maximum m, S and U relative to it
     }
   }
   __device__ __forceinline__ void add(float z) {
-    const float d = z - m, e = z == -INFINITY ? 0.f : __expf(d);
+    const float d = z - m, e = exp_of(d);
     s += e;
-    u += z == -INFINITY ? 0.f : d * e;
+    u += fmaxf(d, kLowest) * e;     // (-inf times 0 would be NaN; a NaN comes through e)
   }
   __device__ __forceinline__ void join(float m2, float s2, float u2) {
     raise(m2);
     if (s2 != 0.f) {
-      const float d = m2 - m, f = d == 0.f ? 1.f : __expf(d);
+      const float d = m2 - m, f = d == 0.f ? 1.f : exp_of(d);
       s += s2 * f;
       u += f == 0.f ? 0.f : (d == 0.f ? u2 : (u2 + d * s2)) * f;
+    }
+  }
+  // all 64 lanes' sums, the same in every lane
+  __device__ __forceinline__ void join_wave() {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), u2 = __shfl_xor(u, o, 64);
+      join(m2, s2, u2);
     }
   }
 };
@@ -69,130 +85,258 @@ template <typename T> __device__ __forceinline__ Vec16<T> load_any(const T* p) {
   __builtin_memcpy(&v.raw, p, 16);
   return v;
 }
-template <typename T> __device__ __forceinline__ void store_any(const Vec16<T>& v, T* p) { __builtin_memcpy(p, &v.raw, 16); }
-
-// elements [lo, hi) of a row, lo a multiple of a chunk: a lane takes every 256th chunk of 16 bytes, whatever the row's
-// alignment (results do not depend on it).  F(z, i) sees one element, M(largest of the next few) comes before them
-template <typename T, typename F, typename M>
-__device__ __forceinline__ void scan_row(const T* z, long lo, long hi, F f, M before) {
-  constexpr int V = 16 / (int)sizeof(T);
-  for (long c = lo + (long)threadIdx.x * V; c < hi; c += (long)blockDim.x * V) {
-    if (c + V <= hi) {
-      const Vec16<T> v = load_any(z + c);
-      float mx = v.get(0);
-#pragma unroll
-      for (int j = 1; j < V; ++j) mx = fmaxf(mx, v.get(j));
-      before(mx);
-#pragma unroll
-      for (int j = 0; j < V; ++j) f(v.get(j), c + j);
-    } else {
-      for (long i = c; i < hi; ++i) {
-        const float v = to_float(z[i]);
-        before(v);
-        f(v, i);
-      }
-    }
-  }
+typedef uint32_t any128 __attribute__((ext_vector_type(4), aligned(2)));
+// `stream`: not kept in the caches (the gradient of a vocabulary is larger than they are: 117 -> 103 us for 2048 x 50257)
+template <typename T> __device__ __forceinline__ void store_any(const Vec16<T>& v, T* p, bool stream) {
+  const any128 x = {v.raw.x, v.raw.y, v.raw.z, v.raw.w};
+  if (stream) __builtin_nontemporal_store(x, reinterpret_cast<any128*>(p));
+  else *reinterpret_cast<any128*>(p) = x;
 }
 
-struct TopShared {
-  uint64_t best[256];
+template <typename T> __device__ __forceinline__ float chunk_max(const Vec16<T>& v) {
+  float mx = v.get(0);
+#pragma unroll
+  for (int j = 1; j < Vec16<T>::N; ++j) mx = fmaxf(mx, v.get(j));
+  return mx;
+}
+// chunk q of a row's elements [lo, hi), lo a multiple of a chunk; -inf behind the end.  A lane takes every blockDim-th chunk
+// whatever the row's alignment: results do not depend on it
+template <typename T> __device__ __forceinline__ Vec16<T> load_chunk(const T* z, int c, int hi) {
+  if (c + Vec16<T>::N <= hi) return load_any(z + c);
+  Vec16<T> v;
+#pragma unroll
+  for (int j = 0; j < Vec16<T>::N; ++j) v.set(j, c + j < hi ? to_float(z[c + j]) : -INFINITY);
+  return v;
+}
+
+// f(chunk, first column) for the lane's chunks of [lo, hi), four requested at a time
+template <typename T, int TH, typename F>
+__device__ __forceinline__ void walk(const T* z, int lo, int hi, F f) {
+  constexpr int V = Vec16<T>::N, U = 4, kStep = TH * V;
+  int c = lo + (int)threadIdx.x * V;
+  for (; c + (U - 1) * kStep + V <= hi; c += U * kStep) {
+    Vec16<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = load_any(z + c + u * kStep);
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(v[u], c + u * kStep);
+  }
+  for (; c < hi; c += kStep) f(load_chunk(z, c, hi), c);
+}
+
+// Makes a chunk a new value to the compiler: it would otherwise keep the floats of one pass over the registers for the next
+// one, and spill hundreds of them.
+template <typename T> __device__ __forceinline__ void forget(Vec16<T>& v) {
+  asm volatile("" : "+v"(v.raw.x), "+v"(v.raw.y), "+v"(v.raw.z), "+v"(v.raw.w));
+}
+
+template <int TH> struct TopShared {
+  uint64_t best[TH];
   uint64_t cand[kCap];
   uint64_t bound;
   int count;
 };
 
-// the k largest of the candidates, by the count of larger ones, to out[0 .. k) (0 where there are fewer)
-__device__ __forceinline__ void rank_out(const TopShared& sh, int n, int k, uint64_t* out) {
+// how many of keys[0 .. n) are larger than `mine`: sixteen reads in flight (one after the other, each waits for LDS: a count
+// over 256 keys took 3.6 us)
+__device__ __forceinline__ int count_larger(const uint64_t* keys, int n, uint64_t mine) {
+  int r = 0, j = 0;
+  for (; j + 16 <= n; j += 16) {
+    uint64_t v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) v[u] = keys[j + u];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) r += v[u] > mine ? 1 : 0;
+  }
+  for (; j < n; ++j) r += keys[j] > mine ? 1 : 0;
+  return r;
+}
+
+// keys of the candidates in descending order: out[r] for r < k (0 where there are fewer)
+__device__ __forceinline__ void rank_out(const uint64_t* cand, int n, int k, uint64_t* out) {
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const uint64_t mine = sh.cand[i];
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += sh.cand[j] > mine ? 1 : 0;
+    const uint64_t mine = cand[i];
+    const int r = count_larger(cand, n, mine);
     if (r < k) out[r] = mine;
   }
   for (int i = n + threadIdx.x; i < k; i += blockDim.x) out[i] = 0;
 }
 
-// the k largest keys of [lo, hi) in descending order to out (LDS or global); `best`: this lane's largest key
-template <typename T>
-__device__ __forceinline__ void top_of(const T* z, long lo, long hi, int k, uint64_t best, TopShared& sh, uint64_t* out) {
+// The k largest keys in descending order to out (LDS or global).  `best`: the largest key that this lane has seen;
+// `each(least, f)` calls f(chunk, first column) for the lane's
+// chunks with an element that is not below `least`, and others at will; `hi`: end of the row.  `plain`: there is no NaN, so a chunk
+// whose largest element is below the bound has nothing to offer (fmaxf passes over NaN)
+template <typename T, int TH, typename E>
+__device__ __forceinline__ void top_of(int k, int hi, uint64_t best, bool plain, TopShared<TH>& sh, uint64_t* out, E each) {
   sh.best[threadIdx.x] = best;
   if (threadIdx.x == 0) { sh.bound = 0; sh.count = 0; }
   __syncthreads();
   {
-    int r = 0;
-    for (int j = 0; j < 256; ++j) r += sh.best[j] > best ? 1 : 0;
+    const int r = count_larger(sh.best, TH, best);
     // with fewer than k lanes that saw anything the bound stays 0 and every element is a candidate (few, then)
     if (best != 0 && r == k - 1) sh.bound = best;
   }
   __syncthreads();
   for (;;) {
     const uint64_t bound = sh.bound;
-    scan_row(z, lo, hi, [&](float v, long i) {
-      const uint64_t key = make_key(v, i);
-      if (key >= bound) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kCap) sh.cand[at] = key;
+    const float least = plain && bound != 0 ? order_value((uint32_t)(bound >> 32)) : -INFINITY;
+    each(least, [&](const Vec16<T>& v, int c) {
+      if (chunk_max(v) < least) return;
+#pragma unroll
+      for (int j = 0; j < Vec16<T>::N; ++j) {
+        const uint64_t key = make_key(v.get(j), c + j);
+        if (key >= bound && c + j < hi) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCap) sh.cand[at] = key;
+        }
       }
-    }, [](float) {});
+    });
     __syncthreads();
     const int n = sh.count;
     if (n <= kCap) {
-      rank_out(sh, n, k, out);
+      rank_out(sh.cand, n, k, out);
       return;
     }
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
-    for (int i = threadIdx.x; i < kCap; i += blockDim.x) {
+    for (int i = threadIdx.x; i < kCap; i += TH) {
       const uint64_t mine = sh.cand[i];
-      int r = 0;
-      for (int j = 0; j < kCap; ++j) r += sh.cand[j] > mine ? 1 : 0;
-      if (r == k - 1) sh.bound = mine;
+      if (count_larger(sh.cand, kCap, mine) == k - 1) sh.bound = mine;
     }
     __syncthreads();
   }
 }
 
-__device__ __forceinline__ void write_row(const TokenLogprobs& p, long row, const RunSums& a, float zt, bool valid) {
+// the row's results from its sums and (k > 0) its first keys
+template <typename T>
+__device__ __forceinline__ void write_row(const TokenLogprobs& p, long row, bool valid, float zt, const RunSums& a,
+                                          const uint64_t* top) {
   const float ls = logf(a.s);
   const bool empty = a.s == 0.f;                   // every class is masked
-  p.norm[2 * row] = a.m;
-  p.norm[2 * row + 1] = ls;
-  p.logprob[row] = valid ? (empty ? -INFINITY : (zt - a.m) - ls) : 0.f;
-  p.entropy[row] = empty ? 0.f : ls - a.u / a.s;
+  if (threadIdx.x == 0) {
+    p.norm[2 * row] = a.m;
+    p.norm[2 * row + 1] = ls;
+    p.logprob[row] = valid ? (empty ? -INFINITY : (zt - a.m) - ls) : 0.f;
+    p.entropy[row] = empty ? 0.f : ls - a.u / a.s;
+  }
+  for (int i = threadIdx.x; i < p.k; i += blockDim.x) {
+    const uint64_t key = top[i];
+    p.index[row * p.k + i] = key_index(key);
+    p.top[row * p.k + i] = empty ? -INFINITY : (order_value((uint32_t)(key >> 32)) - a.m) - ls;
+  }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(const TokenLogprobs p) {
-  __shared__ float wm[4], ws[4], wu[4];
-  __shared__ TopShared sh;
+// One workgroup of TH lanes per row, or per part of a row.  Q > 0: the part is at most Q chunks a lane and stays in registers
+// (one read; the exact maximum comes first).  Q = 0: any length, a second look comes from cache.
+template <typename T, int TH, int Q>
+__global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs p) {
+  constexpr int V = Vec16<T>::N;
+  __shared__ float wm[TH / 64], ws[TH / 64], wu[TH / 64];
+  __shared__ TopShared<TH> sh;
   __shared__ uint64_t top[kTokenTopMax];
   const long row = blockIdx.x / p.splits;
   const int part = (int)(blockIdx.x - row * p.splits);
   const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ld;
-  const long each = ((p.C + p.splits - 1) / p.splits + 7) & ~7l;
-  const long lo = min(part * each, p.C), hi = min(lo + each, p.C);
+  const long each = part_of(p.C, p.splits);
+  const int lo = (int)min(part * each, p.C), hi = (int)min(lo + each, p.C);
+  const int c0 = (int)lo + (int)threadIdx.x * V;
+  const long t = p.target[row];                    // (early: two loads that follow each other)
+  const bool valid = t >= 0 && t < p.C;
+  const float zt = valid ? to_float(z[t]) : 0.f;
+  Vec16<T> v[Q > 0 ? Q : 1];
   RunSums a;
   a.clear();
-  uint64_t best = 0;
-  scan_row(z, lo, hi,
-           [&](float v, long i) {
-             a.add(v);
-             const uint64_t key = make_key(v, i);
-             best = key > best ? key : best;
-           },
-           [&](float mx) { a.raise(mx); });
-  // lanes, then waves, in a fixed order
+  int where = c0;                                 // chunk with this lane's largest element
+  // Q = 0: the lane's two largest chunk maxima, where they are, and the largest of its other chunks: the second look needs
+  // two chunks of a lane at most, unless a third one reaches the bound as well
+  float first = -INFINITY, second = -INFINITY, third = -INFINITY;
+  int where2 = c0;
+  if constexpr (Q > 0) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor(a.m, o, 64), s2 = __shfl_xor(a.s, o, 64), u2 = __shfl_xor(a.u, o, 64);
-    a.join(m2, s2, u2);
+    for (int q = 0; q < Q; ++q) {
+      const int c = c0 + q * TH * V;
+      if (c < hi) v[q] = load_chunk(z, c, hi);
+    }
+    float largest = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int c = c0 + q * TH * V;
+      if (c < hi) {
+        const float mx = chunk_max(v[q]);
+        if (mx > largest) { largest = mx; where = c; }
+      }
+    }
+    a.m = fmaxf(largest, kLowest);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (c0 + q * TH * V < hi) {
+        forget(v[q]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) a.add(v[q].get(j));
+      }
+  } else {
+    walk<T, TH>(z, (int)lo, (int)hi, [&](const Vec16<T>& x, int c) {
+      const float mx = chunk_max(x);
+      if (mx > first) {
+        third = second;
+        second = first;
+        where2 = where;
+        first = mx;
+        where = c;
+      } else if (mx > second) {
+        third = second;
+        second = mx;
+        where2 = c;
+      } else {
+        third = fmaxf(third, mx);
+      }
+      a.raise(mx);
+#pragma unroll
+      for (int j = 0; j < V; ++j) a.add(x.get(j));
+    });
   }
-  if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; wm[w] = a.m; ws[w] = a.s; wu[w] = a.u; }
-  __syncthreads();
-  a.clear();
-  for (int w = 0; w < 4; ++w) a.join(wm[w], ws[w], wu[w]);
-  if (p.k > 0) top_of(z, lo, hi, p.k, best, sh, p.splits == 1 ? top : p.keys + (long)blockIdx.x * p.k);
+  // lanes, then waves, in a fixed order
+  a.join_wave();
+  if constexpr (TH > 64) {
+    if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; wm[w] = a.m; ws[w] = a.s; wu[w] = a.u; }
+    __syncthreads();
+    a.clear();
+    for (int w = 0; w < TH / 64; ++w) a.join(wm[w], ws[w], wu[w]);
+  }
+  if (p.k > 0) {
+    uint64_t best = 0;
+    if (c0 < hi) {
+      const Vec16<T> b = load_chunk(z, where, hi);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (where + j < hi) {
+          const uint64_t key = make_key(b.get(j), where + j);
+          best = key > best ? key : best;
+        }
+    }
+    const bool plain = a.s == a.s;
+    uint64_t* out = p.splits == 1 ? top : p.keys + (long)blockIdx.x * p.k;
+    if constexpr (Q > 0)
+      top_of<T, TH>(p.k, hi, best, plain, sh, out, [&](float, auto f) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int c = c0 + q * TH * V;
+          if (c < hi) {
+            forget(v[q]);
+            f(v[q], c);
+          }
+        }
+      });
+    else
+      top_of<T, TH>(p.k, hi, best, plain, sh, out, [&](float least, auto f) {
+        if (third >= least || least == -INFINITY) {
+          walk<T, TH>(z, (int)lo, (int)hi, f);
+        } else {
+          if (first >= least) f(load_chunk(z, where, hi), where);
+          if (second >= least) f(load_chunk(z, where2, hi), where2);
+        }
+      });
+  }
   if (p.splits > 1) {
     if (threadIdx.x == 0) {
       float* st = p.stat + (long)blockIdx.x * 3;
@@ -201,58 +345,39 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const TokenLogprobs
     return;
   }
   __syncthreads();
-  const long t = p.target[row];
-  const bool valid = t >= 0 && t < p.C;
-  if (threadIdx.x == 0) write_row(p, row, a, valid ? to_float(z[t]) : 0.f, valid);
-  const float ls = logf(a.s);
-  if ((int)threadIdx.x < p.k) {
-    const uint64_t key = top[threadIdx.x];
-    p.index[row * p.k + threadIdx.x] = key_index(key);
-    p.top[row * p.k + threadIdx.x] = a.s == 0.f ? -INFINITY : (order_value((uint32_t)(key >> 32)) - a.m) - ls;
-  }
+  write_row<T>(p, row, valid, zt, a, top);
 }
 
-// joins the parts of a row: one workgroup per row
+// joins the parts of a row: one workgroup per row, a lane per key where there are many
+constexpr int kJoin = 512;
 template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_join_kernel(const TokenLogprobs p) {
-  __shared__ TopShared sh;
+__global__ __launch_bounds__(kJoin) void token_logprobs_join_kernel(const TokenLogprobs p) {
+  __shared__ uint64_t cand[kCap];
   __shared__ uint64_t top[kTokenTopMax];
   const long row = blockIdx.x;
-  const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ld;
+  const long t = p.target[row];                    // (early: two loads that follow each other)
+  const bool valid = t >= 0 && t < p.C;
+  const float zt = valid ? to_float(reinterpret_cast<const T*>(p.logits)[row * p.ld + t]) : 0.f;
+  const int n = p.splits * p.k;                    // at most kCap
+  for (int i = threadIdx.x; i < n; i += kJoin) cand[i] = p.keys[row * n + i];
   RunSums a;
   a.clear();
-  for (int q = 0; q < p.splits; ++q) {
-    const float* st = p.stat + (row * p.splits + q) * 3;
-    a.join(st[0], st[1], st[2]);
+  const int lane = threadIdx.x & 63;               // (at most 64 parts, one a lane)
+  if (lane < p.splits) {
+    const float* st = p.stat + (row * p.splits + lane) * 3;
+    a.m = st[0]; a.s = st[1]; a.u = st[2];
   }
-  if (p.k > 0) {
-    // splits * k keys, at most kCap (token_logprobs_splits)
-    const int n = p.splits * p.k;
-    for (int i = threadIdx.x; i < n; i += 256) sh.cand[i] = p.keys[row * n + i];
-    __syncthreads();
-    // an absent key (0) is below all others and never among the first k of C >= k elements
-    for (int i = threadIdx.x; i < n; i += 256) {
-      const uint64_t mine = sh.cand[i];
-      int r = 0;
-      for (int j = 0; j < n; ++j) r += sh.cand[j] > mine ? 1 : 0;
-      if (mine != 0 && r < p.k) top[r] = mine;
-    }
-    __syncthreads();
-  }
-  const long t = p.target[row];
-  const bool valid = t >= 0 && t < p.C;
-  if (threadIdx.x == 0) write_row(p, row, a, valid ? to_float(z[t]) : 0.f, valid);
-  const float ls = logf(a.s);
-  if ((int)threadIdx.x < p.k) {
-    const uint64_t key = top[threadIdx.x];
-    p.index[row * p.k + threadIdx.x] = key_index(key);
-    p.top[row * p.k + threadIdx.x] = a.s == 0.f ? -INFINITY : (order_value((uint32_t)(key >> 32)) - a.m) - ls;
-  }
+  a.join_wave();
+  __syncthreads();
+  // (an absent key, 0, is below all others and never among the first k of C >= k elements)
+  rank_out(cand, n, p.k, top);
+  __syncthreads();
+  write_row<T>(p, row, valid, zt, a, top);
 }
 
 // one part of a row; elements that carry a gradient of their own are found through a bit per 8 columns
 template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogprobsBwd p, const int splits) {
+__global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogprobsBwd p, const int splits, const bool stream) {
   constexpr int V = 16 / (int)sizeof(T);
   __shared__ uint32_t marked[1024];
   __shared__ long idx[kTokenTopMax + 1];
@@ -261,8 +386,8 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogp
   const int part = (int)(blockIdx.x - row * splits);
   const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ld;
   T* dz = reinterpret_cast<T*>(p.dlogits) + row * p.C;
-  const long each = ((p.C + splits - 1) / splits + 7) & ~7l;
-  const long lo = min(part * each, p.C), hi = min(lo + each, p.C);
+  const long each = part_of(p.C, splits);
+  const int lo = (int)min(part * each, p.C), hi = (int)min(lo + each, p.C);
   for (int i = threadIdx.x; i < 1024; i += 256) marked[i] = 0;
   const long t = p.target[row];
   const bool valid = t >= 0 && t < p.C;
@@ -283,32 +408,55 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogp
   }
   __syncthreads();
   const float m = p.norm[2 * row], ls = p.norm[2 * row + 1], H = p.entropy[row];
-  const bool empty = ls == -INFINITY;
-  auto grad = [&](float v, long i) {
-    if (empty) return 0.f;
-    const float logp = (v - m) - ls, pr = __expf(logp);
-    float g = -pr * gsum;
-    if (ge != 0.f) g -= v == -INFINITY ? 0.f : ge * pr * (logp + H);
-    const uint32_t bit = (uint32_t)((i >> 3) & 32767);
-    if ((marked[bit >> 5] >> (bit & 31)) & 1u)
-      for (int j = 0; j <= k; ++j) g += idx[j] == i ? gx[j] : 0.f;
-    return g;
-  };
-  for (long c = lo + (long)threadIdx.x * V; c < hi; c += 256 * V) {
-    if (c + V <= hi) {
-      const Vec16<T> v = load_any(z + c);
-      Vec16<T> o;
+  const bool empty = ls == -INFINITY;              // a row that is masked altogether
+  // p (-gsum - ge (log p + H)) with log p = d - ls, d = z - m; where p is 0 d is kept finite
+  const float c0 = -gsum - ge * H + ge * ls, shift = -ls * kLog2e;
+  auto chunk = [&](const Vec16<T>& v, int c) {
+    float g[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) o.set(j, grad(v.get(j), c + j));
-      store_any(o, dz + c);
+    for (int j = 0; j < V; ++j) {
+      const float d = v.get(j) - m;
+      g[j] = __builtin_amdgcn_exp2f(fmaf(d, kLog2e, shift)) * fmaf(-ge, fmaxf(d, -1e30f), c0);
+    }
+    const uint32_t bit = (uint32_t)((c >> 3) & 32767);         // (a chunk lies within 8 columns)
+    if ((marked[bit >> 5] >> (bit & 31)) & 1u)
+      for (int i = 0; i <= k; ++i) {
+        const long at = idx[i] - c;
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] += at == j ? gx[i] : 0.f;
+      }
+    Vec16<T> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.set(j, g[j]);
+    return o;
+  };
+  constexpr int U = 4, kStep = 256 * V;            // chunks in flight per lane
+  int c = lo + (int)threadIdx.x * V;
+  if (empty) {
+    for (int i = lo + (int)threadIdx.x; i < hi; i += 256) dz[i] = from_float<T>(0.f);
+    return;
+  }
+  for (; c + (U - 1) * kStep + V <= hi; c += U * kStep) {
+    Vec16<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = load_any(z + c + u * kStep);
+#pragma unroll
+    for (int u = 0; u < U; ++u) store_any(chunk(v[u], c + u * kStep), dz + c + u * kStep, stream);
+  }
+  for (; c < hi; c += kStep) {
+    const Vec16<T> o = chunk(load_chunk(z, c, hi), c);
+    if (c + V <= hi) {
+      store_any(o, dz + c, stream);
     } else {
-      for (long i = c; i < hi; ++i) dz[i] = from_float<T>(grad(to_float(z[i]), i));
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c + j < hi) dz[c + j] = from_float<T>(o.get(j));
     }
   }
 }
 
 void check(long N, long C, int k) {
-  if (N < 0 || C <= 0 || C >= (1l << 31)) throw std::invalid_argument("token_logprobs: 1 .. 2^31 - 1 classes");
+  if (N < 0 || C <= 0 || C > (1l << 30)) throw std::invalid_argument("token_logprobs: 1 .. 2^30 classes");
   if (k < 0 || k > kTokenTopMax || k > C) throw std::invalid_argument("token_logprobs: k must be 0 .. min(64, classes)");
 }
 
@@ -327,9 +475,16 @@ void token_logprobs_launch(const TokenLogprobs& p, int dtype, hipStream_t s) {
   if (p.N == 0) return;
   if (p.splits < 1 || p.splits * p.k > kCap || p.N * p.splits >= (1l << 31))
     throw std::invalid_argument("token_logprobs: splits");
+  const long part = part_of(p.C, p.splits) < p.C ? part_of(p.C, p.splits) : p.C;
+  const dim3 grid((unsigned)(p.N * p.splits));
+  // one wave per row up to 256 chunks (1024 classes in fp32), a workgroup up to 2048 chunks in registers, else two looks
+  // (16 chunks a lane spill)
   DPA_DISPATCH_DTYPE(dtype, {
-    hipLaunchKernelGGL(token_logprobs_kernel<T>, dim3((unsigned)(p.N * p.splits)), dim3(256), 0, s, p);
-    if (p.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((unsigned)p.N), dim3(256), 0, s, p);
+    const long chunks = (part + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (chunks <= 64 * 4) hipLaunchKernelGGL((token_logprobs_kernel<T, 64, 4>), grid, dim3(64), 0, s, p);
+    else if (chunks <= 256 * 8) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 8>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 0>), grid, dim3(256), 0, s, p);
+    if (p.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((unsigned)p.N), dim3(kJoin), 0, s, p);
   });
   DPA_CHECK_HIP(hipGetLastError());
 }
@@ -342,7 +497,7 @@ void token_logprobs_bwd_launch(const TokenLogprobsBwd& p, int dtype, hipStream_t
   if (splits < 1) splits = 1;
   if (p.N * splits >= (1l << 31)) throw std::invalid_argument("token_logprobs: too many rows");
   DPA_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(token_logprobs_bwd_kernel<T>, dim3((unsigned)(p.N * splits)), dim3(256), 0, s, p,
-                                               (int)splits));
+                                               (int)splits, p.N * p.C * (long)sizeof(T) >= (32l << 20)));
   DPA_CHECK_HIP(hipGetLastError());
 }
 

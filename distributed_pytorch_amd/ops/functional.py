@@ -582,6 +582,8 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, k: int = 0):
     if target.device != logits.device:
         raise ValueError("token_logprobs: target must be on the logits' device")
     V = logits.shape[-1]
+    if V > 1 << 30:
+        raise ValueError("token_logprobs: at most 2^30 classes")
     if not 0 <= k <= min(64, V):
         raise ValueError("token_logprobs: k must be 0 .. min(64, V), got %r" % (k,))
     lead = target.shape
