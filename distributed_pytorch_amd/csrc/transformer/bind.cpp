@@ -176,7 +176,9 @@ struct ResidualNormFn : Function<ResidualNormFn> {
     const bool plain = cfg[0] == kNormNone && gate_kind == kGateNone && !v[5].defined();
     const bool branch = !plain && (need_y || need[2] || need[3] || need[4]);
     Tensor dx, dy;
-    if (need_x || (need_y && plain)) dx = at::empty_like(ref);
+    // without `pre` the sum's gradient is x's as it stands
+    const bool same = cfg[1] == kNormNone && ds.defined();
+    if (need_x || (need_y && plain)) dx = same ? ds : at::empty_like(ref);
     if (branch) dy = at::empty_like(ref);
 
     ResidualNormBwd p;
@@ -212,14 +214,14 @@ struct ResidualNormFn : Function<ResidualNormFn> {
       if (sums) partial = floats({parts, 5, r.C}, ref);
       if (gate_sums) gate_partial = floats({ref.size(0) * splits, r.C}, ref);
       p.ds = data<void>(ds); p.dh = data<void>(dh); p.x = data<void>(x); p.y = data<void>(y);
-      p.dx = data<void>(dx); p.dy = data<void>(dy);
+      p.dx = same ? nullptr : data<void>(dx); p.dy = data<void>(dy);
       p.post_w = data<float>(v[0]); p.post_b = data<float>(v[1]); p.pre_w = data<float>(v[2]);
       p.gate = data<float>(v[4]); p.scale = data<float>(v[5]);
       p.post_stat = data<float>(sv[2]); p.pre_stat = data<float>(sv[3]);
       p.partial = data<float>(partial); p.gate_partial = data<float>(gate_partial); p.dgate_sample = data<float>(dgate);
       p.rows = r.rows; p.per_sample = r.per_sample; p.C = r.C;
       p.post = (int)cfg[0]; p.pre = (int)cfg[1]; p.gate_kind = gate_kind;
-      residual_norm_bwd_launch(p, code(ref), stream_of(ref));
+      if (p.dx != nullptr || p.dy != nullptr || sums || gate_sums) residual_norm_bwd_launch(p, code(ref), stream_of(ref));
     } else {                                    // no rows: every sum is zero
       for (int i = 0; i < 5; ++i) {
         if (own[i].defined()) own[i].zero_();

@@ -50,11 +50,12 @@ __device__ __forceinline__ void row_stats(const float (&v)[R][MAXCH][kV<T>], int
 }
 
 template <typename T, int MAXCH, int R, bool WIDE, bool VEC>
-__global__ __launch_bounds__(256) void residual_norm_fwd_kernel(const ResidualNormFwd p, const int G,
+__global__ __launch_bounds__(WIDE ? 512 : 256) void residual_norm_fwd_kernel(const ResidualNormFwd p, const int G,
                                                                 const FastDiv by_sample) {
   constexpr int V = kV<T>;
-  __shared__ float red[WIDE ? 2 * R * 4 : 1];
+  __shared__ __attribute__((aligned(16))) float red[WIDE ? 2 * R * kMaxWaves : 4];
   GroupSum<WIDE, R> gs{red};
+  gs.clear();
   const int lane = threadIdx.x & 63;
   const int gl = WIDE ? threadIdx.x : (lane & (G - 1));
   const int rpw = WIDE ? 1 : 64 / G;
@@ -180,9 +181,9 @@ void launch(const ResidualNormFwd& p, const Plan& pl, bool vec, hipStream_t s) {
   const unsigned blocks = (unsigned)(trips < 2048 ? trips : 2048);
   const FastDiv by_sample = make_fastdiv((uint32_t)p.per_sample);
   if (vec)
-    hipLaunchKernelGGL((residual_norm_fwd_kernel<T, MAXCH, R, WIDE, true>), dim3(blocks), dim3(256), 0, s, p, pl.G, by_sample);
+    hipLaunchKernelGGL((residual_norm_fwd_kernel<T, MAXCH, R, WIDE, true>), dim3(blocks), dim3(pl.threads), 0, s, p, pl.G, by_sample);
   else
-    hipLaunchKernelGGL((residual_norm_fwd_kernel<T, MAXCH, R, WIDE, false>), dim3(blocks), dim3(256), 0, s, p, pl.G, by_sample);
+    hipLaunchKernelGGL((residual_norm_fwd_kernel<T, MAXCH, R, WIDE, false>), dim3(blocks), dim3(pl.threads), 0, s, p, pl.G, by_sample);
 }
 
 }  // namespace
@@ -202,8 +203,7 @@ void residual_norm_fwd_launch(const ResidualNormFwd& p, int dtype, hipStream_t s
     else if (!pl.wide) launch<T, 2, 1, false>(p, pl, vec, s);
     else if (pl.maxch == 1) launch<T, 1, 1, true>(p, pl, vec, s);
     else if (pl.maxch == 2) launch<T, 2, 1, true>(p, pl, vec, s);
-    else if (pl.maxch == 4) launch<T, 4, 1, true>(p, pl, vec, s);
-    else launch<T, 8, 1, true>(p, pl, vec, s);
+    else launch<T, 4, 1, true>(p, pl, vec, s);
   });
   DPA_CHECK_HIP(hipGetLastError());
 }

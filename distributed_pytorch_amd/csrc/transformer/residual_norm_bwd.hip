@@ -58,14 +58,15 @@ __device__ __forceinline__ void merge_out(float (&v)[MAXCH][kV<T>], float* out, 
 }
 
 template <typename T, int MAXCH, bool WIDE, bool VEC, int MODE>
-__global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNormBwd p, const int G, const long units,
+__global__ __launch_bounds__(WIDE ? 512 : 256) void residual_norm_bwd_kernel(const ResidualNormBwd p, const int G, const long units,
                                                                 const long unit_rows, const int splits,
                                                                 const FastDiv by_sample) {
   constexpr int V = kV<T>;
   constexpr bool PRE = MODE != kPostOnly, POST = MODE != kPreOnly;
-  __shared__ float red[WIDE ? 16 : 1];
+  __shared__ __attribute__((aligned(16))) float red[WIDE ? 4 * kMaxWaves : 4];
   __shared__ float lds[WIDE ? 1 : 4 * MAXCH * 64 * V];
   GroupSum<WIDE, 2> gsum{red};
+  gsum.clear();
   const int lane = threadIdx.x & 63;
   const int gl = WIDE ? threadIdx.x : (lane & (G - 1));
   const int rpw = WIDE ? 1 : 64 / G;
@@ -92,6 +93,48 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNo
   };
   clear(a_prew); clear(a_preb); clear(a_postw); clear(a_postb); clear(a_gate);
 
+  // the lane's channels never change: their parameters stay in registers (chunks of a wide lane are read again per row)
+  constexpr bool HOIST = MAXCH <= 2;
+  constexpr int HM = HOIST ? MAXCH : 1;
+  float pre_w[PRE ? HM : 1][V], post_w[POST ? HM : 1][V], post_b[MODE == kAll ? HM : 1][V], gate_v[MODE == kAll ? HM : 1][V];
+  if constexpr (HOIST)
+#pragma unroll
+    for (int k = 0; k < MAXCH; ++k) {
+      if constexpr (PRE) load_vec<V, VEC>(p.pre_w, gl + k * G, C, 1.f, pre_w[k]);
+      if constexpr (POST) load_vec<V, VEC>(p.post_w, gl + k * G, C, 1.f, post_w[k]);
+      if constexpr (MODE == kAll) load_vec<V, VEC>(p.post_b, gl + k * G, C, 0.f, post_b[k]);
+      if constexpr (MODE == kAll) load_vec<V, VEC>(p.gate_kind == kGateChannel ? p.gate : nullptr, gl + k * G, C, 1.f, gate_v[k]);
+    }
+  struct Row {
+    Vec16<T> ds[MAXCH], dh[PRE ? MAXCH : 1], x[PRE ? MAXCH : 1], y[MAXCH];
+    float mean, rstd, ymean, yrstd, sc;
+  };
+  const auto request = [&](Row& r, long base, long hi) {
+    const long row = base + (WIDE ? 0 : lane / G);
+    const bool live = row < hi;
+    const int Cr = live ? C : 0;                         // a dead row has no elements
+    const long at = live ? row * C : 0;
+    r.mean = r.rstd = r.ymean = r.yrstd = 0.f;
+    r.sc = 1.f;
+    if (live) {
+      if (has_pre) { r.mean = p.pre_stat[row]; r.rstd = p.pre_stat[p.rows + row]; }
+      if (has_post) { r.ymean = p.post_stat[row]; r.yrstd = p.post_stat[p.rows + row]; }
+      if (MODE != kPreOnly && p.scale != nullptr) r.sc = p.scale[fdiv((uint32_t)row, by_sample)];
+    }
+#pragma unroll
+    for (int k = 0; k < MAXCH; ++k) {
+      if (ds_in != nullptr) r.ds[k] = load_chunk<T, VEC>(ds_in + at, gl + k * G, Cr);
+      else r.ds[k].raw = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (PRE)
+        if (has_pre) {
+          r.dh[k] = load_chunk<T, VEC>(dh_in + at, gl + k * G, Cr);
+          r.x[k] = load_chunk<T, VEC>(x_in + at, gl + k * G, Cr);
+        }
+      if (y_in != nullptr) r.y[k] = load_chunk<T, VEC>(y_in + at, gl + k * G, Cr);
+      else r.y[k].raw = make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+
   for (long u = blockIdx.x; u < units; u += gridDim.x) {
     // rows of this unit: a part of one sample where the gate is per sample, else a part of all rows
     long lo, hi;
@@ -99,71 +142,70 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNo
       const long n = u / splits, part = u - n * splits;
       lo = n * p.per_sample + part * unit_rows;
       hi = min(lo + unit_rows, (n + 1) * p.per_sample);
+      if constexpr (HOIST && MODE == kAll)
+#pragma unroll
+        for (int k = 0; k < MAXCH; ++k) load_vec<V, VEC>(p.gate + n * C, gl + k * G, C, 1.f, gate_v[k]);
     } else {
       lo = u * unit_rows;
       hi = min(lo + unit_rows, p.rows);
     }
+    // the next row is requested before this one is worked on: with one row in flight a workgroup waits for memory and
+    // for its sums in turn (24 x 257 x 1280 fp32: 70 us)
+    constexpr bool AHEAD = MAXCH == 1;
+    Row cur;
+    if (AHEAD && lo + grp * rpw < hi) request(cur, lo + grp * rpw, hi);
     for (long base = lo + grp * rpw; base < hi; base += groups * rpw) {
       const long row = base + (WIDE ? 0 : lane / G);
       const bool live = row < hi;
-      const int Cr = live ? C : 0;
-      const long at = live ? row * C : 0;
-      Vec16<T> dsv[MAXCH], dhv[PRE ? MAXCH : 1], xv[PRE ? MAXCH : 1], yv[MAXCH];
+      if constexpr (!AHEAD) request(cur, base, hi);
+      Row next;
+      if (AHEAD && base + groups * rpw < hi) request(next, base + groups * rpw, hi);
+      const float sc = cur.sc, ymean = cur.ymean, yrstd = cur.yrstd;
+      const float* gate = p.gate;
+      if (!HOIST && p.gate_kind == kGateSample) gate += (long)fdiv((uint32_t)(live ? row : 0), by_sample) * C;
+      // parameters of chunk k
+      const auto param = [&](const float* from, const float (&kept)[V], int k, float absent, float (&r)[V]) {
+        if constexpr (HOIST) {
 #pragma unroll
-      for (int k = 0; k < MAXCH; ++k) {
-        if (ds_in != nullptr) dsv[k] = load_chunk<T, VEC>(ds_in + at, gl + k * G, Cr);
-        else dsv[k].raw = make_uint4(0u, 0u, 0u, 0u);
-        if (has_pre) {
-          dhv[k] = load_chunk<T, VEC>(dh_in + at, gl + k * G, Cr);
-          xv[k] = load_chunk<T, VEC>(x_in + at, gl + k * G, Cr);
+          for (int j = 0; j < V; ++j) r[j] = kept[j];
+        } else {
+          load_vec<V, VEC>(from, gl + k * G, C, absent, r);
         }
-        if (y_in != nullptr) yv[k] = load_chunk<T, VEC>(y_in + at, gl + k * G, Cr);
-        else yv[k].raw = make_uint4(0u, 0u, 0u, 0u);
-      }
-      const long n = MODE != kPreOnly && (p.scale != nullptr || p.gate_kind == kGateSample)
-                         ? fdiv((uint32_t)(live ? row : 0), by_sample) : 0;
-      const float sc = MODE != kPreOnly && p.scale != nullptr ? p.scale[n] : 1.f;
-      const float* gate = p.gate_kind == kGateSample ? p.gate + n * C : p.gate;
-      float ymean = 0.f, yrstd = 0.f;
-      if (has_post) {
-        ymean = live ? p.post_stat[row] : 0.f;
-        yrstd = live ? p.post_stat[p.rows + row] : 0.f;
-      }
+      };
       float g[MAXCH][V];
 #pragma unroll
       for (int k = 0; k < MAXCH; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) g[k][j] = dsv[k].get(j);
+        for (int j = 0; j < V; ++j) g[k][j] = cur.ds[k].get(j);
+      if constexpr (PRE)
       if (has_pre) {
-        const float mean = live ? p.pre_stat[row] : 0.f, rstd = live ? p.pre_stat[p.rows + row] : 0.f;
+        const float mean = cur.mean, rstd = cur.rstd;
         float m[2] = {0.f, 0.f};
-        float sh[PRE ? MAXCH : 1][V];
+        float sh[MAXCH][V];
 #pragma unroll
         for (int k = 0; k < MAXCH; ++k) {
           float w[V], f[V], pw[V], pb[V];
-          load_vec<V, VEC>(p.pre_w, gl + k * G, C, 1.f, w);
-          if (MODE == kAll) {
-            load_vec<V, VEC>(gate, gl + k * G, C, 1.f, f);
+          param(p.pre_w, pre_w[HOIST ? k : 0], k, 1.f, w);
+          if constexpr (MODE == kAll) {
+            param(gate, gate_v[HOIST ? k : 0], k, 1.f, f);
             if (has_post) {
-              load_vec<V, VEC>(p.post_w, gl + k * G, C, 1.f, pw);
-              load_vec<V, VEC>(p.post_b, gl + k * G, C, 0.f, pb);
+              param(p.post_w, post_w[HOIST ? k : 0], k, 1.f, pw);
+              param(p.post_b, post_b[HOIST ? k : 0], k, 0.f, pb);
             }
           }
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            float z = yv[k].get(j);
+            float z = cur.y[k].get(j);
             if (MODE == kAll) {
               if (has_post) z = (z - ymean) * yrstd * pw[j] + pb[j];
               z *= sc * f[j];
             }
-            const float d = dhv[k].get(j), gw = d * w[j];      // absent: d = 0
-            sh[k][j] = (xv[k].get(j) + z - mean) * rstd;
+            const float d = cur.dh[k].get(j), gw = d * w[j];      // absent: d = 0
+            sh[k][j] = (cur.x[k].get(j) + z - mean) * rstd;
             m[0] += gw;
             m[1] += gw * sh[k][j];
-            if constexpr (PRE) {
-              a_prew[k][j] += d * sh[k][j];
-              a_preb[k][j] += d;
-            }
+            a_prew[k][j] += d * sh[k][j];
+            a_preb[k][j] += d;
           }
         }
         gsum.run(m, G);
@@ -171,34 +213,35 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNo
 #pragma unroll
         for (int k = 0; k < MAXCH; ++k) {
           float w[V];
-          load_vec<V, VEC>(p.pre_w, gl + k * G, C, 1.f, w);
+          param(p.pre_w, pre_w[HOIST ? k : 0], k, 1.f, w);
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[k][j] += rstd * (dhv[k].get(j) * w[j] - m0 - sh[k][j] * m1);
+          for (int j = 0; j < V; ++j) g[k][j] += rstd * (cur.dh[k].get(j) * w[j] - m0 - sh[k][j] * m1);
         }
       }
+      if (dx != nullptr)
 #pragma unroll
-      for (int k = 0; k < MAXCH; ++k) {
-        Vec16<T> o;
+        for (int k = 0; k < MAXCH; ++k) {
+          Vec16<T> o;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o.set(j, g[k][j]);
-        if (live && dx != nullptr) store_chunk<T, VEC>(o, dx + row * C, gl + k * G, C);
-      }
+          for (int j = 0; j < V; ++j) o.set(j, g[k][j]);
+          if (live) store_chunk<T, VEC>(o, dx + row * C, gl + k * G, C);
+        }
       if (dy != nullptr) {
         float m[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < MAXCH; ++k) {
           const int c0 = (gl + k * G) * V;
           float gt[V], w[V], b[V];
-          if (MODE == kAll) load_vec<V, VEC>(gate, gl + k * G, C, 1.f, gt);
-          if (has_post) {
-            load_vec<V, VEC>(p.post_w, gl + k * G, C, 1.f, w);
-            if (has_gate) load_vec<V, VEC>(p.post_b, gl + k * G, C, 0.f, b);
-          }
+          if constexpr (MODE == kAll) param(gate, gate_v[HOIST ? k : 0], k, 1.f, gt);
+          if constexpr (POST)
+            if (has_post) param(p.post_w, post_w[HOIST ? k : 0], k, 1.f, w);
+          if constexpr (MODE == kAll)
+            if (has_post && has_gate) param(p.post_b, post_b[HOIST ? k : 0], k, 0.f, b);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             const bool ok = live && (VEC ? c0 < C : c0 + j < C);
             const float dzs = ok ? sc * g[k][j] : 0.f;
-            const float yj = yv[k].get(j);
+            const float yj = cur.y[k].get(j);
             const float yh = has_post ? (yj - ymean) * yrstd : yj;
             if constexpr (MODE == kAll)
               if (has_gate && ok) a_gate[k][j] += dzs * (has_post ? yh * w[j] + b[j] : yh);
@@ -223,7 +266,7 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNo
           for (int k = 0; k < MAXCH; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j)
-              g[k][j] = yrstd * (g[k][j] - m0 - (yv[k].get(j) - ymean) * yrstd * m1);
+              g[k][j] = yrstd * (g[k][j] - m0 - (cur.y[k].get(j) - ymean) * yrstd * m1);
         }
 #pragma unroll
         for (int k = 0; k < MAXCH; ++k) {
@@ -233,6 +276,7 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNo
           if (live) store_chunk<T, VEC>(o, dy + row * C, gl + k * G, C);
         }
       }
+      if constexpr (AHEAD) cur = next;
     }
     if constexpr (MODE == kAll)
       if (p.gate_kind == kGateSample && p.gate_partial != nullptr) {
@@ -255,17 +299,33 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(const ResidualNo
 }
 
 // out[v][c] = beta * out + sum over the partial rows, in a fixed order: 16 columns x 16 part lanes a workgroup
+// (behind them, one after the other, the samples' gates: the sum over the splits of a sample)
 struct FoldArgs {
   const float* partial; long nparts, part_stride;
   float* out[5]; float beta[5];
-  int C;
+  const float* gate_partial; float* dgate; int splits;
+  int C, vectors, which[5];
 };
 __global__ __launch_bounds__(256) void residual_norm_fold_kernel(const FoldArgs a) {
   __shared__ float red[16][17];
-  const int v = blockIdx.y;
-  if (a.out[v] == nullptr) return;
   const int cl = threadIdx.x & 15, pl = threadIdx.x >> 4;
   const int c = blockIdx.x * 16 + cl;
+  if ((int)blockIdx.y >= a.vectors) {
+    const long n = blockIdx.y - a.vectors;
+    float t = 0.f;
+    if (c < a.C)
+      for (int q = pl; q < a.splits; q += 16) t += a.gate_partial[(n * a.splits + q) * a.C + c];
+    red[pl][cl] = t;
+    __syncthreads();
+    if (pl == 0 && c < a.C) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += red[i][cl];
+      a.dgate[n * a.C + c] = sum;
+    }
+    return;
+  }
+  const int v = a.which[blockIdx.y];
   float t = 0.f;
   if (c < a.C) {
     const float* src = a.partial + (long)v * a.C + c;
@@ -286,17 +346,6 @@ __global__ __launch_bounds__(256) void residual_norm_fold_kernel(const FoldArgs 
     for (int i = 0; i < 16; ++i) sum += red[i][cl];
     a.out[v][c] = a.beta[v] == 0.f ? sum : sum + a.beta[v] * a.out[v][c];
   }
-}
-
-// dgate[n][c] = sum over the splits of sample n
-__global__ __launch_bounds__(256) void residual_norm_fold_gate_kernel(const float* __restrict__ partial, int splits, long total,
-                                                                      int C, float* __restrict__ out) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const long n = i / C, c = i - n * C;
-  float t = 0.f;
-  for (int q = 0; q < splits; ++q) t += partial[(n * splits + q) * C + c];
-  out[i] = t;
 }
 
 struct Units {
@@ -334,7 +383,7 @@ template <typename T, int MAXCH, bool WIDE>
 void launch(const ResidualNormBwd& p, const Plan& pl, const Units& u, bool vec, int mode, hipStream_t s) {
   const FastDiv by_sample = make_fastdiv((uint32_t)p.per_sample);
 #define DPA_RN_BWD(VECB, MODEC)                                                                                       \
-  hipLaunchKernelGGL((residual_norm_bwd_kernel<T, MAXCH, WIDE, VECB, MODEC>), dim3(u.blocks), dim3(256), 0, s, p, pl.G, \
+  hipLaunchKernelGGL((residual_norm_bwd_kernel<T, MAXCH, WIDE, VECB, MODEC>), dim3(u.blocks), dim3(pl.threads), 0, s, p, pl.G, \
                      u.units, u.unit_rows, u.splits, by_sample)
   if (!vec) DPA_RN_BWD(false, kAll);
   else if (mode == kPreOnly) DPA_RN_BWD(true, kPreOnly);
@@ -371,8 +420,7 @@ void residual_norm_bwd_launch(const ResidualNormBwd& p, int dtype, hipStream_t s
     else if (!pl.wide) launch<T, 2, false>(p, pl, u, vec, mode, s);
     else if (pl.maxch == 1) launch<T, 1, true>(p, pl, u, vec, mode, s);
     else if (pl.maxch == 2) launch<T, 2, true>(p, pl, u, vec, mode, s);
-    else if (pl.maxch == 4) launch<T, 4, true>(p, pl, u, vec, mode, s);
-    else launch<T, 8, true>(p, pl, u, vec, mode, s);
+    else launch<T, 4, true>(p, pl, u, vec, mode, s);
   });
   DPA_CHECK_HIP(hipGetLastError());
   FoldArgs f{};
@@ -380,21 +428,28 @@ void residual_norm_bwd_launch(const ResidualNormBwd& p, int dtype, hipStream_t s
   f.nparts = u.blocks;
   f.part_stride = 5l * p.C;
   f.C = p.C;
-  bool any = false;
   for (int v = 0; v < 5; ++v) {
     f.out[v] = p.out[v];
     f.beta[v] = p.beta[v];
-    any = any || p.out[v] != nullptr;
+    if (p.out[v] != nullptr) f.which[f.vectors++] = v;
   }
-  if (any) {
-    hipLaunchKernelGGL(residual_norm_fold_kernel, dim3((unsigned)((p.C + 15) / 16), 5), dim3(256), 0, s, f);
+  const bool gates = p.gate_kind == kGateSample && p.dgate_sample != nullptr;
+  f.gate_partial = p.gate_partial;
+  f.dgate = p.dgate_sample;
+  f.splits = u.splits;
+  // (grid.y holds 65535: samples beyond that many take further launches)
+  long left = gates ? p.rows / p.per_sample : 0;
+  while (f.vectors > 0 || left > 0) {
+    const long now = left < 65535 - f.vectors ? left : 65535 - f.vectors;
+    hipLaunchKernelGGL(residual_norm_fold_kernel, dim3((unsigned)((p.C + 15) / 16), (unsigned)(f.vectors + now)), dim3(256), 0, s,
+                       f);
     DPA_CHECK_HIP(hipGetLastError());
-  }
-  if (p.gate_kind == kGateSample && p.dgate_sample != nullptr) {
-    const long total = p.rows / p.per_sample * p.C;
-    hipLaunchKernelGGL(residual_norm_fold_gate_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, p.gate_partial,
-                       u.splits, total, p.C, p.dgate_sample);
-    DPA_CHECK_HIP(hipGetLastError());
+    if (gates) {
+      f.gate_partial += now * u.splits * p.C;
+      f.dgate += now * p.C;
+    }
+    left -= now;
+    f.vectors = 0;
   }
 }
 

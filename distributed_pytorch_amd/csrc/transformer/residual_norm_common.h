@@ -1,9 +1,9 @@
 // Row layout shared by the two directions of residual_norm: which lanes own a row and how its chunks are moved.
 //
 // A row of C channels is cut into chunks of 16 bytes.  Up to 64 chunks: G lanes of one wave own the row (G the power of
-// two >= chunks, at least 4; 64 / G rows side by side); up to 128: a wave with two chunks a lane; wider: the workgroup's
-// 256 lanes with 1, 2, 4 or 8 chunks each (a sum then takes two barriers, but the per-channel sums of backward stay
-// few enough for registers).  Rows whose length or base is not a multiple of 16 bytes move element by element (VEC =
+// two >= chunks, at least 4; 64 / G rows side by side); up to 128: a wave with two chunks a lane; wider: a workgroup of
+// just the waves that the row fills, with 1 (up to 512 chunks), 2 or 4 chunks a lane (a sum then takes a barrier, but the
+// per-channel sums of backward stay few enough for registers, and 320 chunks do not idle half of 2 x 256 lanes).  Rows whose length or base is not a multiple of 16 bytes move element by element (VEC =
 // false), in the same layout.
 #pragma once
 #include "../common.h"
@@ -18,6 +18,7 @@ struct Plan {
   int G, maxch;
   bool wide;
   int rows_per_trip;      // of a workgroup, with one row per lane group
+  int threads;
 };
 inline Plan plan(int C, int vec) {
   Plan p;
@@ -28,35 +29,69 @@ inline Plan plan(int C, int vec) {
     while (p.G < chunks && p.G < 64) p.G <<= 1;
     p.maxch = chunks <= 64 ? 1 : 2;
     p.rows_per_trip = 4 * (64 / p.G);
+    p.threads = 256;
   } else {
-    p.G = 256;
-    p.maxch = chunks <= 256 ? 1 : (chunks <= 512 ? 2 : (chunks <= 1024 ? 4 : 8));
+    p.maxch = chunks <= 512 ? 1 : (chunks <= 1024 ? 2 : 4);
+    p.threads = ((chunks + p.maxch - 1) / p.maxch + 63) / 64 * 64;
+    p.G = p.threads;
     p.rows_per_trip = 1;
   }
   return p;
 }
 
-// sum over the lanes that own a row; R sums at once.  WIDE: `red` is [2][R][4] floats of LDS; consecutive calls
-// alternate between its halves, so one barrier per call separates a write from the read of the call before the last
+// sum over groups of G (4 .. 64, a power of two) neighbouring lanes, the same in every lane of a group.  Lane exchange in
+// the VALU (DPP inside rows of 16 lanes, the permlane swaps across them): a butterfly of LDS shuffles waits for LDS six
+// times, and two sums per row and norm are the longest chain of these kernels
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_sum(float v, int G) {
+  v += dpp<0xB1>(v);                       // quad_perm 1 0 3 2
+  v += dpp<0x4E>(v);                       // quad_perm 2 3 0 1
+  if (G >= 8) v += dpp<0x141>(v);          // row_half_mirror
+  if (G >= 16) v += dpp<0x140>(v);         // row_mirror
+  if (G >= 32) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  if (G >= 64) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  return v;
+}
+
+// sum over the lanes that own a row; R sums at once.  WIDE: `red` is [2][R][8] floats of LDS, cleared at the start (clear());
+// consecutive calls alternate between its halves, so one barrier per call separates a write from the read of the call
+// before the last
+constexpr int kMaxWaves = 8;
 template <bool WIDE, int R> struct GroupSum {
   float* red;
   int flip = 0;
+  __device__ __forceinline__ void clear() {
+    if constexpr (WIDE) {
+      if (threadIdx.x < 2 * R * kMaxWaves) red[threadIdx.x] = 0.f;
+      __syncthreads();
+    }
+  }
   __device__ __forceinline__ void run(float (&v)[R], int G) {
     if constexpr (!WIDE) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        for (int off = G >> 1; off > 0; off >>= 1) v[r] += __shfl_xor(v[r], off, 64);
+      for (int r = 0; r < R; ++r) v[r] = lane_sum(v[r], G);
     } else {
-      float* half = red + flip * R * 4;
+      float* half = red + flip * R * kMaxWaves;
       flip ^= 1;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        v[r] = wave_sum(v[r]);
-        if ((threadIdx.x & 63) == 0) half[r * 4 + (threadIdx.x >> 6)] = v[r];
+        v[r] = lane_sum(v[r], 64);
+        if ((threadIdx.x & 63) == 0) half[r * kMaxWaves + (threadIdx.x >> 6)] = v[r];
       }
       __syncthreads();
 #pragma unroll
-      for (int r = 0; r < R; ++r) v[r] = (half[r * 4] + half[r * 4 + 1]) + (half[r * 4 + 2] + half[r * 4 + 3]);
+      for (int r = 0; r < R; ++r) {
+        const float4 a = reinterpret_cast<const float4*>(half + r * kMaxWaves)[0], b = reinterpret_cast<const float4*>(half + r * kMaxWaves)[1];
+        v[r] = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+      }
     }
   }
 };
