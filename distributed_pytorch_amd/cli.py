@@ -51,6 +51,12 @@ def add_native_flags(parser: argparse.ArgumentParser) -> None:
     g.add_argument("--steps", default=0, type=int, metavar="N",
                    help="stop every epoch after N iterations (0 = full epoch)")
     g.add_argument("--warmup-epochs", default=5, type=int)
+    g.add_argument("--optimizer", default="sgd", choices=["sgd", "muon"],
+                   help="muon: matrices inside the network take the orthogonalised momentum (optim.FusedMuon), "
+                        "everything else SGD")
+    g.add_argument("--predictions", default="", type=str, metavar="PATH",
+                   help="write every validated sample's log probability, entropy and five most probable classes to "
+                        "PATH (JSON lines; .rankN is appended where ranks validate different samples)")
     g.add_argument("--profile", action="store_true", help="emit roctx ranges around step phases")
     g.add_argument("--hip-graph", action="store_true",
                    help="capture the train step into a hipGraph (static shapes)")

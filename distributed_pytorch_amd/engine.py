@@ -36,7 +36,7 @@ from .data.sampler import DistributedSampler
 from .data import transforms as T
 from .nn.modules import CrossEntropyLoss
 from .ops import functional as F
-from .optim import FusedSGD
+from .optim import FusedMuon, FusedSGD, muon_groups
 from .utils import profiling
 from .utils.meters import AverageMeter, DeviceMeter, ProgressMeter, Summary, format_hms
 from .utils.tb import SummaryWriter
@@ -157,7 +157,10 @@ def main_worker(local_rank: int, ngpus_per_node: int, args) -> None:
     if script == "apex":
         args.lr = schedule.scale_lr_for_global_batch(args.lr, args.batch_size, world)
 
-    optimizer = FusedSGD(model.parameters(), args.lr, momentum=args.momentum, weight_decay=args.weight_decay)
+    if getattr(args, "optimizer", "sgd") == "muon":
+        optimizer = FusedMuon(muon_groups(model), args.lr, momentum=args.momentum, weight_decay=args.weight_decay)
+    else:
+        optimizer = FusedSGD(model.parameters(), args.lr, momentum=args.momentum, weight_decay=args.weight_decay)
     opt_level = args.opt_level if script == "apex" else None
     model, optimizer = amp.initialize(model, optimizer, opt_level=opt_level or "O0",
                                       keep_batchnorm_fp32=args.keep_batchnorm_fp32,
@@ -392,6 +395,29 @@ class _Run:
         return {"throughput": thr_avg.avg, "batch_time": batch_time.avg, "loss": losses.avg,
                 "top1": top1.avg, "top5": top5.avg, "lr": lr}
 
+    # ------------------------------------------------------------------ predictions
+    def _predictions_file(self):
+        """Where this rank writes predictions, or None: every rank of the AMP script validates samples of its own, the
+        others all validate the same ones."""
+        path = getattr(self.args, "predictions", "")
+        if not path:
+            return None
+        if self.script == "apex" and self.args.distributed:
+            return open("%s.rank%d" % (path, self.rank), "w")
+        return open(path, "w") if self.is_main else None
+
+    @staticmethod
+    def _write_predictions(out, held: list, row: int) -> int:
+        """Writes and clears the batches held on the device (one transfer per print window); -> the next sample's number."""
+        if out is None or not held:
+            return row
+        target, lp, ent, top, idx = (torch.cat(c).cpu().tolist() for c in zip(*held))
+        held.clear()
+        for t, a, e, v, j in zip(target, lp, ent, top, idx):
+            out.write(json.dumps({"sample": row, "target": t, "logprob": a, "entropy": e, "top": j, "top_logprob": v}) + "\n")
+            row += 1
+        return row
+
     # ------------------------------------------------------------------ validate
     def validate(self, loader, epoch: int) -> dict:
         args, script = self.args, self.script
@@ -402,6 +428,8 @@ class _Run:
         top5 = AverageMeter("Acc@5", ":6.2f", Summary.AVERAGE)
         progress = ProgressMeter(n_iter, [batch_time, losses, top1, top5], prefix="Test: ")
         dm = DeviceMeter(self.device)
+        predictions = self._predictions_file()
+        held, row = [], 0
         self.model.eval()
         pre = self._prefetcher(loader)
         start = win_start = time.time()
@@ -416,8 +444,11 @@ class _Run:
                 output = self.model(images)
                 _, rec = F.loss_and_metrics(output, target)
                 dm.update(rec)
+                if predictions is not None:
+                    held.append((target,) + F.token_logprobs(output, target, min(5, output.shape[1])))
                 win_iters += 1
                 if i % args.print_freq == 0 or i == n_stop:
+                    row = self._write_predictions(predictions, held, row)
                     (l_loss, l_a1, l_a5, _), (r_loss, r_a1, r_a5, r_n) = DeviceMeter.unpack(
                         self._reduced(dm.packed()).cpu())
                     per_iter = (time.time() - win_start) / max(win_iters, 1)
@@ -436,6 +467,9 @@ class _Run:
                     win_start, win_iters = time.time(), 0
                 if i >= n_stop:
                     break
+        self._write_predictions(predictions, held, row)
+        if predictions is not None:
+            predictions.close()
         if script == "nd":
             progress.display_summary()
         elif script == "ddp" or self.is_main:

@@ -51,6 +51,9 @@ class CNBlock(nn.Module):
         b = self.block
         h = b[5](b[4](b[3](b[2](b[0](x)))))
         n, c = h.shape[0], h.shape[-1]
+        if F.fuse_residual_norm():
+            return F.residual_norm(x, h, gate=self.layer_scale.reshape(c),
+                                   scale=F.stochastic_depth_scale(h, self.stochastic_depth.p, self.training))
         h = F.se_scale(h, self.layer_scale.reshape(1, c).float().expand(n, c))      # per-channel layer scale
         return F.add(self.stochastic_depth(h), x)
 

@@ -215,7 +215,18 @@ class SwinTransformerBlock(nn.Module):
         self.norm2 = LayerNorm(dim, eps=1e-5)
         self.mlp = _MLP(dim, int(dim * mlp_ratio), dropout)
 
+    def _fused(self, x):
+        """The residual sums with their norms and stochastic depth as ``F.residual_norm``."""
+        sd = lambda: F.stochastic_depth_scale(x, self.stochastic_depth.p, self.training)      # noqa: E731
+        if self.v2:
+            x = F.residual_norm(x, self.attn(x), post=self.norm1.spec(), scale=sd())
+            return F.residual_norm(x, self.mlp(x), post=self.norm2.spec(), scale=sd())
+        x, h = F.residual_norm(x, self.attn(self.norm1(x)), scale=sd(), pre=self.norm2.spec())
+        return F.residual_norm(x, self.mlp(h), scale=sd())
+
     def forward(self, x):
+        if F.fuse_residual_norm():
+            return self._fused(x)
         if self.v2:
             x = F.add(x, self.stochastic_depth(self.norm1(self.attn(x))))
             return F.add(x, self.stochastic_depth(self.norm2(self.mlp(x))))

@@ -20,7 +20,7 @@ from collections import OrderedDict
 import torch
 from torch import nn
 
-from ..nn.modules import GELU, Conv2d, Dropout, LayerNorm, Linear
+from ..nn.modules import GELU, AxialRotary, Conv2d, Dropout, LayerNorm, Linear
 from ..ops import functional as F
 from .alexnet_vgg import _ImageNetCNN
 
@@ -50,8 +50,11 @@ class MultiheadSelfAttention(nn.Module):
         self.out_proj = _OutProj(embed_dim, embed_dim)
         nn.init.xavier_uniform_(self.in_proj_weight)
 
-    def forward(self, x):
+    def forward(self, x, rotary=None):
+        """``rotary``: (``AxialRotary``, positions) turns queries and keys by their patch's row and column."""
         qkv = F.linear(x, self.in_proj_weight, self.in_proj_bias)
+        if rotary is not None:
+            qkv = rotary[0](qkv, rotary[1], self.num_heads)
         a = F.attention(qkv, self.num_heads, self.head_dim ** -0.5)
         return self.out_proj(a)
 
@@ -84,12 +87,19 @@ class EncoderBlock(nn.Module):
         self.ln_2 = LayerNorm(hidden_dim, eps=1e-6)
         self.mlp = MLPBlock(hidden_dim, mlp_dim, dropout)
 
-    def forward(self, x):
-        y = self.self_attention(self.ln_1(x))
-        if self.dropout.p:
-            y = self.dropout(y)
-        x = F.add(x, y)
+    def forward(self, x, rotary=None):
+        x = F.add(x, self._attend(self.ln_1(x), rotary))
         return F.add(x, self.mlp(self.ln_2(x)))
+
+    def _attend(self, h, rotary=None):
+        y = self.self_attention(h, rotary)
+        return self.dropout(y) if self.dropout.p else y
+
+    def fused(self, x, h, next_norm, rotary=None):
+        """The block on the residual stream ``x`` and its first norm's result ``h``: -> the stream behind the block and
+        ``next_norm`` of it, each residual sum and the norm behind it in one pass."""
+        x, h = F.residual_norm(x, self._attend(h, rotary), pre=self.ln_2.spec())
+        return F.residual_norm(x, self.mlp(h), pre=next_norm.spec())
 
 
 class Encoder(nn.Module):
@@ -103,16 +113,25 @@ class Encoder(nn.Module):
             for i in range(num_layers)))
         self.ln = LayerNorm(hidden_dim, eps=1e-6)
 
-    def forward(self, x):
+    def forward(self, x, rotary=None):
         x = x + self.pos_embedding.to(x.dtype)
         if self.dropout.p:
             x = self.dropout(x)
-        return self.ln(self.layers(x))
+        if F.fuse_residual_norm():
+            h = self.layers[0].ln_1(x)
+            for i, block in enumerate(self.layers):
+                x, h = block.fused(x, h, self.layers[i + 1].ln_1 if i + 1 < len(self.layers) else self.ln, rotary)
+            return h
+        for block in self.layers:
+            x = block(x, rotary)
+        return self.ln(x)
 
 
 class VisionTransformer(_ImageNetCNN):
     def __init__(self, image_size: int, patch_size: int, num_layers: int, num_heads: int, hidden_dim: int, mlp_dim: int,
-                 dropout: float = 0.0, attention_dropout: float = 0.0, num_classes: int = 1000):
+                 dropout: float = 0.0, attention_dropout: float = 0.0, num_classes: int = 1000, rotary: bool = False):
+        """``rotary=True`` adds rotary positions of the patches' rows and columns (half of every head each) in front of
+        the attention; the learned position embedding stays, so checkpoints keep their keys."""
         super().__init__()
         if image_size % patch_size:
             raise ValueError("Input shape indivisible by patch size!")
@@ -124,6 +143,12 @@ class VisionTransformer(_ImageNetCNN):
         self.encoder = Encoder(seq_length, num_layers, num_heads, hidden_dim, mlp_dim, dropout, attention_dropout)
         self.seq_length = seq_length
         self.heads = nn.Sequential(OrderedDict(head=Linear(hidden_dim, num_classes)))
+        self.rotary = None
+        if rotary:
+            head_dim, side = hidden_dim // num_heads, image_size // patch_size
+            half = head_dim // 4 * 2
+            self.rotary = AxialRotary(head_dim, (half, half), base=100.0)
+            self.register_buffer("rotary_positions", AxialRotary.grid(side, side, class_token=True), persistent=False)
         fan_in = 3 * patch_size * patch_size
         nn.init.trunc_normal_(self.conv_proj.weight, std=math.sqrt(1 / fan_in))
         nn.init.zeros_(self.conv_proj.bias)
@@ -138,7 +163,7 @@ class VisionTransformer(_ImageNetCNN):
         n = x.shape[0]
         x = x.reshape(n, -1, self.hidden_dim)
         x = torch.cat([self.class_token.to(x.dtype).expand(n, -1, -1), x], dim=1)
-        x = self.encoder(x)
+        x = self.encoder(x, None if self.rotary is None else (self.rotary, self.rotary_positions))
         return self.heads.head(x[:, 0].contiguous(), out_dtype=torch.float32)
 
 

@@ -152,11 +152,78 @@ class LayerNorm(nn.Module):
     def forward(self, x):
         return F.layer_norm(x, self.weight, self.bias, self.eps)
 
+    def spec(self) -> F.Norm:
+        """This norm as ``F.residual_norm`` takes it (``post=`` / ``pre=``)."""
+        return F.Norm(self.weight, self.bias, self.eps, "layer")
+
     def extra_repr(self) -> str:
         return "{}, eps={}".format(self.normalized_shape, self.eps)
 
 
 LayerNorm2d = LayerNorm
+
+
+class RMSNorm(nn.Module):
+    """``x / sqrt(mean(x^2) + eps) * weight`` over the channel (last) axis (parameter as in ``nn.RMSNorm(C)``)."""
+
+    def __init__(self, normalized_shape: int, eps: float = 1e-6):
+        super().__init__()
+        self.normalized_shape, self.eps = (int(normalized_shape),), eps
+        self.weight = nn.Parameter(torch.ones(normalized_shape))
+
+    def forward(self, x):
+        return F.rms_norm(x, self.weight, self.eps)
+
+    def spec(self) -> F.Norm:
+        return F.Norm(self.weight, None, self.eps, "rms")
+
+    def extra_repr(self) -> str:
+        return "{}, eps={}".format(self.normalized_shape, self.eps)
+
+
+class AxialRotary(nn.Module):
+    """Rotary positions of several axes on a packed projection (``F.rotary``): the first ``sum(dims)`` elements of every
+    query and key head are split over the axes, ``dims[a]`` (even) of them for axis ``a`` with frequencies
+    ``base ** (-2 i / dims[a])``.  ``forward(qkv, positions, num_heads)`` with ``positions`` ``[S, A]`` or ``[B, S, A]``.
+    ``grid(h, w)`` gives the positions of image patches.  No parameters; the tables keep 64 bits whatever type the module
+    is moved to."""
+
+    def __init__(self, head_dim: int, dims, base: float = 10000.0, interleaved: bool = False):
+        super().__init__()
+        dims = tuple(int(d) for d in dims)
+        if not dims or any(d < 0 or d % 2 for d in dims) or sum(dims) > head_dim:
+            raise ValueError("dims must be even and fit the head")
+        if not base > 0.0:
+            raise ValueError("base must be positive")
+        self.head_dim, self.dims, self.base, self.interleaved = head_dim, dims, float(base), bool(interleaved)
+        freqs, axis = self._tables()
+        self.register_buffer("freqs", freqs, persistent=False)
+        self.register_buffer("axis", axis, persistent=False)
+
+    def _tables(self):
+        freqs = [self.base ** (-2.0 * i / d) for d in self.dims for i in range(d // 2)]
+        axis = [a for a, d in enumerate(self.dims) for _ in range(d // 2)]
+        return torch.tensor(freqs, dtype=torch.float64), torch.tensor(axis, dtype=torch.int32)
+
+    def _apply(self, fn, *args, **kw):
+        super()._apply(fn, *args, **kw)
+        if self.freqs.dtype != torch.float64:
+            self.freqs = self._tables()[0].to(self.freqs.device)
+        return self
+
+    @staticmethod
+    def grid(h: int, w: int, class_token: bool = False) -> torch.Tensor:
+        """Row and column of ``h x w`` patches in raster order, ``[h * w, 2]``; a class token in front sits at (0, 0) and
+        the patches start at (1, 1)."""
+        rows, cols = torch.meshgrid(torch.arange(h), torch.arange(w), indexing="ij")
+        pos = torch.stack([rows.reshape(-1), cols.reshape(-1)], dim=1)
+        return torch.cat([torch.zeros((1, 2), dtype=pos.dtype), pos + 1]) if class_token else pos
+
+    def forward(self, qkv, positions, num_heads: int):
+        return F.rotary(qkv, positions, self.freqs, self.axis, num_heads, interleaved=self.interleaved)
+
+    def extra_repr(self) -> str:
+        return "{}, dims={}, base={}, interleaved={}".format(self.head_dim, self.dims, self.base, self.interleaved)
 
 
 class StochasticDepth(nn.Module):

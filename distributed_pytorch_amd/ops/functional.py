@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import functools
 import math
+import os
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -495,15 +496,34 @@ def se_block(x, w1, b1, w2, b2, act: str, gate: str) -> torch.Tensor:
 def stochastic_depth(x: torch.Tensor, p: float, training: bool) -> torch.Tensor:
     """torchvision ``StochasticDepth(p, "row")``: drops the whole residual branch of a sample with probability
     ``p`` and rescales the survivors by ``1 / (1 - p)``."""
-    if not training or p == 0.0:
+    noise = stochastic_depth_scale(x, p, training)
+    if noise is None:
         return x
+    if _on_gpu(x):
+        return _hip().se_scale(x, noise.view(-1, 1).expand(x.shape[0], x.shape[-1]))
+    return x * noise.to(x.dtype).view(-1, 1, 1, 1)
+
+
+def stochastic_depth_scale(x: torch.Tensor, p: float, training: bool) -> Optional[torch.Tensor]:
+    """The factor of every sample under stochastic depth, ``[N]`` of 0 or ``1 / (1 - p)`` -- ``residual_norm``'s ``scale``;
+    None where nothing is dropped.  The same random numbers as ``stochastic_depth`` draws."""
+    if not training or p == 0.0:
+        return None
     keep = 1.0 - p
     noise = torch.empty((x.shape[0], 1), dtype=torch.float32, device=x.device).bernoulli_(keep)
     if keep > 0.0:
         noise.div_(keep)
-    if _on_gpu(x):
-        return _hip().se_scale(x, noise.expand(x.shape[0], x.shape[-1]))
-    return x * noise.to(x.dtype).view(-1, 1, 1, 1)
+    return noise.view(-1)
+
+
+# DPA_FUSE_RESIDUAL_NORM=1: ViT, Swin, Swin V2 and ConvNeXt blocks run their residual sums with the norms, layer scales and
+# stochastic depth around them as residual_norm calls.  Off by default: a norm then sees the unrounded sum, so results
+# differ from the separate passes by the rounding of the residual stream.
+_FUSE_RESIDUAL_NORM = os.environ.get("DPA_FUSE_RESIDUAL_NORM", "0") == "1"
+
+
+def fuse_residual_norm() -> bool:
+    return _FUSE_RESIDUAL_NORM
 
 
 def dropout(x: torch.Tensor, p: float, training: bool) -> torch.Tensor:
