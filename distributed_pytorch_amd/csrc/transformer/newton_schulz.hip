@@ -58,9 +58,22 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const T* __restrict__ g, l
   const long each = (elems + kNormParts - 1) / kNormParts;
   const long lo = min((long)blockIdx.x * each, elems), hi = min(lo + each, elems);
   double t = 0.0;
-  for (long i = lo + threadIdx.x; i < hi; i += 256) {
-    const double v = (double)to_float(p[i]);
-    t += v * v;
+  constexpr int V = Vec16<T>::N;
+  if (((elems * sizeof(T)) & 15) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {      // whole chunks everywhere
+    const long chunks = elems / V, mine = (chunks + kNormParts - 1) / kNormParts;
+    const long c0 = min((long)blockIdx.x * mine, chunks), c1 = min(c0 + mine, chunks);
+    for (long c = c0 + threadIdx.x; c < c1; c += 256) {
+      Vec16<T> v;
+      v.load(p + c * V);
+      // (eight squares in 32 bits would overflow or vanish where 64 do not)
+#pragma unroll
+      for (int j = 0; j < V; ++j) t += (double)v.get(j) * (double)v.get(j);
+    }
+  } else {
+    for (long i = lo + threadIdx.x; i < hi; i += 256) {
+      const double v = (double)to_float(p[i]);
+      t += v * v;
+    }
   }
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
@@ -81,15 +94,31 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const T* __restrict__ g, 
   __shared__ float tile[64][65];
   __shared__ float inv_s;
   const long b = blockIdx.z;
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int i = 0; i < kNormParts; ++i) t += parts[b * kNormParts + i];
-    inv_s = (float)(1.0 / (sqrt(t) + eps));
+  if (threadIdx.x < kNormParts) {            // one wave
+    double t = parts[b * kNormParts + threadIdx.x];
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (threadIdx.x == 0) inv_s = (float)(1.0 / (sqrt(t) + eps));
   }
   __syncthreads();
   const float inv = inv_s;
   const long i0 = (long)blockIdx.y * 64, j0 = (long)blockIdx.x * 64;     // in X
   const T* p = g + b * rows * cols;
+  constexpr int V = Vec16<T>::N;
+  if (cols % V == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {     // rows of whole chunks
+    for (int e = threadIdx.x; e < 4096 / V; e += 256) {
+      const int r = e / (64 / V), c = e % (64 / V) * V;
+      const long gr = (turned ? j0 : i0) + r, gc = (turned ? i0 : j0) + c;
+      Vec16<T> v;
+      v.raw = make_uint4(0u, 0u, 0u, 0u);
+      if (gr < rows && gc < cols) v.load(p + gr * cols + gc);
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        const float f = v.get(q) * inv * kScale;
+        if (turned) tile[c + q][r] = f;
+        else tile[r][c + q] = f;
+      }
+    }
+  } else
   for (int e = threadIdx.x; e < 4096; e += 256) {
     const int r = e >> 6, c = e & 63;                                    // of G's tile
     const long gr = (turned ? j0 : i0) + r, gc = (turned ? i0 : j0) + c;
@@ -379,6 +408,18 @@ __device__ __forceinline__ void forget(f32x16_t (&acc)[2][2][2]) {
 #pragma unroll
   for (int x = 0; x < 8; ++x) asm volatile("" : "+v"(acc[x >> 2][(x >> 1) & 1][x & 1]));
 }
+// where element (row, col) of a wave's 128 x 64 16-bit results lies in its 16 KiB
+__device__ __forceinline__ int row_place(int row, int col) { return row * 128 + (((col >> 3) ^ (row & 7)) * 16) + (col & 7) * 2; }
+// Puts registers r and r + 1 (16 bits each, the two halves of `both`) of lane row m into the transposed 64 x 128 layout:
+// neighbouring lanes hold neighbouring columns of it and trade, so that each has two columns of one row (an even lane the
+// row of register r, its neighbour that of r + 1)
+__device__ __forceinline__ void to_transpose(unsigned char* my, uint32_t both, int m, int nq, int r, int lh) {
+  const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)both, 0xB1, 0xf, 0xf, true);      // lanes 1 0 3 2
+  const bool odd = m & 1;
+  const uint32_t v = odd ? (other >> 16) | (both & 0xffff0000u) : (both & 0xffffu) | (other << 16);
+  const int n = nq * 32 + ((r + (odd ? 1 : 0)) & 3) + 8 * (r >> 2) + 4 * lh;
+  *reinterpret_cast<uint32_t*>(my + n * 256 + ((((m & ~1) >> 3) ^ (n & 15)) * 16) + ((m & ~1) & 7) * 2) = v;
+}
 // products of one 32 x 32 block over one K slice
 template <bool PAIR> __device__ __forceinline__ void block_mma(f32x16_t& acc, const f16x8_t (&q)[4], const f16x8_t (&f)[4]) {
   if constexpr (PAIR) {                     // [k16 step * 2 + plane]
@@ -624,8 +665,48 @@ __global__ __launch_bounds__(512, 1) void ns_large_kernel(const Product p, const
   }
 
   if constexpr (OP == kFinal) {
-    // the caller's rows may start anywhere: its type and orientation straight from registers
     T* f = reinterpret_cast<T*>(p.fin) + b * p.fin_next;
+    if constexpr (sizeof(T) == 2) {
+      // 16-bit results whose rows are whole chunks leave like the planes below
+      if (p.cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.fin) | (uintptr_t)(p.fin_next * 2)) & 15) == 0) {
+#pragma unroll
+        for (int mq = 0; mq < 2; ++mq)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nq = 0; nq < 2; ++nq)
+#pragma unroll
+              for (int r = 0; r < 16; r += 2) {
+                uint16_t h[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const T v = from_float<T>(acc[mq][mt][nq][r + q] * kInvScale);
+                  __builtin_memcpy(&h[q], &v, 2);
+                }
+                const uint32_t both = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
+                if (p.turned) to_transpose(my, both, mq * 64 + mt * 32 + l31, nq, r, lh);
+                else *reinterpret_cast<uint32_t*>(my + row_place(mq * 64 + mt * 32 + l31, nq * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh)) = both;
+              }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          long row, col;
+          uint4 v;
+          if (p.turned) {
+            const int n = i * 4 + (lane >> 4), ck = lane & 15;
+            v = *reinterpret_cast<const uint4*>(my + n * 256 + ((ck ^ (n & 15)) * 16));
+            row = nw + n; col = mw + ck * 8;
+          } else {
+            const int m = i * 8 + (lane >> 3), ck = lane & 7;
+            v = *reinterpret_cast<const uint4*>(my + m * 128 + ((ck ^ (m & 7)) * 16));
+            row = mw + m; col = nw + ck * 8;
+          }
+          if (row < p.rows && col < p.cols) *reinterpret_cast<uint4*>(f + row * p.cols + col) = v;
+        }
+        return;
+      }
+    }
+    // else its type and orientation straight from registers: rows may start anywhere
 #pragma unroll
     for (int mq = 0; mq < 2; ++mq)
 #pragma unroll
@@ -675,8 +756,7 @@ __global__ __launch_bounds__(512, 1) void ns_large_kernel(const Product p, const
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    // rows of the transpose: neighbouring lanes hold neighbouring columns of it; they trade so that each has two columns
-    // of one row (a lane of even number the row of register r, its neighbour that of r + 1)
+    // rows of the transpose
     if (SYM && at.ti == at.tj) return;
 #pragma unroll
     for (int plane = 0; plane < 2; ++plane) {
@@ -693,13 +773,7 @@ __global__ __launch_bounds__(512, 1) void ns_large_kernel(const Product p, const
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
               const Half2 s0 = split(acc[mq][mt][nq][r]), s1 = split(acc[mq][mt][nq][r + 1]);
-              const uint32_t both = plane ? pack(s0.lo, s1.lo) : pack(s0.hi, s1.hi);
-              const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)both, 0xB1, 0xf, 0xf, true);   // lanes 1 0 3 2
-              const bool odd = lane & 1;
-              const uint32_t v = odd ? (other >> 16) | (both & 0xffff0000u) : (both & 0xffffu) | (other << 16);
-              const int n = nq * 32 + ((r + (odd ? 1 : 0)) & 3) + 8 * (r >> 2) + 4 * lh;
-              const int m = mq * 64 + mt * 32 + (l31 & ~1);
-              *reinterpret_cast<uint32_t*>(my + n * 256 + (((m >> 3) ^ (n & 15)) * 16) + (m & 7) * 2) = v;
+              to_transpose(my, plane ? pack(s0.lo, s1.lo) : pack(s0.hi, s1.hi), mq * 64 + mt * 32 + l31, nq, r, lh);
               if ((r & 3) == 2) __builtin_amdgcn_sched_barrier(0);
             }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
