@@ -50,6 +50,13 @@ __device__ __forceinline__ uint32_t pack(_Float16 a, _Float16 b) {
   return (uint32_t)x | ((uint32_t)y << 16);
 }
 
+// Two registers' 16-bit halves (r in the low half, r + 1 in the high one) of neighbouring lanes, traded so that an even lane
+// has register r of itself and its neighbour and an odd lane register r + 1 of both
+__device__ __forceinline__ uint32_t trade_pair(uint32_t both, bool odd) {
+  const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)both, 0xB1, 0xf, 0xf, true);      // lanes 1 0 3 2
+  return odd ? (other >> 16) | (both & 0xffff0000u) : (both & 0xffffu) | (other << 16);
+}
+
 // ---- |G|_F^2 in 64 bits: kNormParts partial sums a matrix
 template <typename T>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const T* __restrict__ g, long elems, double* __restrict__ parts) {
@@ -212,68 +219,79 @@ template <bool PAIR> __device__ __forceinline__ void slice_mma(f32x16_t (&acc)[2
   }
 }
 
-// what becomes of a wave's sums on a 64 x 64 tile: half of the registers of its 32 x 32 quarter
+// what becomes of four neighbouring sums, elements (i, j .. j + 3); `diag_tile`: on the diagonal of a symmetric result
 template <int OP, typename T>
-__device__ __forceinline__ void small_epilogue(const Product& p, const Place& at, int wave, int lane, const float (&sum)[8]) {
-  const int kg = wave >> 2, wr = (wave >> 1) & 1, wc = wave & 1, l31 = lane & 31, lh = lane >> 5;
-  const long b = at.b, i0 = (long)at.ti * kSmall, j0 = (long)at.tj * kSmall;
-  // sum[r] is element (i0 + wr * 32 + l31, j0 + wc * 32 + 16 * kg + (r & 3) + 8 * (r >> 2) + 4 * lh)
+__device__ __forceinline__ void quad_epilogue(const Product& p, long b, long i, long j, bool diag_tile, float di,
+                                              const float (&sum)[4]) {
   constexpr bool SYM = OP == kGram || OP == kPoly;
-  const long i = i0 + wr * 32 + l31;
-  const float* diag = p.diag + b * p.diag_next;
-  const float di = OP == kGram ? 0.f : diag[i];
+  float v[4];
+  float r[4] = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (OP != kGram) {
+    const long o = b * p.R.next + i * p.R.ld + j;
+    _Float16 h[4];
+    uint2 raw = *reinterpret_cast<const uint2*>(p.R.hi + o);
+    __builtin_memcpy(h, &raw, 8);
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const long j = j0 + wc * 32 + 16 * kg + 8 * g + 4 * lh;
-    float v[4];
-    float r[4] = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (OP != kGram) {
-      const long o = b * p.R.next + i * p.R.ld + j;
-      _Float16 h[4];
-      uint2 raw = *reinterpret_cast<const uint2*>(p.R.hi + o);
+    for (int q = 0; q < 4; ++q) r[q] = (float)h[q];
+    if (p.R.lo != nullptr) {
+      raw = *reinterpret_cast<const uint2*>(p.R.lo + o);
       __builtin_memcpy(h, &raw, 8);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) r[q] = (float)h[q];
-      if (p.R.lo != nullptr) {
-        raw = *reinterpret_cast<const uint2*>(p.R.lo + o);
-        __builtin_memcpy(h, &raw, 8);
+      for (int q = 0; q < 4; ++q) r[q] += (float)h[q];
+    }
+  }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) r[q] += (float)h[q];
+  for (int q = 0; q < 4; ++q) {
+    const float dj = OP == kPoly ? p.diag[b * p.diag_next + j + q] : 0.f;
+    v[q] = combine<OP>(sum[q], r[q], di, dj, p.c0, p.c1);
+    if constexpr (SYM)
+      if (i == j + q) {
+        (OP == kGram ? p.diag : p.diag_out)[b * p.diag_next + i] = on_diagonal<OP>(sum[q], di, p.c0, p.c1);
+        v[q] = 0.f;
       }
+  }
+  if constexpr (OP == kFinal) {
+    T* f = reinterpret_cast<T*>(p.fin) + b * p.fin_next;
+    T t[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[q] = from_float<T>(v[q] * kInvScale);
+    if (!p.turned && p.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(p.fin) & 15) == 0) {      // four columns at once
+      if (i < p.rows && j < p.cols) __builtin_memcpy(__builtin_assume_aligned(f + i * p.cols + j, 4 * sizeof(T)), t, 4 * sizeof(T));
+      return;
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float dj = OP == kPoly ? diag[j + q] : 0.f;
-      v[q] = combine<OP>(sum[g * 4 + q], r[q], di, dj, p.c0, p.c1);
-      if constexpr (SYM)
-        if (i == j + q) {
-          (OP == kGram ? p.diag : p.diag_out)[b * p.diag_next + i] = on_diagonal<OP>(sum[g * 4 + q], di, p.c0, p.c1);
-          v[q] = 0.f;
-        }
+      const long row = p.turned ? j + q : i, col = p.turned ? i : j + q;
+      if (row < p.rows && col < p.cols) f[row * p.cols + col] = t[q];
     }
-    if constexpr (OP == kFinal) {
-      T* f = reinterpret_cast<T*>(p.fin) + b * p.fin_next;
+  } else {
+    Half2 h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) h[q] = split(v[q]);
+    const long o = b * p.out.next + i * p.out.ld + j;
+    *reinterpret_cast<uint2*>(p.out.hi + o) = make_uint2(pack(h[0].hi, h[1].hi), pack(h[2].hi, h[3].hi));
+    if (p.out.lo != nullptr) *reinterpret_cast<uint2*>(p.out.lo + o) = make_uint2(pack(h[0].lo, h[1].lo), pack(h[2].lo, h[3].lo));
+    if (!SYM || !diag_tile) {
+      const long t = b * p.out_t.next + j * p.out_t.ld + i;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const long row = p.turned ? j + q : i, col = p.turned ? i : j + q;
-        if (row < p.rows && col < p.cols) f[row * p.cols + col] = from_float<T>(v[q] * kInvScale);
-      }
-    } else {
-      Half2 h[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) h[q] = split(v[q]);
-      const long o = b * p.out.next + i * p.out.ld + j;
-      *reinterpret_cast<uint2*>(p.out.hi + o) = make_uint2(pack(h[0].hi, h[1].hi), pack(h[2].hi, h[3].hi));
-      if (p.out.lo != nullptr) *reinterpret_cast<uint2*>(p.out.lo + o) = make_uint2(pack(h[0].lo, h[1].lo), pack(h[2].lo, h[3].lo));
-      if (!SYM || at.ti != at.tj) {
-        const long t = b * p.out_t.next + j * p.out_t.ld + i;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          p.out_t.hi[t + q * p.out_t.ld] = h[q].hi;
-          if (p.out_t.lo != nullptr) p.out_t.lo[t + q * p.out_t.ld] = h[q].lo;
-        }
+        p.out_t.hi[t + q * p.out_t.ld] = h[q].hi;
+        if (p.out_t.lo != nullptr) p.out_t.lo[t + q * p.out_t.ld] = h[q].lo;
       }
     }
+  }
+}
+
+// a wave's sums on a 64 x 64 tile: half of the registers of its 32 x 32 quarter
+template <int OP, typename T>
+__device__ __forceinline__ void small_epilogue(const Product& p, const Place& at, int wave, int lane, const float (&sum)[8]) {
+  const int kg = wave >> 2, wr = (wave >> 1) & 1, wc = wave & 1, l31 = lane & 31, lh = lane >> 5;
+  const long i = (long)at.ti * kSmall + wr * 32 + l31;
+  const float di = OP == kGram ? 0.f : p.diag[at.b * p.diag_next + i];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float four[4] = {sum[g * 4], sum[g * 4 + 1], sum[g * 4 + 2], sum[g * 4 + 3]};
+    quad_epilogue<OP, T>(p, at.b, i, (long)at.tj * kSmall + wc * 32 + 16 * kg + 8 * g + 4 * lh, at.ti == at.tj, di, four);
   }
 }
 
@@ -390,6 +408,154 @@ __global__ __launch_bounds__(512) void ns_join_kernel(const Product p, const uin
   small_epilogue<kGram, T>(p, at, wave, lane, sum);
 }
 
+// ================================================================================ 128 x 128 tiles
+// X = a X + B X of small matrices: a contraction of a few slices over many tiles, bound by the traffic into LDS, of which
+// a 64 x 64 tile takes twice as much.  8 waves of 64 x 32, a ring of four slices, three in flight.
+constexpr int kMid = 128;
+
+template <bool PAIR, int OP, typename T>
+__global__ __launch_bounds__(512) void ns_mid_kernel(const Product p, const uint32_t per_matrix) {
+  constexpr int kSlice = 2 * kMid * 128;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * kSlice];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave >> 2, wc = wave & 3, l31 = lane & 31, lh = lane >> 5;
+  const Place at = place_of<OP>(p, per_matrix, xcd_remap(blockIdx.x, gridDim.x));
+  const long b = at.b, i0 = (long)at.ti * kMid, j0 = (long)at.tj * kMid;
+  const _Float16* src[2][2];                 // instruction q of a wave: rows (wave * 2 + q) * 8 + lane / 8
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int row = (wave * 2 + q) * 8 + (lane >> 3);
+    const int ch = (lane & 7) ^ ((row >> 1) & 7);
+    const int k = (PAIR ? ch & 3 : ch) * 8;
+    src[0][q] = (PAIR && ch >= 4 ? p.P.lo : p.P.hi) + b * p.P.next + (i0 + row) * p.P.ld + k;
+    src[1][q] = (PAIR && ch >= 4 ? p.Q.lo : p.Q.hi) + b * p.Q.next + (j0 + row) * p.Q.ld + k;
+  }
+  const int nk = p.ktiles;
+  auto stage = [&](int k) {                  // four loads a wave; behind the last slice the last one again
+    unsigned char* dst = smem + (k & 3) * kSlice + wave * 2048;
+    const long o = (long)min(k, nk - 1) * (PAIR ? 32 : 64);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[0][q] + o), (lds_void_ptr)(dst + q * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gbl_void_ptr)(src[1][q] + o), (lds_void_ptr)(dst + kMid * 128 + q * 1024), 16, 0, 0);
+    }
+  };
+  f32x16_t acc[2][2];                        // [32-row block][accumulator]
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[x >> 1][x & 1][r] = 0.f;
+  stage(0);
+  stage(1);
+  stage(2);
+  for (int k = 0; k < nk; ++k) {
+    // slices k .. k + 2 are requested: eight newer loads than slice k's may stay in flight
+    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();            // slice k has landed for every wave; slice k - 1 has been read by all ...
+    asm volatile("" ::: "memory");
+    stage(k + 3);                            // ... and its slot is free
+    const unsigned char* base = smem + (k & 3) * kSlice;
+    f16x8_t fp[2][4], fq[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int ch = (PAIR ? (c & 1) * 4 + (c >> 1) * 2 + lh : c * 2 + lh) ^ ((l31 >> 1) & 7);
+      fq[c] = *reinterpret_cast<const f16x8_t*>(base + kMid * 128 + (wc * 32 + l31) * 128 + ch * 16);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) fp[m][c] = *reinterpret_cast<const f16x8_t*>(base + (wr * 64 + m * 32 + l31) * 128 + ch * 16);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) slice_mma<PAIR>(acc[m], fq, fp[m]);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // (the requests behind the last slice, too)
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[m][0][r] += acc[m][1][r];
+  if constexpr (OP == kFinal) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const long i = i0 + wr * 64 + m * 32 + l31;
+      const float di = p.diag[b * p.diag_next + i];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float four[4] = {acc[m][0][g * 4], acc[m][0][g * 4 + 1], acc[m][0][g * 4 + 2], acc[m][0][g * 4 + 3]};
+        quad_epilogue<OP, T>(p, b, i, j0 + wc * 32 + 8 * g + 4 * lh, false, di, four);
+      }
+    }
+  } else {
+    // whole row pieces through LDS, as in the large kernel: straight from registers a wave's 64 x 32 results are 16-byte
+    // pieces of rows and 2-byte pieces of columns (22 us in place of 17 for 6 x 256 x 2304).  A wave's own 16 KiB: 64 rows of 64
+    // bytes, or 32 rows of 128 for the transpose, 16-byte chunks swizzled
+    __syncthreads();                         // every wave is past its last read of the ring
+    unsigned char* my = smem + wave * 16384;
+    const long mw = i0 + wr * 64, nw = j0 + wc * 32;
+    const auto row_at = [](int row, int col) { return row * 64 + (((col >> 3) ^ ((row >> 1) & 3)) * 16) + (col & 7) * 2; };
+    float di[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) di[m] = p.c0 + p.diag[b * p.diag_next + mw + m * 32 + l31];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[m][0][r] *= kInvScale;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      const _Float16* R = (plane ? p.R.lo : p.R.hi) + b * p.R.next + mw * p.R.ld + nw;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = q * 16 + (lane >> 2);
+        __builtin_amdgcn_global_load_lds((gbl_void_ptr)(R + row * p.R.ld + ((lane & 3) ^ ((row >> 1) & 3)) * 8),
+                                         (lds_void_ptr)(my + plane * 4096 + q * 1024), 16, 0, 0);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int o = row_at(m * 32 + l31, 8 * g + 4 * lh);
+        _Float16 h[4], l[4];
+        __builtin_memcpy(h, my + o, 8);
+        __builtin_memcpy(l, my + 4096 + o, 8);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[m][0][g * 4 + q] += di[m] * ((float)h[q] + (float)l[q]);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // hi rows, lo rows, hi of the transpose, lo of it: 4 KiB each
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const Half2 s0 = split(acc[m][0][r]), s1 = split(acc[m][0][r + 1]);
+        const uint32_t hi = pack(s0.hi, s1.hi), lo = pack(s0.lo, s1.lo);
+        const int row = m * 32 + l31, o = row_at(row, (r & 3) + 8 * (r >> 2) + 4 * lh);
+        *reinterpret_cast<uint32_t*>(my + o) = hi;
+        *reinterpret_cast<uint32_t*>(my + 4096 + o) = lo;
+        const bool odd = lane & 1;
+        const int n = ((r + (odd ? 1 : 0)) & 3) + 8 * (r >> 2) + 4 * lh, c = row & ~1;
+        const int t = n * 128 + (((c >> 3) ^ (n & 7)) * 16) + (c & 7) * 2;
+        *reinterpret_cast<uint32_t*>(my + 8192 + t) = trade_pair(hi, odd);
+        if (PAIR) *reinterpret_cast<uint32_t*>(my + 12288 + t) = trade_pair(lo, odd);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      _Float16* out = (plane ? p.out.lo : p.out.hi) + b * p.out.next + mw * p.out.ld + nw;
+      _Float16* out_t = plane ? p.out_t.lo : p.out_t.hi;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = q * 16 + (lane >> 2), ck = lane & 3;
+        *reinterpret_cast<uint4*>(out + row * p.out.ld + ck * 8) =
+            *reinterpret_cast<const uint4*>(my + plane * 4096 + row * 64 + ((ck ^ ((row >> 1) & 3)) * 16));
+        if (!PAIR && plane) continue;
+        const int n = q * 8 + (lane >> 3), ct = lane & 7;
+        *reinterpret_cast<uint4*>(out_t + b * p.out_t.next + (nw + n) * p.out_t.ld + mw + ct * 8) =
+            *reinterpret_cast<const uint4*>(my + 8192 + plane * 4096 + n * 128 + ((ct ^ (n & 7)) * 16));
+      }
+    }
+  }
+}
+
 // ================================================================================ 256 x 256 tiles
 constexpr int kLarge = 256;
 constexpr int kHalf = 128 * 128;            // bytes of a half-tile: 128 rows of a 128-byte slice
@@ -414,9 +580,8 @@ __device__ __forceinline__ int row_place(int row, int col) { return row * 128 + 
 // neighbouring lanes hold neighbouring columns of it and trade, so that each has two columns of one row (an even lane the
 // row of register r, its neighbour that of r + 1)
 __device__ __forceinline__ void to_transpose(unsigned char* my, uint32_t both, int m, int nq, int r, int lh) {
-  const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)both, 0xB1, 0xf, 0xf, true);      // lanes 1 0 3 2
   const bool odd = m & 1;
-  const uint32_t v = odd ? (other >> 16) | (both & 0xffff0000u) : (both & 0xffffu) | (other << 16);
+  const uint32_t v = trade_pair(both, odd);
   const int n = nq * 32 + ((r + (odd ? 1 : 0)) & 3) + 8 * (r >> 2) + 4 * lh;
   *reinterpret_cast<uint32_t*>(my + n * 256 + ((((m & ~1) >> 3) ^ (n & 15)) * 16) + ((m & ~1) & 7) * 2) = v;
 }
@@ -796,10 +961,15 @@ bool ns_use_large(long batch, long m, long n) {
 }
 
 template <bool PAIR, int OP, typename T>
-void product(const Product& p, long batch, bool large, hipStream_t s) {
+void product(const Product& p, long batch, bool large, bool mid, hipStream_t s) {
   const uint32_t per = OP == kGram || OP == kPoly ? (uint32_t)p.mt * (p.mt + 1) / 2 : (uint32_t)p.mt * p.nt;
   const long blocks = (long)per * batch * (OP == kGram && !large ? p.splits : 1);
   if (blocks >= (1l << 31)) throw std::invalid_argument("newton_schulz: batch too large");
+  if constexpr (OP == kApply || OP == kFinal)
+    if (mid) {
+      hipLaunchKernelGGL((ns_mid_kernel<PAIR, OP, T>), dim3((unsigned)blocks), dim3(512), 0, s, p, per);
+      return;
+    }
   if (large) hipLaunchKernelGGL((ns_large_kernel<PAIR, OP, T>), dim3((unsigned)blocks), dim3(512), 0, s, p, per);
   else hipLaunchKernelGGL((ns_small_kernel<PAIR, OP, T, OP == kGram || OP == kPoly ? 8 : 4>), dim3((unsigned)blocks), dim3(512), 0, s,
                           p, per);
@@ -809,7 +979,7 @@ void product(const Product& p, long batch, bool large, hipStream_t s) {
 
 struct Sizes {
   long m, n, mp, np;                        // X: m <= n, padded
-  bool large;
+  bool large, mid;                          // 256 x 256 tiles; else 128 x 128 ones for the products with X
   int splits;                               // of the contraction over n
   size_t x, sq, diag, norm;                 // bytes of one plane of X, of A, of a diagonal, of the partial norms
   size_t partial;                           // ... of the split sums
@@ -822,6 +992,9 @@ Sizes sizes(long batch, long rows, long cols) {
   const long tile = z.large ? kLarge : kSmall;
   z.mp = (z.m + tile - 1) / tile * tile;
   z.np = (z.n + tile - 1) / tile * tile;
+  // enough 64 x 64 tiles for two rounds of workgroups, and rows that fill 128-row tiles
+  z.mid = !z.large && z.mp % kMid == 0 && batch * (z.mp / kSmall) * (z.np / kSmall) > 512;
+  if (z.mid) z.np = (z.np + kMid - 1) / kMid * kMid;
   z.x = (size_t)batch * z.mp * z.np * 2;
   z.sq = (size_t)batch * z.mp * z.mp * 2;
   z.diag = (size_t)batch * z.mp * 4;
@@ -867,25 +1040,26 @@ void run(const NewtonSchulz& q, hipStream_t s) {
     a.diag = Da; a.diag_next = z.mp;
     a.mt = a.nt = (int)(z.mp / tile); a.ktiles = (int)(z.np / slice);
     a.splits = z.splits; a.partial = partial;
-    product<PAIR, kGram, T>(a, q.batch, z.large, s);
+    product<PAIR, kGram, T>(a, q.batch, z.large, false, s);
     Product b{};                            // B = b A + c A A
     b.P = b.Q = b.R = A;
     b.out = b.out_t = B;
     b.diag = Da; b.diag_out = Db; b.diag_next = z.mp;
     b.mt = b.nt = (int)(z.mp / tile); b.ktiles = (int)(z.mp / slice);
     b.c0 = q.b; b.c1 = q.c;
-    product<PAIR, kPoly, T>(b, q.batch, z.large, s);
+    product<PAIR, kPoly, T>(b, q.batch, z.large, false, s);
     Product c{};                            // X = a X + B X
     c.P = B; c.Q = XT[it & 1]; c.R = X;
     c.diag = Db; c.diag_next = z.mp;
-    c.mt = (int)(z.mp / tile); c.nt = (int)(z.np / tile); c.ktiles = (int)(z.mp / slice);
+    const long apply = z.mid ? kMid : tile;
+    c.mt = (int)(z.mp / apply); c.nt = (int)(z.np / apply); c.ktiles = (int)(z.mp / slice);
     c.c0 = q.a;
     if (it + 1 == q.steps) {
       c.fin = q.out; c.fin_next = q.rows * q.cols; c.rows = q.rows; c.cols = q.cols; c.turned = turned;
-      product<PAIR, kFinal, T>(c, q.batch, z.large, s);
+      product<PAIR, kFinal, T>(c, q.batch, z.large, z.mid, s);
     } else {
       c.out = X; c.out_t = XT[(it + 1) & 1];
-      product<PAIR, kApply, T>(c, q.batch, z.large, s);
+      product<PAIR, kApply, T>(c, q.batch, z.large, z.mid, s);
     }
   }
 }
