@@ -43,8 +43,8 @@ Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 template <typename T> T* data(const Tensor& t) { return t.defined() ? reinterpret_cast<T*>(t.data_ptr()) : nullptr; }
 // a parameter vector as the kernels read it
 Tensor vec32(const Tensor& t) {
-  if (!t.defined()) return t;
-  return (t.scalar_type() == at::kFloat ? t.detach() : t.detach().to(at::kFloat)).contiguous();
+  if (!t.defined() || (t.scalar_type() == at::kFloat && t.is_contiguous())) return t;
+  return t.detach().to(at::kFloat).contiguous();
 }
 Tensor floats(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options().dtype(at::kFloat)); }
 bool tracked(std::initializer_list<Tensor> ts) {
@@ -52,6 +52,11 @@ bool tracked(std::initializer_list<Tensor> ts) {
   for (const Tensor& t : ts)
     if (t.defined() && t.requires_grad()) return true;
   return false;
+}
+
+// a gradient of a gradient would silently be missing
+void once(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass is not differentiable (create_graph)");
 }
 
 // ------------------------------------------------------------------------------------------ residual norm
@@ -136,7 +141,7 @@ struct ResidualNormFn : Function<ResidualNormFn> {
     const bool pre = c.pre != kNormNone, keep_y = pre || c.post != kNormNone || gate.defined();
     ctx->save_for_backward({pre ? x : Tensor(), keep_y ? y : Tensor(), o.post_stat, o.pre_stat, post_w, post_b, pre_w, pre_b,
                             gate, v[5]});
-    ctx->saved_data["cfg"] = std::vector<int64_t>{c.post, c.pre, y.defined(), c.sinks};
+    ctx->saved_data["cfg"] = c.post | c.pre << 4 | (int64_t)y.defined() << 8 | (int64_t)c.sinks << 9;
     ctx->set_materialize_grads(false);
     variable_list out;
     if (o.s.defined()) out.push_back(o.s);
@@ -145,8 +150,10 @@ struct ResidualNormFn : Function<ResidualNormFn> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("residual_norm");
     const variable_list sv = ctx->get_saved_variables();
-    const std::vector<int64_t> cfg = ctx->saved_data["cfg"].toIntVector();
+    const int64_t packed = ctx->saved_data["cfg"].toInt();
+    const int64_t cfg[4] = {packed & 15, packed >> 4 & 15, packed >> 8 & 1, packed >> 9 & 1};
     const bool has_y = cfg[2] != 0;
     variable_list got(9);
     Tensor ds = has_y ? grads[0] : Tensor(), dh = has_y ? (grads.size() > 1 ? grads[1] : Tensor()) : grads[0];
@@ -304,6 +311,7 @@ struct RotaryFn : Function<RotaryFn> {
     return rotary_new(qkv, pos, freqs, axis, heads, interleaved, false);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("rotary");
     const variable_list sv = ctx->get_saved_variables();
     variable_list got(6);
     got[0] = rotary_new(grads[0], sv[0], sv[1], sv[2], ctx->saved_data["heads"].toInt(), ctx->saved_data["interleaved"].toBool(),
@@ -359,6 +367,7 @@ struct TokenLogprobsFn : Function<TokenLogprobsFn> {
     return {o.lp, o.ent, o.top, o.idx};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("token_logprobs");
     variable_list got(3);
     Tensor g[3];
     bool any = false;

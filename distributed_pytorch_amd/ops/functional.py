@@ -456,8 +456,11 @@ def rotary(qkv: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axis
     if inplace:
         if torch.is_grad_enabled() and qkv.requires_grad:
             raise ValueError("rotary: inplace is for calls without gradients")
-        if qkv.stride(-1) != 1 or (B > 1 and S > 0 and abs(qkv.stride(0)) < qkv.shape[-1]) \
-                or (S > 1 and abs(qkv.stride(1)) < qkv.shape[-1]):
+        # tokens of one after the other of the two axes, the outer one clear of all that the inner one covers
+        reach, ok = qkv.shape[-1], qkv.stride(-1) == 1 or qkv.shape[-1] == 1
+        for stride, size in sorted((qkv.stride(d), qkv.shape[d]) for d in (0, 1) if qkv.shape[d] > 1):
+            ok, reach = ok and stride >= reach, stride * size
+        if not ok:
             raise ValueError("rotary: inplace needs tokens that are dense and do not overlap")
     if _on_gpu(qkv):
         return _tops().rotary(qkv, positions, freqs, axis, num_heads, interleaved, inplace)
@@ -606,6 +609,8 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, k: int = 0):
         raise ValueError("token_logprobs: at most 2^30 classes")
     if not 0 <= k <= min(64, V):
         raise ValueError("token_logprobs: k must be 0 .. min(64, V), got %r" % (k,))
+    if logits.dim() == 2 and _on_gpu(logits):
+        return _tops().token_logprobs(logits, target, int(k))
     lead = target.shape
     z, t = logits.reshape(-1, V) if logits.dim() != 2 else logits, target.reshape(-1)
     if _on_gpu(z):

@@ -243,15 +243,6 @@ class FusedMuon(FusedSGD):
     def __init__(self, params, lr: float = 0.1, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True,
                  matrix_scale: float = 0.2, ns_steps: int = 5, ns_coefficients=(3.4445, -4.7750, 2.0315),
                  ns_eps: float = 1e-7):
-        from .ops.functional import _check_schulz
-
-        if not 0.0 <= momentum < 1.0:
-            raise ValueError("Invalid momentum: {}".format(momentum))
-        if weight_decay < 0.0 or matrix_scale <= 0.0:
-            raise ValueError("weight_decay must not be negative and matrix_scale positive")
-        if ns_steps < 1 or not ns_eps > 0.0:
-            raise ValueError("ns_steps must be at least 1 and ns_eps positive")
-        _check_schulz(tuple(float(v) for v in ns_coefficients), int(ns_steps))
         groups = list(params)
         if groups and not isinstance(groups[0], dict):
             groups = [g for g in (dict(params=[p for p in groups if p.dim() == 2], orthogonal=True),
@@ -264,14 +255,24 @@ class FusedMuon(FusedSGD):
         self._fill_groups()
 
     def _fill_groups(self) -> None:
+        from .ops.functional import _check_schulz
+
         for group in self.param_groups:
             for k, v in self._matrix_defaults.items():
                 group.setdefault(k, v)
+            if not 0.0 <= group["momentum"] < 1.0:
+                raise ValueError("Invalid momentum: {}".format(group["momentum"]))
+            if group["weight_decay"] < 0.0 or group["matrix_scale"] <= 0.0:
+                raise ValueError("weight_decay must not be negative and matrix_scale positive")
+            if group["ns_steps"] < 1 or not group["ns_eps"] > 0.0:
+                raise ValueError("ns_steps must be at least 1 and ns_eps positive")
+            _check_schulz(tuple(float(v) for v in group["ns_coefficients"]), int(group["ns_steps"]))
             if group["orthogonal"]:
                 group["nesterov"] = self._nesterov
-                for p in group["params"]:
-                    if p.dim() < 2:
-                        raise ValueError("FusedMuon: an orthogonal group holds matrices (2 or more dimensions)")
+                if group["dampening"] != 0:
+                    raise ValueError("FusedMuon: no dampening in an orthogonal group")
+                if any(p.dim() < 2 for p in group["params"]):
+                    raise ValueError("FusedMuon: an orthogonal group holds matrices (2 or more dimensions)")
 
     def add_param_group(self, group) -> None:
         super().add_param_group(group)

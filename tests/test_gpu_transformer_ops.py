@@ -597,6 +597,54 @@ def test_graph_of_forward_and_backward():
             z.mul_(0.5)
 
 
+def test_no_second_derivative():
+    """A gradient of a gradient is refused, not left out."""
+    case = _residual_case((2, 3, 16), torch.float32, None, "layer", None, False)
+    x = case[0].requires_grad_()
+    s, h = F().residual_norm(x, case[1], pre=case[5])
+    qkv, pos, freqs, axis = _rotary_case(1, 4, 1, 16, 8, 2, torch.float32)
+    z = normal(gen(0), (3, 20)).requires_grad_()
+    for out, leaf in ((h, x), (F().rotary(qkv.requires_grad_(), pos, freqs, axis, 1), qkv),
+                      (F().token_logprobs(z, torch.zeros(3, dtype=torch.int64, device="cuda"))[0], z)):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(out.sum(), leaf, create_graph=True)
+
+
+def test_same_tensor_twice_and_other_leaves():
+    """x as both operands, one vector for both norms and the gate, an expanded gate, a gradient that is one number."""
+    g = gen(4)
+    x = normal(g, (3, 5, 24)).requires_grad_()
+    w = normal(g, (24,), std=0.2, mean=1.0).requires_grad_()
+    n = F().Norm(w, None, 1e-5, "rms")
+    s, h = F().residual_norm(x, x, post=n, gate=w, pre=n)
+    dx, dw = torch.autograd.grad(s.sum() + 2 * h.sum(), [x, w])
+    ones = torch.ones_like(x)
+    want = ref.residual_norm(x, x, n, w, None, n, ones, 2 * ones)
+    ref.within(dx, want["d_x"][0] + want["d_y"][0], want["d_x"][1] + want["d_y"][1] + 4 * ref.E32 * want["d_x"][0].abs(), "dx")
+    total = sum(want[k][0] for k in ("d_pre_w", "d_post_w", "d_gate"))
+    ref.within(dw, total, sum(want[k][1] for k in ("d_pre_w", "d_post_w", "d_gate")) + 8 * ref.E32 * total.abs(), "dw")
+    v = normal(g, (24,)).requires_grad_()
+    s = F().residual_norm(x, x.detach(), gate=v.expand(3, 24))
+    (dv,) = torch.autograd.grad(s.sum(), v)
+    want = ref.residual_norm(x, x.detach(), None, v, None, None, ones)
+    ref.within(dv, want["d_gate"][0], 4 * want["d_gate"][1], "expanded gate")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_parameters_in_16_bits(dtype):
+    """Parameters of the activations' type (opt level O3): read in 32 bits, gradients rounded to their type."""
+    if dtype == torch.float32:
+        return
+    x, y, post, gate, scale, pre, ds, dh = _residual_case((3, 6, 40), dtype, "layer", "rms", "channel", True)
+    lo = lambda n: F().Norm(n.weight.to(dtype), None if n.bias is None else n.bias.to(dtype), n.eps, n.kind)  # noqa: E731
+    case = (x, y, lo(post), gate.to(dtype), scale, lo(pre), ds, dh)
+    want = ref.residual_norm(*case)
+    got = _residual_run(*case)
+    for name, (value, bound) in want.items():
+        assert got[name].dtype == dtype
+        ref.within(got[name], value, bound + ref.U[dtype] * value.abs(), name)
+
+
 def test_results_repeat():
     ins = _everything_inputs(3)
     first = [o.clone() for o in _everything(*ins)]

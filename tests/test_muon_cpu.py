@@ -92,8 +92,10 @@ def test_muon_refusals():
                dict(ns_eps=0.0), dict(ns_coefficients=(5.0, 1.0, 1.0))):
         with pytest.raises(ValueError):
             FusedMuon(ps, **kw)
-    with pytest.raises(ValueError):
-        FusedMuon([dict(params=[ps[2]], orthogonal=True)])
+    for group in (dict(params=[ps[2]], orthogonal=True), dict(params=[ps[0]], orthogonal=True, ns_coefficients=(5.0, 1.0, 1.0)),
+                  dict(params=[ps[0]], orthogonal=True, ns_steps=0), dict(params=[ps[0]], orthogonal=True, dampening=0.5)):
+        with pytest.raises(ValueError):
+            FusedMuon([group])
 
 
 def test_muon_groups_of_models():

@@ -122,6 +122,10 @@ def test_rotary_refusals():
     _raises(ValueError, r, qkv.clone().requires_grad_(), pos, fr, ax, 2, inplace=True)
     _raises(ValueError, r, qkv[:, :1].expand(2, 5, 48), pos, fr, ax, 2, inplace=True)
     _raises(ValueError, r, torch.randn(2, 5, 96)[..., ::2], pos, fr, ax, 2, inplace=True)
+    # tokens (0, 1) and (1, 0) in the same place
+    _raises(ValueError, r, torch.randn(6 * 48).as_strided((2, 5, 48), (48, 48, 1)), pos, fr, ax, 2, inplace=True)
+    crossed = torch.randn(5, 2, 48).transpose(0, 1)
+    assert r(crossed, pos, fr, ax, 2, inplace=True) is crossed
 
 
 def test_token_logprobs_refusals():
