@@ -343,7 +343,7 @@ LpOut lp_forward(const Tensor& z, const Tensor& t, int64_t k) {
   TokenLogprobs p;
   p.logits = z.data_ptr(); p.target = t.data_ptr<int64_t>();
   p.N = N; p.C = V; p.ld = z.stride(0); p.k = (int)k;
-  p.splits = token_logprobs_splits(N, V, code(z));
+  p.splits = token_logprobs_splits(N, V);
   Tensor stat, keys;
   if (p.splits > 1) {
     stat = floats({N, p.splits, 3}, z);

@@ -311,8 +311,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const Product p, const ui
       part = (int)(lid % (uint32_t)p.splits);
       lid /= (uint32_t)p.splits;
       const int each = (p.ktiles + p.splits - 1) / p.splits;
-      first = min(part * each, p.ktiles);
-      nk = min(first + each, p.ktiles) - first;
+      first = part * each;
+      nk = max(min(first + each, p.ktiles) - first, 0);       // (the last parts can be empty: they stage a slice, unused)
+      first = min(first, p.ktiles - 1);
     }
   const Place at = place_of<OP>(p, per_matrix, lid);
   const long b = at.b, i0 = (long)at.ti * kSmall, j0 = (long)at.tj * kSmall;
@@ -953,11 +954,24 @@ __global__ __launch_bounds__(512, 1) void ns_large_kernel(const Product p, const
   }
 }
 
-// Tile of the products, and with it the padding.
+// Tile of the products, and with it the padding: 256 x 256 where A has enough of those tiles that are not padding.  Five
+// steps, small tiles against large ones, us (tiles of A; volume: what the larger padding multiplies the products by):
+//     bf16  7 x 1024 x 4096 (70 tiles)   1170 : 1170      fp32  2492 : 2628
+//          10 x 1024 x 4096 (100)        1753 : 1463            3574 : 3185
+//          22 x 1024 x 4096 (220)        3768 : 2573            7884 : 5724
+//           5 x 1024 x 1024 (50)          388 :  534             756 : 1137
+//          64 x 448 x 1792  (192, 1.3)   1903 : 1302            3051 : 2544
+//          64 x 384 x 1536  (192, 1.8)   1073 : 1149            1897 : 2175
+//          64 x 300 x 1000  (192, 2.7)    640 :  762            1127 : 1553
+// Between volumes of 1.5 and 1.9 either side won by up to a fifth.
 bool ns_use_large(long batch, long m, long n) {
   const long mt = (m + kLarge - 1) / kLarge;
-  (void)n;
-  return batch * mt * (mt + 1) / 2 >= 96;
+  const auto volume = [&](long tile) {
+    const double mp = (double)((m + tile - 1) / tile * tile), np = (double)((n + tile - 1) / tile * tile);
+    return mp * mp * (3.0 * np + mp);
+  };
+  const double waste = volume(kLarge) / volume(kSmall);
+  return waste <= 1.6 && (double)(batch * mt * (mt + 1) / 2) >= 96.0 * waste;
 }
 
 template <bool PAIR, int OP, typename T>

@@ -17,7 +17,6 @@ namespace {
 using namespace rn;
 
 constexpr int kMaxParts = 768;      // workgroups of the pass = partial rows of the fold
-constexpr int kMaxUnits = 4096;     // parts of samples, where the gate is per sample
 
 // what a kernel is made for: s = x + y, s = x + scale * post(y) without `pre`, or everything
 enum Mode : int { kPreOnly = 0, kPostOnly = 1, kAll = 2 };

@@ -463,7 +463,7 @@ void check(long N, long C, int k) {
 }  // namespace
 
 // workgroups per row: enough of them for the card, at least 4096 elements each, and (with k <= 64) kCap keys to join
-int token_logprobs_splits(long N, long C, int) {
+int token_logprobs_splits(long N, long C) {
   long s = N <= 0 ? 1 : 512 / N;
   if (s > C / 4096) s = C / 4096;
   if (s > kCap / kTokenTopMax) s = kCap / kTokenTopMax;

@@ -73,7 +73,7 @@ struct TokenLogprobsBwd {
   int k = 0;
 };
 constexpr int kTokenTopMax = 64;
-int token_logprobs_splits(long N, long C, int dtype);
+int token_logprobs_splits(long N, long C);
 void token_logprobs_launch(const TokenLogprobs& p, int dtype, hipStream_t s);
 void token_logprobs_bwd_launch(const TokenLogprobsBwd& p, int dtype, hipStream_t s);
 

@@ -444,7 +444,8 @@ def test_newton_schulz(shape, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(96, 40, 72), (97, 256, 130), (33, 300, 513), (10, 1024, 1030), (34, 264, 136),
-                                   (33, 520, 264), (9, 1032, 1040), (6, 256, 2304), (6, 2304, 256), (20, 128, 1000), (5, 380, 1500)])
+                                   (33, 520, 264), (9, 1032, 1040), (6, 256, 2304), (6, 2304, 256), (20, 128, 1000), (5, 380, 1500),
+                                   (150, 250, 300), (110, 500, 250), (1, 128, 2112)])
 def test_newton_schulz_many_matrices(shape, dtype):
     """Enough tiles for the larger product kernels, upright and turned, rows of whole chunks and not."""
     _ns_check(normal(gen(sum(shape)), shape, dtype))
