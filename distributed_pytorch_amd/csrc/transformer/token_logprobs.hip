@@ -135,10 +135,11 @@ template <int TH> struct TopShared {
   uint64_t cand[kCap];
   uint64_t bound;
   int count;
+  int lanes, lane[8];              // lanes whose chunks are all looked at again
 };
 
 // how many of keys[0 .. n) are larger than `mine`: sixteen reads in flight (one after the other, each waits for LDS: a count
-// over 256 keys took 3.6 us)
+// over 256 keys took 3.6 us); keys has whole sixteens of room
 __device__ __forceinline__ int count_larger(const uint64_t* keys, int n, uint64_t mine) {
   int r = 0, j = 0;
   for (; j + 16 <= n; j += 16) {
@@ -148,8 +149,57 @@ __device__ __forceinline__ int count_larger(const uint64_t* keys, int n, uint64_
 #pragma unroll
     for (int u = 0; u < 16; ++u) r += v[u] > mine ? 1 : 0;
   }
-  for (; j < n; ++j) r += keys[j] > mine ? 1 : 0;
+  if (j < n) {
+    uint64_t v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) v[u] = keys[j + u];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) r += (v[u] > mine) & (j + u < n) ? 1 : 0;
+  }
   return r;
+}
+
+// A bound that at least k of the TH keys reach, and kSlack more at most; 0 if fewer than k are there.  One wave builds it
+// bit by bit from ballots, the value's bits, then (among equal values) the index's, until few enough keys reach it
+constexpr int kSlack = 16;
+template <int TH> __device__ __forceinline__ void kth_bound(const uint64_t* keys, int k, uint64_t* bound) {
+  constexpr int U = TH / 64;
+  uint32_t hi[U], lo[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint64_t key = keys[threadIdx.x + 64 * u];
+    hi[u] = (uint32_t)(key >> 32);
+    lo[u] = (uint32_t)key;
+  }
+  // a word that `need` of the words reach, and kSlack more at most (`enough`), else the largest such
+  const auto search = [&](const uint32_t (&w)[U], int need, bool& enough) {
+    uint32_t at = 0;
+    enough = false;
+    for (uint32_t bit = 0x80000000u; bit != 0 && !enough; bit >>= 1) {
+      const uint32_t t = at | bit;
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) n += __popcll(__ballot(w[u] >= t));
+      if (n >= need) {
+        at = t;
+        enough = n <= need + kSlack;
+      }
+    }
+    return at;
+  };
+  bool enough;
+  const uint32_t value = search(hi, k, enough);
+  uint32_t index = 0;
+  if (value != 0 && !enough) {
+    int larger = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      larger += __popcll(__ballot(hi[u] > value));
+      lo[u] = hi[u] == value ? lo[u] : 0;
+    }
+    index = search(lo, k - larger, enough);
+  }
+  if (threadIdx.x == 0) *bound = (uint64_t)value << 32 | index;
 }
 
 // keys of the candidates in descending order: out[r] for r < k (0 where there are fewer)
@@ -169,12 +219,16 @@ __device__ __forceinline__ void rank_out(const uint64_t* cand, int n, int k, uin
 template <typename T, int TH, typename E>
 __device__ __forceinline__ void top_of(int k, int hi, uint64_t best, bool plain, TopShared<TH>& sh, uint64_t* out, E each) {
   sh.best[threadIdx.x] = best;
-  if (threadIdx.x == 0) { sh.bound = 0; sh.count = 0; }
+  if (threadIdx.x == 0) {
+    sh.bound = 0;
+    sh.count = sh.lanes = 0;
+  }
   __syncthreads();
-  {
-    const int r = count_larger(sh.best, TH, best);
-    // with fewer than k lanes that saw anything the bound stays 0 and every element is a candidate (few, then)
-    if (best != 0 && r == k - 1) sh.bound = best;
+  // with fewer than k lanes that saw anything the bound is 0 and every element is a candidate (few, then)
+  if constexpr (TH == 64) {
+    if (best != 0 && count_larger(sh.best, TH, best) == k - 1) sh.bound = best;
+  } else {
+    if (threadIdx.x < 64) kth_bound<TH>(sh.best, k, &sh.bound);
   }
   __syncthreads();
   for (;;) {
@@ -182,14 +236,18 @@ __device__ __forceinline__ void top_of(int k, int hi, uint64_t best, bool plain,
     const float least = plain && bound != 0 ? order_value((uint32_t)(bound >> 32)) : -INFINITY;
     each(least, [&](const Vec16<T>& v, int c) {
       if (chunk_max(v) < least) return;
+      uint32_t take = 0;
 #pragma unroll
-      for (int j = 0; j < Vec16<T>::N; ++j) {
-        const uint64_t key = make_key(v.get(j), c + j);
-        if (key >= bound && c + j < hi) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCap) sh.cand[at] = key;
+      for (int j = 0; j < Vec16<T>::N; ++j)
+        if (make_key(v.get(j), c + j) >= bound && c + j < hi) take |= 1u << j;
+      if (take == 0) return;
+      int at = atomicAdd(&sh.count, __popc(take));       // (one wait for LDS in place of one per element)
+#pragma unroll
+      for (int j = 0; j < Vec16<T>::N; ++j)
+        if (take >> j & 1u) {
+          if (at < kCap) sh.cand[at] = make_key(v.get(j), c + j);
+          ++at;
         }
-      }
     });
     __syncthreads();
     const int n = sh.count;
@@ -198,7 +256,7 @@ __device__ __forceinline__ void top_of(int k, int hi, uint64_t best, bool plain,
       return;
     }
     __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x == 0) sh.count = sh.lanes = 0;
     for (int i = threadIdx.x; i < kCap; i += TH) {
       const uint64_t mine = sh.cand[i];
       if (count_larger(sh.cand, kCap, mine) == k - 1) sh.bound = mine;
@@ -295,6 +353,12 @@ __global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs 
       for (int j = 0; j < V; ++j) a.add(x.get(j));
     });
   }
+  // the lane's largest chunks again, on their way while the sums meet
+  Vec16<T> b1, b2;
+  if (p.k > 0 && c0 < hi) {
+    b1 = load_chunk(z, where, hi);
+    if constexpr (Q == 0) b2 = load_chunk(z, where2, hi);
+  }
   // lanes, then waves, in a fixed order
   a.join_wave();
   if constexpr (TH > 64) {
@@ -306,11 +370,10 @@ __global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs 
   if (p.k > 0) {
     uint64_t best = 0;
     if (c0 < hi) {
-      const Vec16<T> b = load_chunk(z, where, hi);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (where + j < hi) {
-          const uint64_t key = make_key(b.get(j), where + j);
+          const uint64_t key = make_key(b1.get(j), where + j);
           best = key > best ? key : best;
         }
     }
@@ -329,11 +392,27 @@ __global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs 
       });
     else
       top_of<T, TH>(p.k, hi, best, plain, sh, out, [&](float least, auto f) {
-        if (third >= least || least == -INFINITY) {
+        if (least == -INFINITY) {
           walk<T, TH>(z, (int)lo, (int)hi, f);
+          return;
+        }
+        // a lane that walks its chunks alone keeps the workgroup waiting for all of their latencies: a few such lanes are
+        // shared out, a chunk a lane
+        const bool all = third >= least;
+        if (all) {
+          const int at = atomicAdd(&sh.lanes, 1);
+          if (at < 8) sh.lane[at] = threadIdx.x;
         } else {
-          if (first >= least) f(load_chunk(z, where, hi), where);
-          if (second >= least) f(load_chunk(z, where2, hi), where2);
+          if (first >= least) f(b1, where);
+          if (second >= least) f(b2, where2);
+        }
+        __syncthreads();
+        const int lanes = sh.lanes;
+        if (lanes <= 8) {
+          for (int i = 0; i < lanes; ++i)
+            for (int c = lo + (sh.lane[i] + (int)threadIdx.x * TH) * V; c < hi; c += TH * TH * V) f(load_chunk(z, c, hi), c);
+        } else if (all) {
+          walk<T, TH>(z, (int)lo, (int)hi, f);
         }
       });
   }
@@ -375,11 +454,12 @@ __global__ __launch_bounds__(kJoin) void token_logprobs_join_kernel(const TokenL
   write_row<T>(p, row, valid, zt, a, top);
 }
 
-// one part of a row; elements that carry a gradient of their own are found through a bit per 8 columns
+// One part of a row.  The elements that carry a gradient of their own (the target and the k listed ones) are few: the pass
+// writes all elements without them, and a lane each then writes those again.  (Looking for them in the pass, by a bit per 8
+// columns, took 26 of 124 us of 2048 x 50257 bf16 with k = 20: nearly every row has waves that stop for them.)
 template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogprobsBwd p, const int splits, const bool stream) {
   constexpr int V = 16 / (int)sizeof(T);
-  __shared__ uint32_t marked[1024];
   __shared__ long idx[kTokenTopMax + 1];
   __shared__ float gx[kTokenTopMax + 1];
   const long row = blockIdx.x / splits;
@@ -388,63 +468,51 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogp
   T* dz = reinterpret_cast<T*>(p.dlogits) + row * p.C;
   const long each = part_of(p.C, splits);
   const int lo = (int)min(part * each, p.C), hi = (int)min(lo + each, p.C);
-  for (int i = threadIdx.x; i < 1024; i += 256) marked[i] = 0;
+  const float m = p.norm[2 * row], ls = p.norm[2 * row + 1], H = p.entropy[row];
   const long t = p.target[row];
   const bool valid = t >= 0 && t < p.C;
   const float glp = p.d_logprob != nullptr && valid ? p.d_logprob[row] : 0.f;
   const float ge = p.d_entropy != nullptr ? p.d_entropy[row] : 0.f;
-  const int k = p.d_top != nullptr ? p.k : 0;
-  if ((int)threadIdx.x < k) {
-    idx[threadIdx.x] = p.index[row * p.k + threadIdx.x];
-    gx[threadIdx.x] = p.d_top[row * p.k + threadIdx.x];
+  const int k = p.d_top != nullptr ? p.k : 0, tid = threadIdx.x;
+  long at = -1;                                    // this lane's own element
+  if (tid <= k) {
+    at = tid < k ? p.index[row * p.k + tid] : (valid ? t : -1);
+    idx[tid] = at;
+    gx[tid] = tid < k ? p.d_top[row * p.k + tid] : glp;
   }
-  if (threadIdx.x == 255) { idx[k] = valid ? t : -1; gx[k] = glp; }
+  if (at < lo || at >= hi) at = -1;
+  const float own = at >= 0 ? to_float(z[at]) : 0.f;
   __syncthreads();
   float gsum = glp;
   for (int j = 0; j < k; ++j) gsum += gx[j];
-  if ((int)threadIdx.x <= k && idx[threadIdx.x] >= 0) {
-    const uint32_t bit = (uint32_t)((idx[threadIdx.x] >> 3) & 32767);
-    atomicOr(&marked[bit >> 5], 1u << (bit & 31));
-  }
-  __syncthreads();
-  const float m = p.norm[2 * row], ls = p.norm[2 * row + 1], H = p.entropy[row];
   const bool empty = ls == -INFINITY;              // a row that is masked altogether
+  if (empty) {
+    for (int i = lo + tid; i < hi; i += 256) dz[i] = from_float<T>(0.f);
+    return;
+  }
   // p (-gsum - ge (log p + H)) with log p = d - ls, d = z - m; where p is 0 d is kept finite
   const float c0 = -gsum - ge * H + ge * ls, shift = -ls * kLog2e;
-  auto chunk = [&](const Vec16<T>& v, int c) {
-    float g[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float d = v.get(j) - m;
-      g[j] = __builtin_amdgcn_exp2f(fmaf(d, kLog2e, shift)) * fmaf(-ge, fmaxf(d, -1e30f), c0);
-    }
-    const uint32_t bit = (uint32_t)((c >> 3) & 32767);         // (a chunk lies within 8 columns)
-    if ((marked[bit >> 5] >> (bit & 31)) & 1u)
-      for (int i = 0; i <= k; ++i) {
-        const long at = idx[i] - c;
-#pragma unroll
-        for (int j = 0; j < V; ++j) g[j] += at == j ? gx[i] : 0.f;
-      }
+  const auto grad = [&](float v) {
+    const float d = v - m;
+    return __builtin_amdgcn_exp2f(fmaf(d, kLog2e, shift)) * fmaf(-ge, fmaxf(d, -1e30f), c0);
+  };
+  const auto chunk = [&](const Vec16<T>& v) {
     Vec16<T> o;
 #pragma unroll
-    for (int j = 0; j < V; ++j) o.set(j, g[j]);
+    for (int j = 0; j < V; ++j) o.set(j, grad(v.get(j)));
     return o;
   };
   constexpr int U = 4, kStep = 256 * V;            // chunks in flight per lane
-  int c = lo + (int)threadIdx.x * V;
-  if (empty) {
-    for (int i = lo + (int)threadIdx.x; i < hi; i += 256) dz[i] = from_float<T>(0.f);
-    return;
-  }
+  int c = lo + tid * V;
   for (; c + (U - 1) * kStep + V <= hi; c += U * kStep) {
     Vec16<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = load_any(z + c + u * kStep);
 #pragma unroll
-    for (int u = 0; u < U; ++u) store_any(chunk(v[u], c + u * kStep), dz + c + u * kStep, stream);
+    for (int u = 0; u < U; ++u) store_any(chunk(v[u]), dz + c + u * kStep, stream);
   }
   for (; c < hi; c += kStep) {
-    const Vec16<T> o = chunk(load_chunk(z, c, hi), c);
+    const Vec16<T> o = chunk(load_chunk(z, c, hi));
     if (c + V <= hi) {
       store_any(o, dz + c, stream);
     } else {
@@ -453,6 +521,16 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogp
         if (c + j < hi) dz[c + j] = from_float<T>(o.get(j));
     }
   }
+  float g = grad(own);
+  if (at >= 0)
+    for (int j = 0; j <= k; ++j) {
+      if (idx[j] != at) continue;
+      g += gx[j];
+      if (j < tid) at = -2;                        // (an element listed twice is written by the first lane that has it)
+    }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the pass has written, streaming stores too
+  __syncthreads();
+  if (at >= 0) dz[at] = from_float<T>(g);
 }
 
 void check(long N, long C, int k) {
