@@ -342,6 +342,27 @@ def test_token_logprobs_ties_and_orders(V, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("crowd", [(0,), (255,), (3, 64, 65, 66, 67, 68, 69, 250), tuple(range(100, 112)), tuple(range(256))])
+def test_token_logprobs_crowded_lanes(crowd, dtype):
+    """Whole rows of a workgroup (many rows), the largest values in chunks that few lanes visit, several chunks each."""
+    N, V, k = 520, 34001, 40
+    g = gen(len(crowd))
+    step = 16 // (torch.finfo(dtype).bits // 8)
+    lane = torch.arange(V, device="cuda") // step % 256
+    z = normal(g, (N, V), torch.float32)
+    z[1] += torch.where(torch.isin(lane, torch.tensor(crowd, device="cuda")), 9.0, 0.0)
+    z[N - 1] += torch.where(torch.isin(lane, torch.tensor(crowd, device="cuda")), 3.0, 0.0)
+    z = z.to(dtype)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    out = F().token_logprobs(z, t, k)
+    rows = torch.tensor([0, 1, N - 1], device="cuda")
+    want = ref.token_logprobs(z[rows], t[rows], k)
+    assert torch.equal(out[3][rows].cpu(), want["index"][0])
+    for name, got in zip(("logprob", "entropy", "top"), out):
+        ref.within(got[rows], *want[name], name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [9, 3000, 40000])
 def test_token_logprobs_masks(V, dtype):
     g = gen(V)
