@@ -207,7 +207,7 @@ class FusedSGD(Optimizer):
 def muon_groups(model) -> list:
     """Parameter groups for ``FusedMuon``: the matrices inside the network are orthogonalised (Linear weights,
     attention projections, dense convolution filters as ``[K, C * R * S]``); the first convolution, the classifier,
-    embeddings, depthwise filters, biases and norms take plain SGD."""
+    embeddings, position bias tables, depthwise filters, biases and norms take plain SGD."""
     from .nn.modules import Conv2d, Linear
 
     convs = [m for m in model.modules() if isinstance(m, Conv2d)]
@@ -216,11 +216,12 @@ def muon_groups(model) -> list:
     last = linears[-1].weight if linears else (convs[-1].weight if convs else None)
     grouped = {id(m.weight) for m in convs if m.groups > 1}
     matrices, rest = [], []
-    for p in model.parameters():
+    tables = {id(m.weight) for m in model.modules() if isinstance(m, torch.nn.Embedding)}
+    for name, p in model.named_parameters():
         if not p.requires_grad:
             continue
-        inside = p.dim() in (2, 4) and p is not first and p is not last and id(p) not in grouped \
-            and min(p.shape[0], p.numel() // p.shape[0]) > 1
+        inside = name.endswith("weight") and p.dim() in (2, 4) and p is not first and p is not last \
+            and id(p) not in grouped and id(p) not in tables and min(p.shape[0], p.numel() // p.shape[0]) > 1
         (matrices if inside else rest).append(p)
     return [g for g in (dict(params=matrices, orthogonal=True), dict(params=rest, orthogonal=False)) if g["params"]]
 

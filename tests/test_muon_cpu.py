@@ -183,3 +183,17 @@ def test_trainer_with_muon_and_predictions(tmp_path):
         assert l["logprob"] <= 0.0 and l["top_logprob"] == sorted(l["top_logprob"], reverse=True)
         if l["target"] in l["top"]:
             assert l["logprob"] == pytest.approx(l["top_logprob"][l["top"].index(l["target"])], abs=1e-6)
+
+
+@pytest.mark.parametrize("arch", ["swin_t", "swin_v2_t", "vit_b_32"])
+def test_groups_hold_products_only(arch):
+    """Every orthogonalised parameter is the weight of a product: no position table, embedding, token or norm is one."""
+    model = models.create_model(arch)
+    names = {id(p): n for n, p in model.named_parameters()}
+    groups = muon_groups(model)
+    assert sum(len(g["params"]) for g in groups) == len(names)
+    for p in groups[0]["params"]:
+        assert names[id(p)].endswith("weight") and p.dim() in (2, 4)
+    rest = {names[id(p)] for p in groups[1]["params"]}
+    assert not any(n.endswith("bias_table") for n in names.values()) or any(n.endswith("bias_table") for n in rest)
+    assert not any("bias_table" in names[id(p)] or "pos_embedding" in names[id(p)] for p in groups[0]["params"])
