@@ -381,7 +381,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post: Optional[Norm] = No
     ``gate``: learnable, ``[C]`` (layer scale) or ``[N, C]`` (a conditioned block).  ``scale``: ``[N]``, a constant for
     each sample (stochastic depth: 0 or 1 / keep; a dropped sample's branch still has to be finite).  Returns ``s``, or
     ``(s, h)`` with ``pre``.  Everything between the inputs and the results is 32-bit arithmetic, rounded once: ``h`` is
-    the norm of the unrounded sum.  On the GPU one pass per direction (``csrc/kernels/residual_norm*.hip``), any ``C`` up
+    the norm of the unrounded sum.  On the GPU one pass per direction (``csrc/transformer/residual_norm*.hip``), any ``C`` up
     to 16384 (16-bit types; 8192 in float32)."""
     _check_rows("residual_norm", x)
     if x.dim() < 2 or y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
