@@ -13,7 +13,7 @@
 // order of collection.  If more than the list's capacity reach the bound (many large elements with one lane), the k-th
 // largest collected becomes the new bound and the row is looked at again.  Few long rows are split over workgroups and
 // joined.  Bound by memory bandwidth: 2048 x 50257 bf16 with k = 20 73 us behind a backward pass's writes (54 us alone, of
-// which the k largest take 14), backward 86 us (4.8 TB/s); 1024 x 1000 fp32 8 + 6 us; one row of 128000 fp32 11 us and 7 to
+// which the k largest take 14), backward 86 us (4.8 TB/s); 1024 x 1000 fp32 8 + 6 us; one row of 128000 fp32 10 us and 5 to
 // join, bound by latency.
 #include "../common.h"
 #include "transformer.h"
@@ -180,12 +180,12 @@ template <int TH> __device__ __forceinline__ void kth_bound(const uint64_t* keys
     enough = false;
     for (uint32_t bit = 0x80000000u; bit != 0 && !enough; bit >>= 1) {
       const uint32_t t = at | bit;
-      int n = 0;
+      int reach = 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) n += __popcll(__ballot(w[u] >= t));
-      if (n >= need) {
+      for (int u = 0; u < U; ++u) reach += __popcll(__ballot(w[u] >= t));
+      if (reach >= need) {
         at = t;
-        enough = n <= need + kSlack;
+        enough = reach <= need + kSlack;
       }
     }
     return at;
@@ -430,21 +430,25 @@ __global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs 
   write_row<T>(p, row, valid, zt, a, top);
 }
 
-// joins the parts of a row: one workgroup per row, a lane per key where there are many
-constexpr int kJoin = 512;
+// joins the parts of a row: one workgroup per row.  The parts' lists are in descending order, so where m of them have a t-th
+// key that reaches a bound, m t keys do: with m t >= k the m-th largest of the t-th keys is one.  Few more than k keys reach
+// it, and only those are ranked.
+constexpr int kJoin = 512, kParts = 32;
 template <typename T>
 __global__ __launch_bounds__(kJoin) void token_logprobs_join_kernel(const TokenLogprobs p) {
-  __shared__ uint64_t cand[kCap];
+  __shared__ uint64_t keys[kParts * kTokenTopMax], cand[kParts * kTokenTopMax], bound;
   __shared__ uint64_t top[kTokenTopMax];
+  __shared__ int count;
   const long row = blockIdx.x;
   const long t = p.target[row];                    // (early: two loads that follow each other)
   const bool valid = t >= 0 && t < p.C;
   const float zt = valid ? to_float(reinterpret_cast<const T*>(p.logits)[row * p.ld + t]) : 0.f;
-  const int n = p.splits * p.k;                    // at most kCap
-  for (int i = threadIdx.x; i < n; i += kJoin) cand[i] = p.keys[row * n + i];
+  const int n = p.splits * p.k;
+  for (int i = threadIdx.x; i < n; i += kJoin) keys[i] = p.keys[row * n + i];
+  if (threadIdx.x == 0) count = 0;
   RunSums a;
   a.clear();
-  const int lane = threadIdx.x & 63;               // (at most 64 parts, one a lane)
+  const int lane = threadIdx.x & 63;               // (one part a lane)
   if (lane < p.splits) {
     const float* st = p.stat + (row * p.splits + lane) * 3;
     a.m = st[0]; a.s = st[1]; a.u = st[2];
@@ -452,7 +456,24 @@ __global__ __launch_bounds__(kJoin) void token_logprobs_join_kernel(const TokenL
   a.join_wave();
   __syncthreads();
   // (an absent key, 0, is below all others and never among the first k of C >= k elements)
-  rank_out(cand, n, p.k, top);
+  if (p.k > 0) {
+    const int depth = (p.k + p.splits - 1) / p.splits, m = (p.k + depth - 1) / depth;
+    if ((int)threadIdx.x < p.splits) {
+      const uint64_t mine = keys[threadIdx.x * p.k + depth - 1];
+      int r = 0;                                   // (absent keys are equal: the lower part comes first)
+#pragma unroll 8
+      for (int q = 0; q < p.splits; ++q) {
+        const uint64_t other = keys[q * p.k + depth - 1];
+        r += other > mine || (other == mine && q < (int)threadIdx.x) ? 1 : 0;
+      }
+      if (r == m - 1) bound = mine;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kJoin)
+      if (keys[i] >= bound) cand[atomicAdd(&count, 1)] = keys[i];
+    __syncthreads();
+    rank_out(cand, count, p.k, top);
+  }
   __syncthreads();
   write_row<T>(p, row, valid, zt, a, top);
 }
@@ -543,18 +564,20 @@ void check(long N, long C, int k) {
 
 }  // namespace
 
-// workgroups per row: enough of them for the card, at least 4096 elements each, and (with k <= 64) kCap keys to join
+// workgroups per row: enough of them for the card, of at least 2048 elements each.  A row below 8192 stays whole: the join costs
+// more than the shorter parts save (one row of 4200 bf16, k = 5: 9.5 us whole, 12.0 in two; of 128000, k = 20: 18.7 in 16
+// parts, 15.8 in 32)
 int token_logprobs_splits(long N, long C) {
-  long s = N <= 0 ? 1 : 512 / N;
-  if (s > C / 4096) s = C / 4096;
-  if (s > kCap / kTokenTopMax) s = kCap / kTokenTopMax;
+  long s = N <= 0 || C < 8192 ? 1 : 512 / N;
+  if (s > C / 2048) s = C / 2048;
+  if (s > kParts) s = kParts;
   return (int)(s < 1 ? 1 : s);
 }
 
 void token_logprobs_launch(const TokenLogprobs& p, int dtype, hipStream_t s) {
   check(p.N, p.C, p.k);
   if (p.N == 0) return;
-  if (p.splits < 1 || p.splits * p.k > kCap || p.N * p.splits >= (1l << 31))
+  if (p.splits < 1 || p.splits > kParts || p.N * p.splits >= (1l << 31))
     throw std::invalid_argument("token_logprobs: splits");
   const long part = part_of(p.C, p.splits) < p.C ? part_of(p.C, p.splits) : p.C;
   const dim3 grid((unsigned)(p.N * p.splits));
