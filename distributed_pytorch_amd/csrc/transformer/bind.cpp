@@ -2,7 +2,8 @@
 //
 // A training step of a small batch is bound by the host: as Python autograd functions a forward and backward call of one
 // of these operators took 120 - 200 us of host time around 25 - 60 us of kernels.  So this module, unlike _C, is built
-// against torch's headers.  Arguments are checked in ops/functional.py.
+// against torch's headers.  Arguments are checked here (a few tenths of a microsecond; in Python 3 to 5 of the 7 that a small
+// call takes): an operator returns None for what it does not take, and ops/functional.py then says what is wrong.
 //
 // Outputs and workspaces come from torch's allocator per call and launches go to torch's current stream of the tensors'
 // device: nothing is shared between two calls or two graphs, and nothing synchronises with the host.
@@ -52,6 +53,23 @@ bool tracked(std::initializer_list<Tensor> ts) {
   for (const Tensor& t : ts)
     if (t.defined() && t.requires_grad()) return true;
   return false;
+}
+
+// ---- what ops/functional.py checks, argument by argument
+bool float_type(const Tensor& t) {
+  const auto d = t.scalar_type();
+  return d == at::kFloat || d == at::kBFloat16 || d == at::kHalf;
+}
+bool rows_taken(const Tensor& x) {
+  return float_type(x) && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) * (int64_t)x.element_size() <= 2048 * 16;
+}
+bool vector_taken(const Tensor& t, const Tensor& x) {
+  return t.dim() == 1 && t.size(0) == x.size(-1) && t.device() == x.device();
+}
+bool norm_taken(const OptTensor& w, const OptTensor& b, int64_t kind, double eps, const Tensor& x) {
+  if (!w.has_value()) return kind == kNormNone;
+  return (kind == kNormLayer || (kind == kNormRms && !b.has_value())) && vector_taken(*w, x) &&
+         (!b.has_value() || vector_taken(*b, x)) && eps >= 0.0;
 }
 
 // a gradient of a gradient would silently be missing
@@ -257,11 +275,22 @@ struct ResidualNormFn : Function<ResidualNormFn> {
   }
 };
 
-// -> (s, h), None where there is none
-std::pair<OptTensor, OptTensor> residual_norm(const Tensor& x, const OptTensor& y, const OptTensor& post_w,
+// -> (s, h), None where there is none; None for arguments that it does not take
+std::optional<std::pair<OptTensor, OptTensor>> residual_norm(const Tensor& x, const OptTensor& y, const OptTensor& post_w,
                                               const OptTensor& post_b, int64_t post, double post_eps, const OptTensor& pre_w,
                                               const OptTensor& pre_b, int64_t pre, double pre_eps, const OptTensor& gate,
                                               const OptTensor& scale, bool sinks) {
+  if (!x.is_cuda() || !rows_taken(x) || !norm_taken(post_w, post_b, post, post_eps, x) || !norm_taken(pre_w, pre_b, pre, pre_eps, x))
+    return std::nullopt;
+  if (y.has_value()) {
+    if (x.dim() < 2 || y->sizes() != x.sizes() || y->scalar_type() != x.scalar_type() || y->device() != x.device()) return std::nullopt;
+    if (gate.has_value() &&
+        !(vector_taken(*gate, x) || (gate->dim() == 2 && gate->size(0) == x.size(0) && gate->size(1) == x.size(-1) && gate->device() == x.device())))
+      return std::nullopt;
+    if (scale.has_value() &&
+        (scale->dim() != 1 || scale->size(0) != x.size(0) || scale->device() != x.device() || scale->requires_grad()))
+      return std::nullopt;
+  }
   const Tensor Y = given(y), pw = given(post_w), pb = given(post_b), qw = given(pre_w), qb = given(pre_b), g = given(gate),
                sc = given(scale);
   const NormCfg c{post, pre, post_eps, pre_eps, sinks};
@@ -269,11 +298,11 @@ std::pair<OptTensor, OptTensor> residual_norm(const Tensor& x, const OptTensor& 
   if (!tracked({x, Y, pw, pb, qw, qb, g})) {
     const RnOut o = rn_forward(x.contiguous(), dense(Y), {vec32(pw), vec32(pb), vec32(qw), vec32(qb), vec32(g), vec32(sc)}, c,
                                false);
-    return {opt(o.s), opt(o.h)};
+    return std::make_pair(opt(o.s), opt(o.h));
   }
   variable_list out = ResidualNormFn::apply(x, y, post_w, post_b, pre_w, pre_b, gate, scale, c);
-  if (!Y.defined()) return {OptTensor(), out[0]};
-  return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
+  if (!Y.defined()) return std::make_pair(OptTensor(), OptTensor(out[0]));
+  return std::make_pair(OptTensor(out[0]), out.size() > 1 ? OptTensor(out[1]) : OptTensor());
 }
 
 // ------------------------------------------------------------------------------------------ rotary
@@ -320,8 +349,24 @@ struct RotaryFn : Function<RotaryFn> {
   }
 };
 
-Tensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs, const Tensor& axis, int64_t heads,
-              bool interleaved, bool inplace) {
+bool rotary_taken(const Tensor& qkv, const Tensor& pos, const Tensor& freqs, const Tensor& axis, int64_t heads) {
+  if (!qkv.is_cuda() || !float_type(qkv) || qkv.dim() != 3 || heads < 1 || qkv.size(2) == 0 || qkv.size(2) % (3 * heads) != 0)
+    return false;
+  const int64_t d = pos.dim();
+  if ((d != 2 && d != 3) || pos.size(d - 2) != qkv.size(1) || (d == 3 && pos.size(0) != qkv.size(0)) || pos.size(d - 1) < 1)
+    return false;
+  const auto pt = pos.scalar_type(), ft = freqs.scalar_type(), at = axis.scalar_type();
+  if ((pt != at::kLong && pt != at::kInt && pt != at::kFloat && pt != at::kDouble) || (ft != at::kFloat && ft != at::kDouble) ||
+      (at != at::kInt && at != at::kLong))
+    return false;
+  return freqs.dim() == 1 && axis.sizes() == freqs.sizes() && 2 * freqs.numel() <= qkv.size(2) / (3 * heads) &&
+         freqs.numel() <= 4096 && pos.device() == qkv.device() && freqs.device() == qkv.device() &&
+         axis.device() == qkv.device() && !pos.requires_grad() && !freqs.requires_grad();
+}
+// (`inplace`: its strides have been checked)
+OptTensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs, const Tensor& axis, int64_t heads,
+                 bool interleaved, bool inplace) {
+  if (!rotary_taken(qkv, positions, freqs, axis, heads)) return std::nullopt;
   const Tensor pos = positions.contiguous(), f = freqs.contiguous(), a = axis.to(at::kInt).contiguous();
   if (inplace) {
     rotary_run(qkv, qkv, pos, f, a, heads, interleaved, false);
@@ -329,7 +374,7 @@ Tensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs, c
     return qkv;
   }
   if (!tracked({qkv})) return rotary_new(qkv, pos, f, a, heads, interleaved, false);
-  return RotaryFn::apply(qkv, pos, f, a, heads, interleaved);
+  return OptTensor(RotaryFn::apply(qkv, pos, f, a, heads, interleaved));
 }
 
 // ------------------------------------------------------------------------------------------ log probabilities
@@ -392,14 +437,20 @@ struct TokenLogprobsFn : Function<TokenLogprobsFn> {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& target, int64_t k) {
+// logits [N, V]
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const Tensor& logits, const Tensor& target, int64_t k) {
+  const auto type = target.scalar_type();
+  if (!logits.is_cuda() || !float_type(logits) || logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > 1l << 30 ||
+      target.dim() != 1 || target.size(0) != logits.size(0) || target.device() != logits.device() ||
+      (type != at::kLong && type != at::kInt && type != at::kShort && type != at::kByte) || k < 0 || k > 64 || k > logits.size(1))
+    return std::nullopt;
   const Tensor t = target.to(at::kLong).contiguous();
   if (!tracked({logits})) {
     const LpOut o = lp_forward(logits.stride(1) == 1 ? logits : logits.contiguous(), t, k);
-    return {o.lp, o.ent, o.top, o.idx};
+    return std::make_tuple(o.lp, o.ent, o.top, o.idx);
   }
   variable_list o = TokenLogprobsFn::apply(logits, t, k);
-  return {o[0], o[1], o[2], o[3]};
+  return std::make_tuple(o[0], o[1], o[2], o[3]);
 }
 
 // ------------------------------------------------------------------------------------------ Newton-Schulz and Muon

@@ -364,6 +364,11 @@ def _check_rows(name: str, x: torch.Tensor) -> None:
         raise ValueError("%s: at most %d channels in %s" % (name, most, x.dtype))
 
 
+def _never_on_gpu(name: str, x: torch.Tensor) -> None:
+    if _on_gpu(x):
+        raise RuntimeError("%s: arguments that the kernels do not take" % name)
+
+
 def _norm_reference(v: torch.Tensor, norm: Norm) -> torch.Tensor:
     if norm.kind == "layer":
         return TF.layer_norm(v, (v.shape[-1],), norm.weight.float(), None if norm.bias is None else norm.bias.float(), norm.eps)
@@ -383,6 +388,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post: Optional[Norm] = No
     ``(s, h)`` with ``pre``.  Everything between the inputs and the results is 32-bit arithmetic, rounded once: ``h`` is
     the norm of the unrounded sum.  On the GPU one pass per direction (``csrc/transformer/residual_norm*.hip``), any ``C`` up
     to 16384 (16-bit types; 8192 in float32)."""
+    if _on_gpu(x):
+        out = _tops().residual_norm(x, y, post, gate, scale, pre)
+        if out is not None:
+            return out                              # (what it does not take is named here)
     _check_rows("residual_norm", x)
     if x.dim() < 2 or y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
         raise ValueError("residual_norm: x and y must be [N, ..., C] of the same shape, dtype and device")
@@ -398,8 +407,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post: Optional[Norm] = No
             raise ValueError("residual_norm: scale must be [N] on the input's device")
         if scale.requires_grad:
             raise ValueError("residual_norm: scale is a constant (use a gate for a learnable factor)")
-    if _on_gpu(x):
-        return _tops().residual_norm(x, y, post, gate, scale, pre)
+    _never_on_gpu("residual_norm", x)
     z = y.float()
     if post is not None:
         z = _norm_reference(z, post)
@@ -415,11 +423,14 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post: Optional[Norm] = No
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """RMSNorm over the last axis: ``x / sqrt(mean(x^2) + eps) * weight``."""
+    if _on_gpu(x):
+        out = _tops().rms_norm(x, weight, eps)
+        if out is not None:
+            return out
     _check_rows("rms_norm", x)
     norm = Norm(weight, None, eps, "rms")
     _check_norm("rms_norm", norm, x)
-    if _on_gpu(x):
-        return _tops().rms_norm(x, weight, eps)
+    _never_on_gpu("rms_norm", x)
     return _norm_reference(x.float(), norm).to(x.dtype)
 
 
@@ -433,6 +444,10 @@ def rotary(qkv: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axis
     or float64; ``axis``: ``[P]`` whole numbers in ``[0, A)`` (an entry outside turns its pair into NaN).  Angles are
     formed in 64 bits.  ``inplace`` (without gradients) overwrites ``qkv``.  ``nn.AxialRotary`` holds ``freqs`` and
     ``axis`` for the usual splits of a head."""
+    if not inplace and _on_gpu(qkv):
+        out = _tops().rotary(qkv, positions, freqs, axis, num_heads, interleaved, False)
+        if out is not None:
+            return out
     if qkv.dtype not in _NORM_DTYPES:
         raise TypeError("rotary: float32, bfloat16 or float16 expected, got %s" % (qkv.dtype,))
     if qkv.dim() != 3 or num_heads < 1 or qkv.shape[-1] % (3 * num_heads) or qkv.shape[-1] == 0:
@@ -462,8 +477,9 @@ def rotary(qkv: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axis
             ok, reach = ok and stride >= reach, stride * size
         if not ok:
             raise ValueError("rotary: inplace needs tokens that are dense and do not overlap")
-    if _on_gpu(qkv):
-        return _tops().rotary(qkv, positions, freqs, axis, num_heads, interleaved, inplace)
+    if inplace and _on_gpu(qkv):
+        return _tops().rotary(qkv, positions, freqs, axis, num_heads, interleaved, True)
+    _never_on_gpu("rotary", qkv)
     P = freqs.numel()
     ok = (axis >= 0) & (axis < positions.shape[-1])
     angle = positions.double()[..., axis.long().clamp(0, positions.shape[-1] - 1)] * freqs.double()
@@ -596,6 +612,10 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, k: int = 0):
     A logit of -inf (a masked class) has probability zero and adds nothing.  A row that is masked altogether has entropy
     0, log probabilities -inf and no gradient.  A ``target`` outside ``[0, V)`` is ignored: its log probability is 0 and
     carries no gradient, the row's other results are as usual.  A row with a NaN or a +inf gives NaN."""
+    if _on_gpu(logits):
+        out = _tops().token_logprobs(logits, target, k)
+        if out is not None:
+            return out                              # [N, V]
     if logits.dtype not in _NORM_DTYPES:
         raise TypeError("token_logprobs: float32, bfloat16 or float16 expected, got %s" % (logits.dtype,))
     if logits.dim() < 1 or logits.shape[-1] < 1 or logits.shape[:-1] != target.shape:
@@ -609,8 +629,6 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, k: int = 0):
         raise ValueError("token_logprobs: at most 2^30 classes")
     if not 0 <= k <= min(64, V):
         raise ValueError("token_logprobs: k must be 0 .. min(64, V), got %r" % (k,))
-    if logits.dim() == 2 and _on_gpu(logits):
-        return _tops().token_logprobs(logits, target, int(k))
     lead = target.shape
     z, t = logits.reshape(-1, V) if logits.dim() != 2 else logits, target.reshape(-1)
     if _on_gpu(z):

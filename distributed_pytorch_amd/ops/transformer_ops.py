@@ -1,5 +1,6 @@
 """GPU side of the transformer-block operators: ``csrc/transformer`` does allocation, launches and autograd in C++ (module
-``_T``); here are the calls into it and the device tables of the Muon step.  Arguments are checked in ``functional``."""
+``_T``); here are the calls into it and the device tables of the Muon step.  ``_T`` checks arguments and returns None for
+what it does not take; ``functional`` then raises the error that names it."""
 from __future__ import annotations
 
 import struct
@@ -22,27 +23,35 @@ def T():
 
 
 def residual_norm(x, y, post, gate, scale, pre):
-    pw, pb, pe, pk = (None, None, 0.0, 0) if post is None else (post.weight, post.bias, post.eps, _KINDS[post.kind])
-    qw, qb, qe, qk = (None, None, 0.0, 0) if pre is None else (pre.weight, pre.bias, pre.eps, _KINDS[pre.kind])
-    if grad_sink.any_sinks:
+    pw, pb, pe, pk = (None, None, 0.0, 0) if post is None else (post[0], post[1], post[2], _KINDS.get(post[3], -1))
+    qw, qb, qe, qk = (None, None, 0.0, 0) if pre is None else (pre[0], pre[1], pre[2], _KINDS.get(pre[3], -1))
+    if y is None:
+        return None
+    sinks = grad_sink.any_sinks
+    out = (_T or T()).residual_norm(x, y, pw, pb, pk, pe, qw, qb, qk, qe, gate, scale, sinks)
+    if out is None:
+        return None
+    if sinks:
         grad_sink.note_use(pw, pb, qw, qb, gate)
-    s, h = T().residual_norm(x, y, pw, pb, pk, pe, qw, qb, qk, qe, gate, scale, grad_sink.any_sinks)
-    return s if h is None else (s, h)
+    return out[0] if qk == 0 else out
 
 
 def rms_norm(x, weight, eps):
-    if grad_sink.any_sinks:
+    sinks = grad_sink.any_sinks
+    out = (_T or T()).residual_norm(x, None, None, None, 0, 0.0, weight, None, _KINDS["rms"], eps, None, None, sinks)
+    if out is None:
+        return None
+    if sinks:
         grad_sink.note_use(weight)
-    return T().residual_norm(x, None, None, None, 0, 0.0, weight, None, _KINDS["rms"], eps, None, None,
-                             grad_sink.any_sinks)[1]
+    return out[1]
 
 
 def rotary(qkv, positions, freqs, axis, num_heads, interleaved, inplace):
-    return T().rotary(qkv, positions, freqs, axis, num_heads, interleaved, inplace)
+    return (_T or T()).rotary(qkv, positions, freqs, axis, num_heads, interleaved, inplace)
 
 
 def token_logprobs(logits, target, k):
-    return T().token_logprobs(logits, target, k)
+    return (_T or T()).token_logprobs(logits, target, k)
 
 
 def newton_schulz(g, steps, coefficients, eps):

@@ -673,3 +673,25 @@ def test_results_repeat():
     for _ in range(3):
         for a, b in zip(_everything(*ins), first):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", ["residual_norm", "rotary", "token_logprobs", "newton_schulz"])
+def test_refusals_on_the_device(name):
+    """What the CPU backend refuses is refused here, with the same error, before anything is launched."""
+    import test_transformer_ops_cpu as cpu
+
+    with torch.device("cuda"):
+        getattr(cpu, "test_%s_refusals" % name)()
+
+
+def test_refuses_mixed_devices():
+    x, w = torch.randn(2, 3, 8, device="cuda"), torch.ones(8)
+    for call in (lambda: F().residual_norm(x, x.cpu()), lambda: F().residual_norm(x, x, pre=F().Norm(w)),
+                 lambda: F().residual_norm(x, x, post=F().Norm(w.cuda(), w)), lambda: F().residual_norm(x, x, gate=w),
+                 lambda: F().residual_norm(x, x, scale=torch.ones(2)), lambda: F().rms_norm(x, w),
+                 lambda: F().token_logprobs(x, torch.zeros(2, 3, dtype=torch.int64)),
+                 lambda: F().token_logprobs(x[0], torch.zeros(3, dtype=torch.int64)),
+                 lambda: F().rotary(torch.randn(1, 3, 48, device="cuda"), torch.zeros(3, 1), torch.ones(4),
+                                    torch.zeros(4, dtype=torch.int32), 2)):
+        with pytest.raises(ValueError):
+            call()
