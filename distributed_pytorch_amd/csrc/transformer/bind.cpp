@@ -234,18 +234,20 @@ struct ResidualNormFn : Function<ResidualNormFn> {
     const bool gate_sums = gate_kind == kGateSample && need[4];
     if (gate_sums) dgate = floats({ref.size(0), r.C}, ref);
     if (r.rows > 0) {
-      long splits = 1;
-      const long parts = residual_norm_parts(r.rows, r.per_sample, r.C, code(ref), gate_kind, &splits);
-      if (sums) partial = floats({parts, 5, r.C}, ref);
-      if (gate_sums) gate_partial = floats({ref.size(0) * splits, r.C}, ref);
       p.ds = data<void>(ds); p.dh = data<void>(dh); p.x = data<void>(x); p.y = data<void>(y);
       p.dx = same ? nullptr : data<void>(dx); p.dy = data<void>(dy);
       p.post_w = data<float>(v[0]); p.post_b = data<float>(v[1]); p.pre_w = data<float>(v[2]);
       p.gate = data<float>(v[4]); p.scale = data<float>(v[5]);
-      p.post_stat = data<float>(sv[2]); p.pre_stat = data<float>(sv[3]);
-      p.partial = data<float>(partial); p.gate_partial = data<float>(gate_partial); p.dgate_sample = data<float>(dgate);
+      p.post_stat = data<float>(sv[2]); p.pre_stat = data<float>(sv[3]); p.dgate_sample = data<float>(dgate);
       p.rows = r.rows; p.per_sample = r.per_sample; p.C = r.C;
       p.post = (int)cfg[0]; p.pre = (int)cfg[1]; p.gate_kind = gate_kind;
+      if (sums || gate_sums) {
+        long splits = 1;
+        const long parts = residual_norm_parts(p, code(ref), &splits);
+        if (sums) partial = floats({parts, 5, r.C}, ref);
+        if (gate_sums) gate_partial = floats({ref.size(0) * splits, r.C}, ref);
+        p.partial = data<float>(partial); p.gate_partial = data<float>(gate_partial);
+      }
       if (p.dx != nullptr || p.dy != nullptr || sums || gate_sums) residual_norm_bwd_launch(p, code(ref), stream_of(ref));
     } else {                                    // no rows: every sum is zero
       for (int i = 0; i < 5; ++i) {

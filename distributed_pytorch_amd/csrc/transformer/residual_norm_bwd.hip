@@ -13,12 +13,14 @@
 // LDS, and every workgroup writes one partial row; residual_norm_fold_kernel adds those in a fixed order, straight into
 // the gradients' buffers.  A per-sample gate's sums are flushed at the end of every unit, a part of one sample's rows.
 #include "residual_norm_common.h"
+#include <atomic>
 
 namespace dpa {
 namespace {
 using namespace rn;
 
-constexpr int kMaxParts = 768;      // workgroups of the pass = partial rows of the fold
+constexpr int kCompute = 256;       // compute units
+constexpr int kMaxParts = 1024;     // workgroups of the pass = partial rows of the fold, at most
 
 // what a kernel is made for: s = x + y, s = x + scale * post(y) without `pre`, or everything
 enum Mode : int { kPreOnly = 0, kPostOnly = 1, kAll = 2 };
@@ -150,11 +152,13 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void residual_norm_bwd_kernel(con
       lo = u * unit_rows;
       hi = min(lo + unit_rows, p.rows);
     }
-    // the next row is requested before this one is worked on: with one row in flight a workgroup waits for memory and
-    // for its sums in turn (24 x 257 x 1280 fp32: 70 us)
-    constexpr bool AHEAD = MAXCH == 1;
+    // the next row is requested before this one is worked on: a workgroup waits for memory and for its sums in turn otherwise
+    // (24 x 257 x 1280 fp32: 57 us against 44), where registers hold two rows without giving up residency
+    constexpr bool AHEAD = MAXCH == 1 || (MAXCH == 2 && MODE != kAll);
     Row cur;
     if (AHEAD && lo + grp * rpw < hi) request(cur, lo + grp * rpw, hi);
+    // (vmcnt(0): the compiler would otherwise place this wait in the loop, behind the next row's requests)
+    if constexpr (AHEAD) __builtin_amdgcn_s_waitcnt(0x0f70);
     for (long base = lo + grp * rpw; base < hi; base += groups * rpw) {
       const long row = base + (WIDE ? 0 : lane / G);
       const bool live = row < hi;
@@ -219,14 +223,12 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void residual_norm_bwd_kernel(con
           for (int j = 0; j < V; ++j) g[k][j] += rstd * (cur.dh[k].get(j) * w[j] - m0 - sh[k][j] * m1);
         }
       }
-      if (dx != nullptr)
+      // the results are stored at the end of the row's work, behind the wait for the next row (stores count in it)
+      Vec16<T> odx[MAXCH], ody[MAXCH];
 #pragma unroll
-        for (int k = 0; k < MAXCH; ++k) {
-          Vec16<T> o;
+      for (int k = 0; k < MAXCH; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) o.set(j, g[k][j]);
-          if (live) store_chunk<T, VEC>(o, dx + row * C, gl + k * G, C);
-        }
+        for (int j = 0; j < V; ++j) odx[k].set(j, g[k][j]);
       if (dy != nullptr) {
         float m[2] = {0.f, 0.f};
 #pragma unroll
@@ -270,14 +272,22 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void residual_norm_bwd_kernel(con
               g[k][j] = yrstd * (g[k][j] - m0 - (cur.y[k].get(j) - ymean) * yrstd * m1);
         }
 #pragma unroll
-        for (int k = 0; k < MAXCH; ++k) {
-          Vec16<T> o;
+        for (int k = 0; k < MAXCH; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) o.set(j, g[k][j]);
-          if (live) store_chunk<T, VEC>(o, dy + row * C, gl + k * G, C);
-        }
+          for (int j = 0; j < V; ++j) ody[k].set(j, g[k][j]);
       }
-      if constexpr (AHEAD) cur = next;
+      if constexpr (AHEAD) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        cur = next;
+      }
+      if (live) {
+        if (dx != nullptr)
+#pragma unroll
+          for (int k = 0; k < MAXCH; ++k) store_chunk<T, VEC>(odx[k], dx + row * C, gl + k * G, C);
+        if (dy != nullptr)
+#pragma unroll
+          for (int k = 0; k < MAXCH; ++k) store_chunk<T, VEC>(ody[k], dy + row * C, gl + k * G, C);
+      }
     }
     if constexpr (MODE == kAll)
       if (p.gate_kind == kGateSample && p.gate_partial != nullptr) {
@@ -299,54 +309,53 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void residual_norm_bwd_kernel(con
     if (p.out[4] != nullptr) merge_out<T, MAXCH, WIDE, VEC>(a_gate, part + 4 * C, lds, gl, G, C);
 }
 
-// out[v][c] = beta * out + sum over the partial rows, in a fixed order: 16 columns x 16 part lanes a workgroup
-// (behind them, one after the other, the samples' gates: the sum over the splits of a sample)
+// out[v][c] = beta * out + sum over the partial rows, in a fixed order: workgroups of 16 columns x 64 part lanes, all reads of
+// a lane in flight; behind them, for the samples' gates, the sum over the few splits of a sample: 64 columns x 16 lanes
 struct FoldArgs {
   const float* partial; long nparts, part_stride;
   float* out[5]; float beta[5];
   const float* gate_partial; float* dgate; int splits;
-  int C, vectors, which[5];
+  int C, which[5], of_vector, of_sample;      // workgroups of one vector, of one sample's gate
+  long vectors;                               // workgroups of all vectors
 };
-__global__ __launch_bounds__(256) void residual_norm_fold_kernel(const FoldArgs a) {
-  __shared__ float red[16][17];
-  const int cl = threadIdx.x & 15, pl = threadIdx.x >> 4;
-  const int c = blockIdx.x * 16 + cl;
-  if ((int)blockIdx.y >= a.vectors) {
-    const long n = blockIdx.y - a.vectors;
-    float t = 0.f;
-    if (c < a.C)
-      for (int q = pl; q < a.splits; q += 16) t += a.gate_partial[(n * a.splits + q) * a.C + c];
-    red[pl][cl] = t;
-    __syncthreads();
-    if (pl == 0 && c < a.C) {
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += red[i][cl];
-      a.dgate[n * a.C + c] = sum;
-    }
-    return;
-  }
-  const int v = a.which[blockIdx.y];
+template <int COLS> __device__ __forceinline__ void fold(const FoldArgs& a, long part, long tile, bool vector, float* red) {
+  constexpr int LANES = 1024 / COLS, S = COLS + 1;
+  const int cl = threadIdx.x % COLS, pl = threadIdx.x / COLS;
+  const long c = tile * COLS + cl;
+  const int v = vector ? a.which[part] : 0;
+  const float* src = vector ? a.partial + (long)v * a.C + c : a.gate_partial + part * a.splits * a.C + c;
+  const long stride = vector ? a.part_stride : a.C, parts = vector ? a.nparts : a.splits;
   float t = 0.f;
-  if (c < a.C) {
-    const float* src = a.partial + (long)v * a.C + c;
-    long q = pl;
-    for (; q + 7 * 16 < a.nparts; q += 8 * 16) {
+  if (c < a.C)
+    for (long q = pl; q < parts; q += 8 * LANES) {
       float r[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = src[(q + i * 16) * a.part_stride];
+      for (int i = 0; i < 8; ++i) r[i] = q + i * LANES < parts ? src[(q + i * LANES) * stride] : 0.f;
       t += ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
     }
-    for (; q < a.nparts; q += 16) t += src[q * a.part_stride];
+  red[pl * S + cl] = t;
+  __syncthreads();
+  if (pl < 8) {
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < LANES / 8; ++i) t += red[(pl * (LANES / 8) + i) * S + cl];
   }
-  red[pl][cl] = t;
+  __syncthreads();
+  if (pl < 8) red[pl * S + cl] = t;
   __syncthreads();
   if (pl == 0 && c < a.C) {
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += red[i][cl];
-    a.out[v][c] = a.beta[v] == 0.f ? sum : sum + a.beta[v] * a.out[v][c];
+    for (int i = 0; i < 8; ++i) sum += red[i * S + cl];
+    float* out = vector ? a.out[v] + c : a.dgate + part * a.C + c;
+    *out = vector && a.beta[v] != 0.f ? sum + a.beta[v] * *out : sum;
   }
+}
+__global__ __launch_bounds__(1024) void residual_norm_fold_kernel(const FoldArgs a) {
+  __shared__ float red[64 * 17];
+  const long b = blockIdx.x;
+  if (b < a.vectors) fold<16>(a, b / a.of_vector, b % a.of_vector, true, red);
+  else fold<64>(a, (b - a.vectors) / a.of_sample, (b - a.vectors) % a.of_sample, false, red);
 }
 
 struct Units {
@@ -354,23 +363,24 @@ struct Units {
   int splits;
   unsigned blocks;
 };
-Units units_of(long rows, long per_sample, int C, int dtype, int gate_kind) {
-  const Plan pl = plan(C, dtype == kF32 ? 4 : 8);
+// `parts`: how many workgroups the card holds at once.  More wait for a second turn, with a whole row of sums each; fewer leave
+// room (forward sums of 64 x 197 x 1024 bf16: 31 us with the 512 that fit, 37 with 768)
+Units units_of(long rows, long per_sample, const Plan& pl, long parts, int gate_kind) {
   Units u;
   const long trip = pl.rows_per_trip;
   if (gate_kind == kGateSample) {
     const long samples = rows / per_sample;
-    long splits = (kMaxParts + samples - 1) / samples;
+    long splits = (parts + samples - 1) / samples;
     const long most = (per_sample + trip - 1) / trip;
     if (splits > most) splits = most;
     u.unit_rows = (per_sample + splits - 1) / splits;
     u.unit_rows = (u.unit_rows + trip - 1) / trip * trip;
     u.splits = (int)((per_sample + u.unit_rows - 1) / u.unit_rows);
     u.units = samples * u.splits;
-    u.blocks = (unsigned)(u.units < kMaxParts ? u.units : kMaxParts);
+    u.blocks = (unsigned)(u.units < parts ? u.units : parts);
   } else {
     long blocks = (rows + trip - 1) / trip;
-    if (blocks > kMaxParts) blocks = kMaxParts;
+    if (blocks > parts) blocks = parts;
     u.unit_rows = (rows + blocks - 1) / blocks;
     u.unit_rows = (u.unit_rows + trip - 1) / trip * trip;
     u.units = (rows + u.unit_rows - 1) / u.unit_rows;
@@ -380,78 +390,102 @@ Units units_of(long rows, long per_sample, int C, int dtype, int gate_kind) {
   return u;
 }
 
-template <typename T, int MAXCH, bool WIDE>
-void launch(const ResidualNormBwd& p, const Plan& pl, const Units& u, bool vec, int mode, hipStream_t s) {
-  const FastDiv by_sample = make_fastdiv((uint32_t)p.per_sample);
-#define DPA_RN_BWD(VECB, MODEC)                                                                                       \
-  hipLaunchKernelGGL((residual_norm_bwd_kernel<T, MAXCH, WIDE, VECB, MODEC>), dim3(u.blocks), dim3(pl.threads), 0, s, p, pl.G, \
-                     u.units, u.unit_rows, u.splits, by_sample)
-  if (!vec) DPA_RN_BWD(false, kAll);
-  else if (mode == kPreOnly) DPA_RN_BWD(true, kPreOnly);
-  else if (mode == kPostOnly) DPA_RN_BWD(true, kPostOnly);
-  else DPA_RN_BWD(true, kAll);
-#undef DPA_RN_BWD
+template <typename T, int MAXCH, bool WIDE> using Kernel = void (*)(ResidualNormBwd, int, long, long, int, FastDiv);
+template <typename T, int MAXCH, bool WIDE> Kernel<T, MAXCH, WIDE> kernel_of(bool vec, int mode) {
+  if (!vec) return residual_norm_bwd_kernel<T, MAXCH, WIDE, false, kAll>;
+  if (mode == kPreOnly) return residual_norm_bwd_kernel<T, MAXCH, WIDE, true, kPreOnly>;
+  if (mode == kPostOnly) return residual_norm_bwd_kernel<T, MAXCH, WIDE, true, kPostOnly>;
+  return residual_norm_bwd_kernel<T, MAXCH, WIDE, true, kAll>;
+}
+// workgroups that the card holds at once; asked for once for each kernel and size of workgroup
+template <typename T, int MAXCH, bool WIDE> long resident(bool vec, int mode, int threads) {
+  static std::atomic<int> known[4][9];
+  std::atomic<int>& k = known[vec ? mode : 3][threads / 64];
+  int n = k.load(std::memory_order_relaxed);
+  if (n == 0) {
+    DPA_CHECK_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(
+        &n, reinterpret_cast<const void*>(kernel_of<T, MAXCH, WIDE>(vec, mode)), threads, 0));
+    if (n < 1) n = 1;
+    k.store(n, std::memory_order_relaxed);
+  }
+  const long all = (long)n * kCompute;
+  return all < kMaxParts ? all : kMaxParts;
 }
 
-}  // namespace
+// f(type, chunks a lane, wide) for the row's layout
+#define DPA_RN_LAYOUT(pl, dtype, ...)                                                                              \
+  DPA_DISPATCH_DTYPE(dtype, {                                                                                      \
+    if (!(pl).wide && (pl).maxch == 1) { constexpr int MAXCH = 1; constexpr bool WIDE = false; __VA_ARGS__; }      \
+    else if (!(pl).wide) { constexpr int MAXCH = 2; constexpr bool WIDE = false; __VA_ARGS__; }                    \
+    else if ((pl).maxch == 1) { constexpr int MAXCH = 1; constexpr bool WIDE = true; __VA_ARGS__; }                \
+    else if ((pl).maxch == 2) { constexpr int MAXCH = 2; constexpr bool WIDE = true; __VA_ARGS__; }                \
+    else { constexpr int MAXCH = 4; constexpr bool WIDE = true; __VA_ARGS__; }                                     \
+  })
 
-long residual_norm_parts(long rows, long per_sample, int C, int dtype, int gate_kind, long* splits) {
-  if (rows <= 0 || per_sample <= 0 || C <= 0) throw std::invalid_argument("residual_norm: empty shape");
-  const Units u = units_of(rows, per_sample, C, dtype, gate_kind);
-  *splits = u.splits;
-  return u.blocks;
-}
-
-void residual_norm_bwd_launch(const ResidualNormBwd& p, int dtype, hipStream_t s) {
-  if (p.rows <= 0) return;
+struct Pick {
+  Plan pl;
+  bool vec;
+  int mode;
+  Units u;
+};
+Pick pick(const ResidualNormBwd& p, int dtype) {
+  if (p.rows <= 0 || p.per_sample <= 0) throw std::invalid_argument("residual_norm: empty shape");
   if (p.rows >= (1l << 31)) throw std::invalid_argument("residual_norm: at most 2^31 - 1 rows");
   const int vecn = dtype == kF32 ? 4 : 8;
   if (p.C <= 0 || (p.C + vecn - 1) / vecn > kResidualNormMaxChunks)
     throw std::invalid_argument("residual_norm: C must be 1 .. 2048 16-byte chunks");
-  const Plan pl = plan(p.C, vecn);
-  const Units u = units_of(p.rows, p.per_sample, p.C, dtype, p.gate_kind);
+  Pick k;
+  k.pl = plan(p.C, vecn);
   auto off16 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0; };
-  const bool vec = p.C % vecn == 0 && !(off16(p.ds) || off16(p.dh) || off16(p.x) || off16(p.y) || off16(p.dx) || off16(p.dy) ||
-                                        off16(p.post_w) || off16(p.post_b) || off16(p.pre_w) || off16(p.gate));
+  k.vec = p.C % vecn == 0 && !(off16(p.ds) || off16(p.dh) || off16(p.x) || off16(p.y) || off16(p.dx) || off16(p.dy) ||
+                               off16(p.post_w) || off16(p.post_b) || off16(p.pre_w) || off16(p.gate));
   const bool plain = p.post == kNormNone && p.gate_kind == kGateNone && p.scale == nullptr;
-  const int mode = plain ? kPreOnly : (p.pre == kNormNone && p.gate_kind == kGateNone && p.post != kNormNone ? kPostOnly : kAll);
+  k.mode = plain ? kPreOnly : (p.pre == kNormNone && p.gate_kind == kGateNone && p.post != kNormNone ? kPostOnly : kAll);
   if (plain && p.dy != nullptr) throw std::invalid_argument("residual_norm: without a branch of its own dy is dx");
-  DPA_DISPATCH_DTYPE(dtype, {
-    if (!pl.wide && pl.maxch == 1) launch<T, 1, false>(p, pl, u, vec, mode, s);
-    else if (!pl.wide) launch<T, 2, false>(p, pl, u, vec, mode, s);
-    else if (pl.maxch == 1) launch<T, 1, true>(p, pl, u, vec, mode, s);
-    else if (pl.maxch == 2) launch<T, 2, true>(p, pl, u, vec, mode, s);
-    else launch<T, 4, true>(p, pl, u, vec, mode, s);
-  });
+  long parts = 0;
+  DPA_RN_LAYOUT(k.pl, dtype, (parts = resident<T, MAXCH, WIDE>(k.vec, k.mode, k.pl.threads)));
+  k.u = units_of(p.rows, p.per_sample, k.pl, parts, p.gate_kind);
+  return k;
+}
+
+}  // namespace
+
+long residual_norm_parts(const ResidualNormBwd& p, int dtype, long* splits) {
+  const Pick k = pick(p, dtype);
+  *splits = k.u.splits;
+  return k.u.blocks;
+}
+
+void residual_norm_bwd_launch(const ResidualNormBwd& p, int dtype, hipStream_t s) {
+  if (p.rows <= 0) return;
+  const Pick k = pick(p, dtype);
+  const Units& u = k.u;
+  const FastDiv by_sample = make_fastdiv((uint32_t)p.per_sample);
+  DPA_RN_LAYOUT(k.pl, dtype, hipLaunchKernelGGL((kernel_of<T, MAXCH, WIDE>(k.vec, k.mode)), dim3(u.blocks), dim3(k.pl.threads), 0, s, p,
+                                                k.pl.G, u.units, u.unit_rows, u.splits, by_sample));
   DPA_CHECK_HIP(hipGetLastError());
   FoldArgs f{};
   f.partial = p.partial;
   f.nparts = u.blocks;
   f.part_stride = 5l * p.C;
   f.C = p.C;
+  f.of_vector = (p.C + 15) / 16;
+  f.of_sample = (p.C + 63) / 64;
   for (int v = 0; v < 5; ++v) {
     f.out[v] = p.out[v];
     f.beta[v] = p.beta[v];
     if (p.out[v] != nullptr) f.which[f.vectors++] = v;
   }
-  const bool gates = p.gate_kind == kGateSample && p.dgate_sample != nullptr;
+  f.vectors *= f.of_vector;
   f.gate_partial = p.gate_partial;
   f.dgate = p.dgate_sample;
   f.splits = u.splits;
-  // (grid.y holds 65535: samples beyond that many take further launches)
-  long left = gates ? p.rows / p.per_sample : 0;
-  while (f.vectors > 0 || left > 0) {
-    const long now = left < 65535 - f.vectors ? left : 65535 - f.vectors;
-    hipLaunchKernelGGL(residual_norm_fold_kernel, dim3((unsigned)((p.C + 15) / 16), (unsigned)(f.vectors + now)), dim3(256), 0, s,
-                       f);
-    DPA_CHECK_HIP(hipGetLastError());
-    if (gates) {
-      f.gate_partial += now * u.splits * p.C;
-      f.dgate += now * p.C;
-    }
-    left -= now;
-    f.vectors = 0;
-  }
+  const bool gates = p.gate_kind == kGateSample && p.dgate_sample != nullptr;
+  const long all = f.vectors + (gates ? p.rows / p.per_sample * f.of_sample : 0);
+  if (all >= (1l << 31)) throw std::invalid_argument("residual_norm: too many gates");
+  if (all == 0) return;
+  hipLaunchKernelGGL(residual_norm_fold_kernel, dim3((unsigned)all), dim3(1024), 0, s, f);
+  DPA_CHECK_HIP(hipGetLastError());
 }
 
 }  // namespace dpa

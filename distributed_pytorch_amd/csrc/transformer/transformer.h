@@ -41,7 +41,7 @@ struct ResidualNormBwd {
   int C = 0, post = 0, pre = 0, gate_kind = 0;
 };
 constexpr int kResidualNormMaxChunks = 2048;                       // 16-byte chunks of one row
-long residual_norm_parts(long rows, long per_sample, int C, int dtype, int gate_kind, long* splits);
+long residual_norm_parts(const ResidualNormBwd& p, int dtype, long* splits);
 void residual_norm_fwd_launch(const ResidualNormFwd& p, int dtype, hipStream_t s);
 void residual_norm_bwd_launch(const ResidualNormBwd& p, int dtype, hipStream_t s);
 
