@@ -12,16 +12,19 @@
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/DeviceGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "transformer.h"
 
 namespace py = pybind11;
 using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::Function;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
@@ -75,6 +78,18 @@ bool norm_taken(const OptTensor& w, const OptTensor& b, int64_t kind, double eps
 // a gradient of a gradient would silently be missing
 void once(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass is not differentiable (create_graph)");
+}
+
+// Nodes of the graph are written out like torch's own, not as torch::autograd::Function: that class looks its inputs, outputs
+// and saved values up in maps, 4 us a call.  `inputs`: one edge for each argument of the gradient, undefined ones too.
+template <typename N, typename... Inputs> std::shared_ptr<N> make_node(const Inputs&... inputs) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return node;
+}
+SavedVariable saved(const Tensor& t, bool is_output = false) { return t.defined() ? SavedVariable(t, is_output) : SavedVariable(); }
+void has_history(const Tensor& t, const std::shared_ptr<Node>& node) {
+  if (t.defined()) torch::autograd::set_history(t, node);
 }
 
 // ------------------------------------------------------------------------------------------ residual norm
@@ -147,33 +162,25 @@ Tensor deliver(const Tensor& param, const Tensor& grad) {
   return g.is_none() ? Tensor() : g.cast<Tensor>();
 }
 
-struct ResidualNormFn : Function<ResidualNormFn> {
+struct ResidualNormBackward : Node {
   // y undefined: h = pre(x) alone
-  static variable_list forward(AutogradContext* ctx, const Tensor& x0, const OptTensor& y0, const OptTensor& post_w0,
-                               const OptTensor& post_b0, const OptTensor& pre_w0, const OptTensor& pre_b0,
-                               const OptTensor& gate0, const OptTensor& scale, const NormCfg& c) {
-    const Tensor x = x0.contiguous(), y = dense(given(y0)), post_w = given(post_w0), post_b = given(post_b0),
-                 pre_w = given(pre_w0), pre_b = given(pre_b0), gate = given(gate0);
-    const Vecs v{vec32(post_w), vec32(post_b), vec32(pre_w), vec32(pre_b), vec32(gate), vec32(given(scale))};
-    RnOut o = rn_forward(x, y, v, c, true);
-    const bool pre = c.pre != kNormNone, keep_y = pre || c.post != kNormNone || gate.defined();
-    ctx->save_for_backward({pre ? x : Tensor(), keep_y ? y : Tensor(), o.post_stat, o.pre_stat, post_w, post_b, pre_w, pre_b,
-                            gate, v[5]});
-    ctx->saved_data["cfg"] = c.post | c.pre << 4 | (int64_t)y.defined() << 8 | (int64_t)c.sinks << 9;
-    ctx->set_materialize_grads(false);
-    variable_list out;
-    if (o.s.defined()) out.push_back(o.s);
-    if (o.h.defined()) out.push_back(o.h);
-    return out;
+  SavedVariable x_, y_, post_stat_, pre_stat_, post_w_, post_b_, pre_w_, pre_b_, gate_, scale_;
+  int64_t post = 0, pre = 0;
+  bool has_y = false, may_sink = false;
+
+  std::string name() const override { return "ResidualNormBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&x_, &y_, &post_stat_, &pre_stat_, &post_w_, &post_b_, &pre_w_, &pre_b_, &gate_, &scale_}) v->reset_data();
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  variable_list apply(variable_list&& grads) override {
     once("residual_norm");
-    const variable_list sv = ctx->get_saved_variables();
-    const int64_t packed = ctx->saved_data["cfg"].toInt();
-    const int64_t cfg[4] = {packed & 15, packed >> 4 & 15, packed >> 8 & 1, packed >> 9 & 1};
-    const bool has_y = cfg[2] != 0;
-    variable_list got(9);
+    const std::lock_guard<std::mutex> lock(mutex_);
+    const std::array<Tensor, 10> sv{x_.unpack(), y_.unpack(), post_stat_.unpack(), pre_stat_.unpack(), post_w_.unpack(),
+                                    post_b_.unpack(), pre_w_.unpack(), pre_b_.unpack(), gate_.unpack(), scale_.unpack()};
+    const int64_t cfg[4] = {post, pre, has_y, may_sink};
+    variable_list got(7);
     Tensor ds = has_y ? grads[0] : Tensor(), dh = has_y ? (grads.size() > 1 ? grads[1] : Tensor()) : grads[0];
     if (!ds.defined() && !dh.defined()) return got;
     ds = dense(ds);
@@ -187,10 +194,8 @@ struct ResidualNormFn : Function<ResidualNormFn> {
     const Vecs v{vec32(sv[4]), vec32(sv[5]), vec32(sv[6]), vec32(sv[7]), vec32(sv[8]), sv[9]};
     const RowShape r = row_shape(ref);
     const int gate_kind = v[4].defined() ? (int)v[4].dim() : kGateNone;
-    // autograd counts the arguments that were given
-    const bool here[7] = {true, has_y, sv[4].defined(), sv[5].defined(), sv[6].defined(), sv[7].defined(), sv[8].defined()};
     bool needs[7];
-    for (int i = 0, edge = 0; i < 7; ++i) needs[i] = here[i] && ctx->needs_input_grad(edge++);
+    for (int i = 0; i < 7; ++i) needs[i] = task_should_compute_output(i);
     const bool need_x = needs[0], need_y = needs[1];
     bool need[5], any_leaf = false;
     for (int i = 0; i < 5; ++i) {
@@ -302,9 +307,33 @@ std::optional<std::pair<OptTensor, OptTensor>> residual_norm(const Tensor& x, co
                                false);
     return std::make_pair(opt(o.s), opt(o.h));
   }
-  variable_list out = ResidualNormFn::apply(x, y, post_w, post_b, pre_w, pre_b, gate, scale, c);
-  if (!Y.defined()) return std::make_pair(OptTensor(), OptTensor(out[0]));
-  return std::make_pair(OptTensor(out[0]), out.size() > 1 ? OptTensor(out[1]) : OptTensor());
+  const auto node = make_node<ResidualNormBackward>(x, Y, pw, pb, qw, qb, g);
+  RnOut o;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor X = x.contiguous();
+    const Tensor y0 = dense(Y);
+    const Vecs v{vec32(pw), vec32(pb), vec32(qw), vec32(qb), vec32(g), vec32(sc)};
+    o = rn_forward(X, y0, v, c, true);
+    const bool has_pre = pre != kNormNone;
+    if (has_pre) node->x_ = saved(X);
+    if (has_pre || post != kNormNone || g.defined()) node->y_ = saved(y0);
+    node->post_stat_ = saved(o.post_stat);
+    node->pre_stat_ = saved(o.pre_stat);
+    node->post_w_ = saved(pw);
+    node->post_b_ = saved(pb);
+    node->pre_w_ = saved(qw);
+    node->pre_b_ = saved(qb);
+    node->gate_ = saved(g);
+    node->scale_ = saved(v[5]);
+    node->post = post;
+    node->pre = pre;
+    node->has_y = Y.defined();
+    node->may_sink = sinks;
+  }
+  has_history(o.s, node);
+  has_history(o.h, node);
+  return std::make_pair(opt(o.s), opt(o.h));
 }
 
 // ------------------------------------------------------------------------------------------ rotary
@@ -333,20 +362,22 @@ Tensor rotary_new(const Tensor& t, const Tensor& pos, const Tensor& freqs, const
   return out;
 }
 
-struct RotaryFn : Function<RotaryFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& pos, const Tensor& freqs, const Tensor& axis,
-                        int64_t heads, bool interleaved) {
-    ctx->save_for_backward({pos, freqs, axis});
-    ctx->saved_data["heads"] = heads;
-    ctx->saved_data["interleaved"] = interleaved;
-    return rotary_new(qkv, pos, freqs, axis, heads, interleaved, false);
+struct RotaryBackward : Node {
+  SavedVariable pos_, freqs_, axis_;
+  int64_t heads = 0;
+  bool interleaved = false;
+
+  std::string name() const override { return "RotaryBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&pos_, &freqs_, &axis_}) v->reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  variable_list apply(variable_list&& grads) override {
     once("rotary");
-    const variable_list sv = ctx->get_saved_variables();
-    variable_list got(6);
-    got[0] = rotary_new(grads[0], sv[0], sv[1], sv[2], ctx->saved_data["heads"].toInt(), ctx->saved_data["interleaved"].toBool(),
-                        true);
+    const std::lock_guard<std::mutex> lock(mutex_);
+    variable_list got(1);
+    const Tensor pos = pos_.unpack(), freqs = freqs_.unpack(), axis = axis_.unpack();
+    if (grads[0].defined()) got[0] = rotary_new(grads[0], pos, freqs, axis, heads, interleaved, true);
     return got;
   }
 };
@@ -376,7 +407,19 @@ OptTensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs
     return qkv;
   }
   if (!tracked({qkv})) return rotary_new(qkv, pos, f, a, heads, interleaved, false);
-  return OptTensor(RotaryFn::apply(qkv, pos, f, a, heads, interleaved));
+  const auto node = make_node<RotaryBackward>(qkv);
+  Tensor out;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    out = rotary_new(qkv, pos, f, a, heads, interleaved, false);
+    node->pos_ = saved(pos);
+    node->freqs_ = saved(f);
+    node->axis_ = saved(a);
+    node->heads = heads;
+    node->interleaved = interleaved;
+  }
+  has_history(out, node);
+  return out;
 }
 
 // ------------------------------------------------------------------------------------------ log probabilities
@@ -403,19 +446,21 @@ LpOut lp_forward(const Tensor& z, const Tensor& t, int64_t k) {
   return o;
 }
 
-struct TokenLogprobsFn : Function<TokenLogprobsFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& target, int64_t k) {
-    const Tensor z = logits.stride(1) == 1 ? logits : logits.contiguous();
-    LpOut o = lp_forward(z, target, k);
-    ctx->save_for_backward({z, target, o.norm, o.ent, o.idx});
-    ctx->saved_data["k"] = k;
-    ctx->mark_non_differentiable({o.idx});
-    ctx->set_materialize_grads(false);
-    return {o.lp, o.ent, o.top, o.idx};
+struct TokenLogprobsBackward : Node {
+  SavedVariable logits_, target_, norm_, entropy_, index_;
+  int64_t k = 0;
+
+  std::string name() const override { return "TokenLogprobsBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&logits_, &target_, &norm_, &entropy_, &index_}) v->reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  variable_list apply(variable_list&& grads) override {
     once("token_logprobs");
-    variable_list got(3);
+    const std::lock_guard<std::mutex> lock(mutex_);
+    variable_list got(1);
+    const std::array<Tensor, 5> sv{logits_.unpack(), target_.unpack(), norm_.unpack(), entropy_.unpack(shared_from_this()),
+                                   index_.unpack()};
     Tensor g[3];
     bool any = false;
     for (int i = 0; i < 3; ++i) {
@@ -423,7 +468,6 @@ struct TokenLogprobsFn : Function<TokenLogprobsFn> {
       any = any || g[i].defined();
     }
     if (!any) return got;
-    const variable_list sv = ctx->get_saved_variables();
     const Tensor& z = sv[0];
     const c10::DeviceGuard guard(z.device());
     const Tensor dz = at::empty(z.sizes(), z.options());
@@ -432,7 +476,7 @@ struct TokenLogprobsFn : Function<TokenLogprobsFn> {
     p.entropy = sv[3].data_ptr<float>(); p.index = sv[4].data_ptr<int64_t>();
     p.d_logprob = data<float>(g[0]); p.d_entropy = data<float>(g[1]); p.d_top = data<float>(g[2]);
     p.dlogits = dz.data_ptr();
-    p.N = z.size(0); p.C = z.size(1); p.ld = z.stride(0); p.k = (int)ctx->saved_data["k"].toInt();
+    p.N = z.size(0); p.C = z.size(1); p.ld = z.stride(0); p.k = (int)k;
     token_logprobs_bwd_launch(p, code(z), stream_of(z));
     got[0] = dz;
     return got;
@@ -451,8 +495,21 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const T
     const LpOut o = lp_forward(logits.stride(1) == 1 ? logits : logits.contiguous(), t, k);
     return std::make_tuple(o.lp, o.ent, o.top, o.idx);
   }
-  variable_list o = TokenLogprobsFn::apply(logits, t, k);
-  return std::make_tuple(o[0], o[1], o[2], o[3]);
+  const auto node = make_node<TokenLogprobsBackward>(logits);
+  LpOut o;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor z = logits.stride(1) == 1 ? logits : logits.contiguous();
+    o = lp_forward(z, t, k);
+    node->logits_ = saved(z);
+    node->target_ = saved(t);
+    node->norm_ = saved(o.norm);
+    node->index_ = saved(o.idx);
+    node->k = k;
+  }
+  for (const Tensor& out : {o.lp, o.ent, o.top}) has_history(out, node);
+  node->entropy_ = saved(o.ent, true);
+  return std::make_tuple(o.lp, o.ent, o.top, o.idx);
 }
 
 // ------------------------------------------------------------------------------------------ Newton-Schulz and Muon
