@@ -23,7 +23,7 @@ __device__ __forceinline__ double position(const void* p, long i, int kind) {
   }
 }
 
-// VEC: P (interleaved: 2 P), D and every row are whole 16-byte chunks; else element by element
+// VEC: D, P (not INTER) and every row are whole 16-byte chunks; else element by element
 template <typename T, bool VEC, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const int tt, const FastDiv by_items,
                                                      const FastDiv by_chunks, const FastDiv by_rest) {
@@ -54,8 +54,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
   T* out = reinterpret_cast<T*>(p.out);
   const bool copy = p.in != p.out;
   // items of one token: the chunks (pairs of chunks) that turn, then the ones that are copied
-  const int chunks = (INTER ? 2 * P : P) / V;      // per head; not INTER: with a partner P further on
-  const int rest = (D - 2 * P) / V;
+  // per head; INTER: the last one may hold pairs that stay; not INTER: with a partner P further on
+  const int chunks = ((INTER ? 2 * P : P) + V - 1) / V;
+  const int rest = INTER ? D / V - chunks : (D - 2 * P) / V;
   const int n_turn = 2 * H * chunks;
   const int n_rest = copy ? 2 * H * rest : 0;
   const int items = n_turn + n_rest + (copy ? H * D / V : 0);
@@ -77,6 +78,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
           v.load(src + o);
 #pragma unroll
           for (int j = 0; j < V; j += 2) {
+            if (j0 + j >= 2 * P) break;
             const float2 c = cs[(j0 + j) / 2];
             const float a = v.get(j), b2 = v.get(j + 1);
             v.set(j, a * c.x - b2 * c.y);
@@ -115,7 +117,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
       long o;
       if (it < n_rest) {
         const int head = (int)fdiv((uint32_t)it, by_rest);
-        o = (long)head * D + 2 * P + (it - head * rest) * V;
+        o = (long)head * D + (INTER ? chunks * V : 2 * P) + (it - head * rest) * V;
       } else {
         o = 2l * H * D + (long)(it - n_rest) * V;
       }
@@ -134,12 +136,13 @@ template <typename T>
 void launch(const RotaryParams& p, hipStream_t s) {
   const int V = 16 / (int)sizeof(T);
   auto off16 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0; };
-  const bool vec = p.D % V == 0 && (p.interleaved ? 2 * p.pairs : p.pairs) % V == 0 && (2 * p.pairs) % V == 0 &&
+  const bool vec = p.D % V == 0 && (p.interleaved || p.pairs % V == 0) &&
                    !off16(p.in) && !off16(p.out) && p.in_batch % V == 0 && p.in_token % V == 0 && p.out_batch % V == 0 &&
                    p.out_token % V == 0;
   const int v = vec ? V : 1;
   const bool copy = p.in != p.out;
-  const int chunks = (p.interleaved ? 2 * p.pairs : p.pairs) / v, rest = (p.D - 2 * p.pairs) / v;
+  const int chunks = ((p.interleaved ? 2 * p.pairs : p.pairs) + v - 1) / v;
+  const int rest = p.interleaved ? p.D / v - chunks : (p.D - 2 * p.pairs) / v;
   const int items = 2 * p.H * chunks + (copy ? 2 * p.H * rest + p.H * p.D / v : 0);
   if (items <= 0) return;
   // many short workgroups, whose angles and copies overlap, one token each for short calls (4 x 3137 tokens of 3 x 16 x 64

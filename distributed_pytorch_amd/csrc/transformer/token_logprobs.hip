@@ -127,12 +127,6 @@ __device__ __forceinline__ void walk(const T* z, int lo, int hi, F f) {
   for (; c < hi; c += kStep) f(load_chunk(z, c, hi), c);
 }
 
-// Makes a chunk a new value to the compiler: it would otherwise keep the floats of one pass over the registers for the next
-// one, and spill hundreds of them.
-template <typename T> __device__ __forceinline__ void forget(Vec16<T>& v) {
-  asm volatile("" : "+v"(v.raw.x), "+v"(v.raw.y), "+v"(v.raw.z), "+v"(v.raw.w));
-}
-
 template <int TH> struct TopShared {
   uint64_t best[TH];
   uint64_t cand[kCap];
@@ -287,9 +281,9 @@ __device__ __forceinline__ void write_row(const TokenLogprobs& p, long row, bool
   }
 }
 
-// One workgroup of TH lanes per row, or per part of a row.  Q > 0: the part is at most Q chunks a lane and stays in registers
-// (one read; the exact maximum comes first).  Q = 0: any length, a second look comes from cache.
-template <typename T, int TH, int Q>
+// One workgroup of TH lanes per row, or per part of a row; a second look comes from cache.  (Keeping a row's chunks in registers
+// from the first look cost more residency than it saved: 4457 x 15054 bf16 with k = 5 233 us against 67.)
+template <typename T, int TH>
 __global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs p) {
   constexpr int V = Vec16<T>::N;
   __shared__ float wm[TH / 64], ws[TH / 64], wu[TH / 64];
@@ -304,63 +298,37 @@ __global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs 
   const long t = p.target[row];                    // (early: two loads that follow each other)
   const bool valid = t >= 0 && t < p.C;
   const float zt = valid ? to_float(z[t]) : 0.f;
-  Vec16<T> v[Q > 0 ? Q : 1];
   RunSums a;
   a.clear();
   int where = c0;                                 // chunk with this lane's largest element
-  // Q = 0: the lane's two largest chunk maxima, where they are, and the largest of its other chunks: the second look needs
+  // the lane's two largest chunk maxima, where they are, and the largest of its other chunks: the second look needs
   // two chunks of a lane at most, unless a third one reaches the bound as well
   float first = -INFINITY, second = -INFINITY, third = -INFINITY;
   int where2 = c0;
-  if constexpr (Q > 0) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int c = c0 + q * TH * V;
-      if (c < hi) v[q] = load_chunk(z, c, hi);
+  walk<T, TH>(z, (int)lo, (int)hi, [&](const Vec16<T>& x, int c) {
+    const float mx = chunk_max(x);
+    if (mx > first) {
+      third = second;
+      second = first;
+      where2 = where;
+      first = mx;
+      where = c;
+    } else if (mx > second) {
+      third = second;
+      second = mx;
+      where2 = c;
+    } else {
+      third = fmaxf(third, mx);
     }
-    float largest = -INFINITY;
+    a.raise(mx);
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int c = c0 + q * TH * V;
-      if (c < hi) {
-        const float mx = chunk_max(v[q]);
-        if (mx > largest) { largest = mx; where = c; }
-      }
-    }
-    a.m = fmaxf(largest, kLowest);
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-      if (c0 + q * TH * V < hi) {
-        forget(v[q]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) a.add(v[q].get(j));
-      }
-  } else {
-    walk<T, TH>(z, (int)lo, (int)hi, [&](const Vec16<T>& x, int c) {
-      const float mx = chunk_max(x);
-      if (mx > first) {
-        third = second;
-        second = first;
-        where2 = where;
-        first = mx;
-        where = c;
-      } else if (mx > second) {
-        third = second;
-        second = mx;
-        where2 = c;
-      } else {
-        third = fmaxf(third, mx);
-      }
-      a.raise(mx);
-#pragma unroll
-      for (int j = 0; j < V; ++j) a.add(x.get(j));
-    });
-  }
+    for (int j = 0; j < V; ++j) a.add(x.get(j));
+  });
   // the lane's largest chunks again, on their way while the sums meet
   Vec16<T> b1, b2;
   if (p.k > 0 && c0 < hi) {
     b1 = load_chunk(z, where, hi);
-    if constexpr (Q == 0) b2 = load_chunk(z, where2, hi);
+    b2 = load_chunk(z, where2, hi);
   }
   // lanes, then waves, in a fixed order
   a.join_wave();
@@ -382,42 +350,30 @@ __global__ __launch_bounds__(TH) void token_logprobs_kernel(const TokenLogprobs 
     }
     const bool plain = a.s == a.s;
     uint64_t* out = p.splits == 1 ? top : p.keys + (long)blockIdx.x * p.k;
-    if constexpr (Q > 0)
-      top_of<T, TH>(p.k, hi, best, plain, sh, out, [&](float, auto f) {
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          const int c = c0 + q * TH * V;
-          if (c < hi) {
-            forget(v[q]);
-            f(v[q], c);
-          }
-        }
-      });
-    else
-      top_of<T, TH>(p.k, hi, best, plain, sh, out, [&](float least, auto f) {
-        if (least == -INFINITY) {
-          walk<T, TH>(z, (int)lo, (int)hi, f);
-          return;
-        }
-        // a lane that walks its chunks alone keeps the workgroup waiting for all of their latencies: a few such lanes are
-        // shared out, a chunk a lane
-        const bool all = third >= least;
-        if (all) {
-          const int at = atomicAdd(&sh.lanes, 1);
-          if (at < 8) sh.lane[at] = threadIdx.x;
-        } else {
-          if (first >= least) f(b1, where);
-          if (second >= least) f(b2, where2);
-        }
-        __syncthreads();
-        const int lanes = sh.lanes;
-        if (lanes <= 8) {
-          for (int i = 0; i < lanes; ++i)
-            for (int c = lo + (sh.lane[i] + (int)threadIdx.x * TH) * V; c < hi; c += TH * TH * V) f(load_chunk(z, c, hi), c);
-        } else if (all) {
-          walk<T, TH>(z, (int)lo, (int)hi, f);
-        }
-      });
+    top_of<T, TH>(p.k, hi, best, plain, sh, out, [&](float least, auto f) {
+      if (least == -INFINITY) {
+        walk<T, TH>(z, (int)lo, (int)hi, f);
+        return;
+      }
+      // a lane that walks its chunks alone keeps the workgroup waiting for all of their latencies: a few such lanes are
+      // shared out, a chunk a lane
+      const bool all = third >= least;
+      if (all) {
+        const int at = atomicAdd(&sh.lanes, 1);
+        if (at < 8) sh.lane[at] = threadIdx.x;
+      } else {
+        if (first >= least) f(b1, where);
+        if (second >= least) f(b2, where2);
+      }
+      __syncthreads();
+      const int lanes = sh.lanes;
+      if (lanes <= 8) {
+        for (int i = 0; i < lanes; ++i)
+          for (int c = lo + (sh.lane[i] + (int)threadIdx.x * TH) * V; c < hi; c += TH * TH * V) f(load_chunk(z, c, hi), c);
+      } else if (all) {
+        walk<T, TH>(z, (int)lo, (int)hi, f);
+      }
+    });
   }
   if (p.splits > 1) {
     if (threadIdx.x == 0) {
@@ -581,13 +537,14 @@ void token_logprobs_launch(const TokenLogprobs& p, int dtype, hipStream_t s) {
     throw std::invalid_argument("token_logprobs: splits");
   const long part = part_of(p.C, p.splits) < p.C ? part_of(p.C, p.splits) : p.C;
   const dim3 grid((unsigned)(p.N * p.splits));
-  // one wave per row up to 256 chunks (1024 classes in fp32), a workgroup up to 2048 chunks in registers, else two looks
-  // (16 chunks a lane spill)
   DPA_DISPATCH_DTYPE(dtype, {
-    const long chunks = (part + Vec16<T>::N - 1) / Vec16<T>::N;
-    if (chunks <= 64 * 4) hipLaunchKernelGGL((token_logprobs_kernel<T, 64, 4>), grid, dim3(64), 0, s, p);
-    else if (chunks <= 256 * 8) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 8>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 0>), grid, dim3(256), 0, s, p);
+    // as few waves a row as fill the card (4096 are resident), since a row's waves wait for each other at the end of each pass;
+    // with 1, 2 or 4 waves, k = 5, us: 8192 x 4000 bf16 32 : 47 : 72, 2048 x 50257 bf16 50 : 47 : 53, 1024 x 16000 fp32
+    // 22 : 19 : 19, 300 x 16000 fp32 19 : 16 : 13; 64 x 1000 bf16 7.1 : 7.5 : 7.9
+    const long rows = p.N * p.splits, chunks = (part + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (rows >= 4096 || chunks <= 256) hipLaunchKernelGGL((token_logprobs_kernel<T, 64>), grid, dim3(64), 0, s, p);
+    else if (rows >= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 128>), grid, dim3(128), 0, s, p);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, 256>), grid, dim3(256), 0, s, p);
     if (p.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((unsigned)p.N), dim3(kJoin), 0, s, p);
   });
   DPA_CHECK_HIP(hipGetLastError());

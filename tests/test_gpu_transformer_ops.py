@@ -247,6 +247,24 @@ def test_rotary(B, S, H, D, P, A, batched, dtype, interleaved):
         assert back is same and torch.equal(same, out)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,P", [(48, 15), (48, 9), (24, 1), (16, 7), (40, 20), (32, 13)])
+def test_rotary_pairs_end_inside_a_chunk(D, P, interleaved, dtype):
+    """What lies behind the pairs is copied as it is, infinities and NaN too, out of place and in place."""
+    qkv, pos, freqs, axis = _rotary_case(2, 9, 3, D, P, 2, dtype)
+    value, bound = ref.rotary(qkv, pos, freqs, axis, 3, interleaved)
+    ref.within(F().rotary(qkv, pos, freqs, axis, 3, interleaved=interleaved), value, bound, "out")
+    special = qkv.clone().view(2, 9, 3, 3, D)
+    special[..., 2 * P:] = torch.tensor([math.inf, -math.inf, math.nan, 1.5], device="cuda").to(dtype).repeat(D)[:D - 2 * P]
+    flat = special.view(2, 9, -1)
+    out = F().rotary(flat, pos, freqs, axis, 3, interleaved=interleaved)
+    again = F().rotary(flat.clone(), pos, freqs, axis, 3, interleaved=interleaved, inplace=True)
+    assert torch.equal(out.view(torch.uint8), again.view(torch.uint8))
+    tail = out.view(2, 9, 3, 3, D)[..., 2 * P:].contiguous()
+    assert torch.equal(tail.view(torch.uint8), special[..., 2 * P:].contiguous().view(torch.uint8))
+
+
 @pytest.mark.parametrize("kind", [torch.int64, torch.int32, torch.float32, torch.float64])
 def test_rotary_far_positions(kind):
     """Angles of 10^6 and more turns' worth: 32 bits would be off by a tenth of a radian."""
