@@ -6,8 +6,9 @@
 //
 // One pass: x and y are read once, s and h written once; s stays in registers in 32 bits between the sum and the
 // statistics of `pre` (which therefore see the unrounded sum), statistics are a true two-pass mean / variance.  Bound by
-// memory bandwidth (the layout of a row is in residual_norm_common.h): 64 x 197 x 1024 bf16 with `pre` 21 us, 4.8 TB/s; 64 x
-// 3136 x 96 bf16 with `post` 26 us; 24 x 257 x 1280 fp32 with both and a gate 24 us, 5.3 TB/s.
+// memory bandwidth (the layout of a row is in residual_norm_common.h): 64 x 197 x 1024 bf16 with `pre` 24 us, 4.3 TB/s; 64 x
+// 3136 x 96 bf16 with `post` 32 us, 3.6 TB/s; 24 x 257 x 1280 fp32 with both and a gate 31 us, 4.1 TB/s, behind the writes
+// of a backward pass (21, 26 and 24 us with inputs in the last-level cache).
 #include "residual_norm_common.h"
 
 namespace dpa {

@@ -4,9 +4,9 @@
 //     dx = gs,  dz = scale * gate * gs,  dgate = sum scale * gs * z,  dw_pre = sum dh * sh,  db_pre = sum dh
 //     dy = dz, or the same formula of `post` applied to it;  dw_post = sum dz * yh,  db_post = sum dz
 //
-// One pass: ds, dh, x, y are read once, dx and dy written once (64 x 197 x 1024 bf16 with `pre` 27 us, 4.8 TB/s; 64 x 3136 x
-// 96 bf16 with `post` 31 us; 24 x 257 x 1280 fp32 with both and a per-sample gate 51 us, 3.7 TB/s, bound by the two sums of a
-// row that follow each other; the fold 5.5 us, a launch and two waits for memory).  s is formed again from x and y in 32 bits: the s of
+// One pass: ds, dh, x, y are read once, dx and dy written once (64 x 197 x 1024 bf16 with `pre` 24 us, 5.3 TB/s; 64 x 3136 x
+// 96 bf16 with `post` 28 us, 4.1 TB/s; 24 x 257 x 1280 fp32 with both and a per-sample gate 42 us, 4.5 TB/s; the fold 4 us, a
+// launch and a wait for memory).  s is formed again from x and y in 32 bits: the s of
 // the forward pass is rounded to T, and 1 / deviation and the sums over rows magnify that (dw_pre of bf16 rows is off by
 // 2e-3 from it, by 2e-7 from this), for one more tensor to read where there is no `post` (5 in place of 4).  The per-channel sums stay with the lane across all rows
 // that it visits (its channels never change), meet across the row groups of a wave with shuffles and across waves in
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void residual_norm_bwd_kernel(con
       hi = min(lo + unit_rows, p.rows);
     }
     // the next row is requested before this one is worked on: a workgroup waits for memory and for its sums in turn otherwise
-    // (24 x 257 x 1280 fp32: 57 us against 44), where registers hold two rows without giving up residency
+    // (24 x 257 x 1280 fp32: 57 us against 42), where registers hold two rows without giving up residency
     constexpr bool AHEAD = MAXCH == 1 || (MAXCH == 2 && MODE != kAll);
     Row cur;
     if (AHEAD && lo + grp * rpw < hi) request(cur, lo + grp * rpw, hi);
@@ -363,8 +363,8 @@ struct Units {
   int splits;
   unsigned blocks;
 };
-// `parts`: how many workgroups the card holds at once.  More wait for a second turn, with a whole row of sums each; fewer leave
-// room (forward sums of 64 x 197 x 1024 bf16: 31 us with the 512 that fit, 37 with 768)
+// `parts`: how many workgroups the card holds at once (64 x 197 x 1024 bf16 with its fold: 31 us with the 512 that fit, 32 with
+// 256, 35 with 768, which take two turns)
 Units units_of(long rows, long per_sample, const Plan& pl, long parts, int gate_kind) {
   Units u;
   const long trip = pl.rows_per_trip;

@@ -6,8 +6,8 @@
 // pairs (2j, 2j + 1) or (j, j + P); the values and what lies behind the P pairs are copied.  The gradient is the same
 // with the angles negated.  The angle is formed in 64 bits and reduced to a fraction of a turn there (32 bits lose it for
 // far positions), sine and cosine of the fraction in 32: they are computed once per token and pair into LDS and serve
-// the 2 H heads.  Bound by memory bandwidth: 32 x 257 tokens of 3 x 16 x 80 bf16 23 us (5.5 TB/s, partly from cache), 4 x 3137
-// tokens of 3 x 16 x 64 fp16 37 us (4.2 TB/s).
+// the 2 H heads.  Bound by memory bandwidth: 32 x 257 tokens of 3 x 16 x 80 bf16 27 us (4.7 TB/s), 4 x 3137 tokens of 3 x 16 x 64
+// fp16 35 us (4.4 TB/s).
 #include "../common.h"
 #include "transformer.h"
 

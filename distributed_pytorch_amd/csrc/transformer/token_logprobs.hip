@@ -12,9 +12,9 @@
 // (order-preserving value bits, then the lower index), so ties go to the lowest index and the result does not depend on the
 // order of collection.  If more than the list's capacity reach the bound (many large elements with one lane), the k-th
 // largest collected becomes the new bound and the row is looked at again.  Few long rows are split over workgroups and
-// joined.  Bound by memory bandwidth: 2048 x 50257 bf16 with k = 20 73 us behind a backward pass's writes (54 us alone, of
-// which the k largest take 14), backward 86 us (4.8 TB/s); 1024 x 1000 fp32 8 + 6 us; one row of 128000 fp32 10 us and 5 to
-// join, bound by latency.
+// joined.  Bound by memory bandwidth and the exponentials' issue rate together: 2048 x 50257 bf16 with k = 20 48 us from the
+// last-level cache, 83 behind a backward pass's writes; backward 80 us (5.2 TB/s); 1024 x 1000 fp32 8 + 6 us; one row of 128000
+// fp32 9 us and 5 to join, bound by latency.
 #include "../common.h"
 #include "transformer.h"
 
