@@ -713,3 +713,31 @@ def test_refuses_mixed_devices():
                                     torch.zeros(4, dtype=torch.int32), 2)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_second_backward():
+    """A kept graph gives the same gradients again; a released one says so."""
+    case = _residual_case((2, 3, 16), torch.float32, None, "layer", None, False)
+    x = case[0].requires_grad_()
+    s, h = F().residual_norm(x, case[1], pre=case[5])
+    qkv, pos, freqs, axis = _rotary_case(1, 4, 1, 16, 8, 2, torch.float32)
+    z = normal(gen(0), (3, 20)).requires_grad_()
+    lp, ent, top, _ = F().token_logprobs(z, torch.zeros(3, dtype=torch.int64, device="cuda"), 4)
+    for out, leaf in ((s.sum() + h.square().sum(), x), (F().rotary(qkv.requires_grad_(), pos, freqs, axis, 1).square().sum(), qkv),
+                      (lp.sum() + (ent * ent).sum() + top.sum(), z)):
+        a, = torch.autograd.grad(out, leaf, retain_graph=True)
+        b, = torch.autograd.grad(out, leaf)
+        assert torch.equal(a, b)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out, leaf)
+
+
+def test_saved_values_changed_in_place():
+    """A value that backward needs and that was overwritten is noticed."""
+    z = normal(gen(0), (3, 20)).requires_grad_()
+    y = z * 1.0
+    lp, ent, _, _ = F().token_logprobs(y, torch.zeros(3, dtype=torch.int64, device="cuda"))
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lp.sum().backward()
