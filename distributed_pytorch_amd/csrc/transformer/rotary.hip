@@ -23,8 +23,10 @@ __device__ __forceinline__ double position(const void* p, long i, int kind) {
   }
 }
 
-// VEC: D, P (not INTER) and every row are whole 16-byte chunks; else element by element
-template <typename T, bool VEC, bool INTER>
+// VEC: D, P (not INTER) and every row are whole 16-byte chunks; else element by element.  ANY (not INTER, not in place): P may
+// be anything, a chunk's partners come from wherever they start (33 x 1765 tokens of 3 x 6 x 48 bf16, P = 15: 68 us, element
+// by element 115)
+template <typename T, bool VEC, bool INTER, bool ANY>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const int tt, const FastDiv by_items,
                                                      const FastDiv by_chunks, const FastDiv by_rest) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
@@ -55,8 +57,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
   const bool copy = p.in != p.out;
   // items of one token: the chunks (pairs of chunks) that turn, then the ones that are copied
   // per head; INTER: the last one may hold pairs that stay; not INTER: with a partner P further on
-  const int chunks = ((INTER ? 2 * P : P) + V - 1) / V;
-  const int rest = INTER ? D / V - chunks : (D - 2 * P) / V;
+  const int chunks = ANY ? D / V : ((INTER ? 2 * P : P) + V - 1) / V;
+  const int rest = ANY ? 0 : (INTER ? D / V - chunks : (D - 2 * P) / V);
   const int n_turn = 2 * H * chunks;
   const int n_rest = copy ? 2 * H * rest : 0;
   const int items = n_turn + n_rest + (copy ? H * D / V : 0);
@@ -83,6 +85,26 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
             const float a = v.get(j), b2 = v.get(j + 1);
             v.set(j, a * c.x - b2 * c.y);
             v.set(j + 1, a * c.y + b2 * c.x);
+          }
+          v.store(dst + o);
+        } else if constexpr (ANY) {
+          // (behind the last key head lie the values: a read of up to V - 1 elements too many stays in the token's row)
+          Vec16<T> v, above, below;
+          v.load(src + o);
+          if (j0 < P) __builtin_memcpy(&above.raw, src + o + P, 16);
+          if (j0 >= P && j0 < 2 * P) __builtin_memcpy(&below.raw, src + o - P, 16);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const int e = j0 + j;
+            if (e < P) {
+              const float2 c = cs[e];
+              const float a = v.get(j), b2 = above.get(j);
+              v.set(j, a * c.x - b2 * c.y);
+            } else if (e < 2 * P) {
+              const float2 c = cs[e - P];
+              const float a = j0 >= P ? below.get(j) : to_float(src[o + j - P]), b2 = v.get(j);
+              v.set(j, a * c.y + b2 * c.x);
+            }
           }
           v.store(dst + o);
         } else {
@@ -136,13 +158,14 @@ template <typename T>
 void launch(const RotaryParams& p, hipStream_t s) {
   const int V = 16 / (int)sizeof(T);
   auto off16 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0; };
-  const bool vec = p.D % V == 0 && (p.interleaved || p.pairs % V == 0) &&
+  const bool copy = p.in != p.out;
+  const bool any = !p.interleaved && p.pairs % V != 0 && copy;
+  const bool vec = p.D % V == 0 && (p.interleaved || p.pairs % V == 0 || any) &&
                    !off16(p.in) && !off16(p.out) && p.in_batch % V == 0 && p.in_token % V == 0 && p.out_batch % V == 0 &&
                    p.out_token % V == 0;
   const int v = vec ? V : 1;
-  const bool copy = p.in != p.out;
-  const int chunks = ((p.interleaved ? 2 * p.pairs : p.pairs) + v - 1) / v;
-  const int rest = p.interleaved ? p.D / v - chunks : (p.D - 2 * p.pairs) / v;
+  const int chunks = vec && any ? p.D / v : ((p.interleaved ? 2 * p.pairs : p.pairs) + v - 1) / v;
+  const int rest = vec && any ? 0 : (p.interleaved ? p.D / v - chunks : (p.D - 2 * p.pairs) / v);
   const int items = 2 * p.H * chunks + (copy ? 2 * p.H * rest + p.H * p.D / v : 0);
   if (items <= 0) return;
   // many short workgroups, whose angles and copies overlap, one token each for short calls (4 x 3137 tokens of 3 x 16 x 64
@@ -155,14 +178,15 @@ void launch(const RotaryParams& p, hipStream_t s) {
   const size_t lds = (size_t)(tt * p.pairs * 8 + 8);
   const FastDiv bi = make_fastdiv((uint32_t)items), bc = make_fastdiv((uint32_t)(chunks > 0 ? chunks : 1)),
                 br = make_fastdiv((uint32_t)(rest > 0 ? rest : 1));
-#define DPA_ROTARY(VECB, INTERB) \
-  hipLaunchKernelGGL((rotary_kernel<T, VECB, INTERB>), dim3((unsigned)blocks), dim3(256), lds, s, p, (int)tt, bi, bc, br)
+#define DPA_ROTARY(VECB, INTERB, ANYB) \
+  hipLaunchKernelGGL((rotary_kernel<T, VECB, INTERB, ANYB>), dim3((unsigned)blocks), dim3(256), lds, s, p, (int)tt, bi, bc, br)
   if (vec) {
-    if (p.interleaved) DPA_ROTARY(true, true);
-    else DPA_ROTARY(true, false);
+    if (p.interleaved) DPA_ROTARY(true, true, false);
+    else if (any) DPA_ROTARY(true, false, true);
+    else DPA_ROTARY(true, false, false);
   } else {
-    if (p.interleaved) DPA_ROTARY(false, true);
-    else DPA_ROTARY(false, false);
+    if (p.interleaved) DPA_ROTARY(false, true, false);
+    else DPA_ROTARY(false, false, false);
   }
 #undef DPA_ROTARY
   DPA_CHECK_HIP(hipGetLastError());
