@@ -514,7 +514,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const T
 
 // ------------------------------------------------------------------------------------------ Newton-Schulz and Muon
 // out may be g itself (contiguous then)
-Tensor newton_schulz(const Tensor& g0, const OptTensor& into, int64_t steps, double a, double b, double c, double eps) {
+Tensor newton_schulz(const Tensor& g0, const OptTensor& into, int64_t steps, double a, double b, double c, double eps, bool fast) {
   const Tensor g = g0.contiguous();
   const c10::DeviceGuard guard(g.device());
   const Tensor out = into.has_value() ? *into : at::empty_like(g);
@@ -522,7 +522,7 @@ Tensor newton_schulz(const Tensor& g0, const OptTensor& into, int64_t steps, dou
   p.rows = g.size(-2); p.cols = g.size(-1); p.batch = g.numel() / (p.rows * p.cols);
   const Tensor work = at::empty({(int64_t)newton_schulz_workspace(p.batch, p.rows, p.cols)}, g.options().dtype(at::kByte));
   p.g = g.data_ptr(); p.out = out.data_ptr(); p.work = work.data_ptr();
-  p.steps = (int)steps; p.a = (float)a; p.b = (float)b; p.c = (float)c; p.eps = eps;
+  p.steps = (int)steps; p.a = (float)a; p.b = (float)b; p.c = (float)c; p.eps = eps; p.fast = fast;
   newton_schulz_launch(p, code(g), stream_of(g));
   return out;
 }

@@ -7,12 +7,14 @@
 // and the scale keeps small entries clear of the subnormals) in fp16 planes: `hi`, and `lo` with what hi leaves, together
 // 22 significant bits.
 //
-//  * PAIR (fp32 and fp16 results): every operand is hi + lo and a product is hi hi + hi lo + lo hi in fp32 accumulators,
-//    32-bit products at three times the cost of one fp16 product; fp32's own matrix rate is 1 / 16 of fp16's.
-//  * single (bf16 results): products take the hi planes alone, a third of the cost.  What keeps the error (2e-4 .. 7e-4,
-//    2e-3 where a few directions are 100 times the rest) below the rounding of the result (1.7e-3): X itself stays hi + lo
-//    (with one plane: 5e-3 to 2e-2 there), and the diagonals of A and B, which are near 1 and -2.7 and would be rounded
-//    as such (1.4e-3 to 1.8e-3 by themselves), are kept apart in fp32; with A = Ao + Da,
+//  * PAIR (whatever the caller's type): every operand is hi + lo and a product is hi hi + hi lo + lo hi in fp32
+//    accumulators, 32-bit products at three times the cost of one fp16 product; fp32's own matrix rate is 1 / 16 of fp16's.
+//    A bf16 result is the 32-bit one, rounded once.
+//  * single (bf16 results of a caller who asks for it, `fast`): products take the hi planes alone, a third of the cost, and
+//    11 significant bits.  What keeps the error (2e-4 .. 7e-4 of the result's norm, 2e-3 where a few directions are 100
+//    times the rest) below the rounding of the result (1.7e-3): X itself stays hi + lo (with one plane: 5e-3 to 2e-2 there),
+//    and the diagonals of A and B, which are near 1 and -2.7 and would be rounded as such (1.4e-3 to 1.8e-3 by
+//    themselves), are kept apart in fp32; with A = Ao + Da,
 //        A A = Ao Ao + (Da_i + Da_j) Ao_ij + Da^2,   a X + B X = (a + Db_i) X_ij + Bo X.
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed.  X is also kept transposed, because B X needs
@@ -957,7 +959,7 @@ __global__ __launch_bounds__(512, 1) void ns_large_kernel(const Product p, const
 
 // Tile of the products, and with it the padding: 256 x 256 where A has enough of those tiles that are not padding.  Five
 // steps, small tiles against large ones, us (tiles of A; volume: what the larger padding multiplies the products by):
-//     bf16  7 x 1024 x 4096 (70 tiles)   1170 : 1170      fp32  2492 : 2628
+//     fast  7 x 1024 x 4096 (70 tiles)   1170 : 1170      fp32  2492 : 2628
 //          10 x 1024 x 4096 (100)        1753 : 1463            3574 : 3185
 //          22 x 1024 x 4096 (220)        3768 : 2573            7884 : 5724
 //           5 x 1024 x 1024 (50)          388 :  534             756 : 1137
@@ -1009,7 +1011,7 @@ Sizes sizes(long batch, long rows, long cols) {
   z.np = (z.n + tile - 1) / tile * tile;
   // enough 64 x 64 tiles for two rounds of workgroups, and rows that fill 128-row tiles.  Five steps with 64 x 64 tiles against
   // 128 x 128 ones, us: 256 x 2304 fp32, 3 matrices (432 tiles) 195 : 202, 4 (576) 216 : 201, 6 (864) 238 : 217; 768 x 768
-  // bf16, 3 (432) 162 : 169, 4 (576) 242 : 225; 1024 x 1024 bf16, 2 (512) 234 : 246, 3 (768) 279 : 259
+  // fast, 3 (432) 162 : 169, 4 (576) 242 : 225; 1024 x 1024 fast, 2 (512) 234 : 246, 3 (768) 279 : 259
   z.mid = !z.large && z.mp % kMid == 0 && batch * (z.mp / kSmall) * (z.np / kSmall) > 512;
   if (z.mid) z.np = (z.np + kMid - 1) / kMid * kMid;
   z.x = (size_t)batch * z.mp * z.np * 2;
@@ -1093,10 +1095,14 @@ void newton_schulz_launch(const NewtonSchulz& q, int dtype, hipStream_t s) {
   if (q.batch <= 0 || q.rows <= 0 || q.cols <= 0 || q.steps <= 0) throw std::invalid_argument("newton_schulz: empty shape or no steps");
   const Sizes z = sizes(q.batch, q.rows, q.cols);
   if (q.batch > 65535 || z.mp / 64 > 65535) throw std::invalid_argument("newton_schulz: too many matrices");
+  if (q.fast && dtype != kBF16) throw std::invalid_argument("newton_schulz: fast products are for bfloat16");
   switch (dtype) {
     case kF32: run<true, float>(q, s); break;
     case kF16: run<true, f16_t>(q, s); break;
-    case kBF16: run<false, bf16_t>(q, s); break;
+    case kBF16:
+      if (q.fast) run<false, bf16_t>(q, s);
+      else run<true, bf16_t>(q, s);
+      break;
     default: throw std::invalid_argument("unsupported dtype");
   }
   DPA_CHECK_HIP(hipGetLastError());

@@ -85,6 +85,7 @@ struct NewtonSchulz {
   int steps = 0;
   float a = 0.f, b = 0.f, c = 0.f;
   double eps = 0.0;
+  bool fast = false;                                               // bf16 alone: products of single fp16 planes
 };
 size_t newton_schulz_workspace(long batch, long rows, long cols);
 void newton_schulz_launch(const NewtonSchulz& p, int dtype, hipStream_t s);      // out may be g

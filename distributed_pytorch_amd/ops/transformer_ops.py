@@ -54,9 +54,9 @@ def token_logprobs(logits, target, k):
     return (_T or T()).token_logprobs(logits, target, k)
 
 
-def newton_schulz(g, steps, coefficients, eps):
+def newton_schulz(g, steps, coefficients, eps, fast):
     a, b, c = coefficients
-    return T().newton_schulz(g.detach(), None, steps, a, b, c, eps)
+    return T().newton_schulz(g.detach(), None, steps, a, b, c, eps, fast)
 
 
 def matrix_shape(p):
@@ -147,7 +147,7 @@ class MuonPlan:
             T().muon_begin(gt["table"], gt["n"], gt["chunks"], gt["g_dtype"], gt["hyper"], inv, found, u)
             for at, count, rows, cols in gt["buckets"]:
                 m = u[at:at + count * rows * cols].view(count, rows, cols)
-                T().newton_schulz(m, m, g["ns_steps"], a, b, c, g["ns_eps"])
+                T().newton_schulz(m, m, g["ns_steps"], a, b, c, g["ns_eps"], False)
             T().muon_end(gt["table"], gt["n"], gt["chunks"], gt["lp_dtype"], gt["hyper"], found, u)
 
     def stamp_copies(self) -> None:
