@@ -58,6 +58,13 @@ bool tracked(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// A tangent would be left out of the results without a word: these operators have no forward-mode derivative.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename... Ts> void no_tangents(const char* op, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(ts) || ...), op, ": forward-mode derivatives are not implemented");
+}
+
 // ---- what ops/functional.py checks, argument by argument
 bool float_type(const Tensor& t) {
   const auto d = t.scalar_type();
@@ -287,6 +294,7 @@ std::optional<std::pair<OptTensor, OptTensor>> residual_norm(const Tensor& x, co
                                               const OptTensor& post_b, int64_t post, double post_eps, const OptTensor& pre_w,
                                               const OptTensor& pre_b, int64_t pre, double pre_eps, const OptTensor& gate,
                                               const OptTensor& scale, bool sinks) {
+  no_tangents("residual_norm", x, y, post_w, post_b, pre_w, pre_b, gate, scale);
   if (!x.is_cuda() || !rows_taken(x) || !norm_taken(post_w, post_b, post, post_eps, x) || !norm_taken(pre_w, pre_b, pre, pre_eps, x))
     return std::nullopt;
   if (y.has_value()) {
@@ -399,6 +407,7 @@ bool rotary_taken(const Tensor& qkv, const Tensor& pos, const Tensor& freqs, con
 // (`inplace`: its strides have been checked)
 OptTensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs, const Tensor& axis, int64_t heads,
                  bool interleaved, bool inplace) {
+  no_tangents("rotary", qkv, positions, freqs);
   if (!rotary_taken(qkv, positions, freqs, axis, heads)) return std::nullopt;
   const Tensor pos = positions.contiguous(), f = freqs.contiguous(), a = axis.to(at::kInt).contiguous();
   if (inplace) {
@@ -485,6 +494,7 @@ struct TokenLogprobsBackward : Node {
 
 // logits [N, V]
 std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const Tensor& logits, const Tensor& target, int64_t k) {
+  no_tangents("token_logprobs", logits);
   const auto type = target.scalar_type();
   if (!logits.is_cuda() || !float_type(logits) || logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > 1l << 30 ||
       target.dim() != 1 || target.size(0) != logits.size(0) || target.device() != logits.device() ||

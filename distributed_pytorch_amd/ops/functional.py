@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as TF
+from torch.autograd import forward_ad
 
 
 def _on_gpu(t: torch.Tensor) -> bool:
@@ -674,6 +675,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
     _check_schulz(tuple(float(v) for v in coefficients), int(steps))
     if torch.is_grad_enabled() and g.requires_grad:
         raise ValueError("newton_schulz: has no gradient (detach the update)")
+    if forward_ad.unpack_dual(g).tangent is not None:
+        raise ValueError("newton_schulz: has no gradient, forward-mode either (detach the update)")
     if _on_gpu(g):
         return _tops().newton_schulz(g, steps, coefficients, eps, bool(fast))
     a, b, c = coefficients

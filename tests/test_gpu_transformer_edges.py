@@ -2,6 +2,7 @@
 size of workgroup, vectors, sinks of gates, extreme gradients.  Bounds are those of tests/_transformer_ref.py."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import _transformer_ref as ref
 
@@ -29,6 +30,38 @@ def gen(seed):
 
 def normal(g, shape, dtype=torch.float32, std=1.0, mean=0.0):
     return (torch.randn(shape, generator=g, device="cuda") * std + mean).to(dtype)
+
+
+def _calls():
+    """{name: (call of one tensor, that tensor)}; every floating-point argument of every operator once."""
+    g = gen(0)
+    x, y, w, b = normal(g, (2, 3, 16)), normal(g, (2, 3, 16)), normal(g, (16,)), normal(g, (16,))
+    pos = torch.arange(4, device="cuda")[:, None].expand(4, 2).contiguous()
+    qkv, freqs, axis = normal(g, (1, 4, 48)), normal(g, (8,)).double(), torch.zeros(8, dtype=torch.int32, device="cuda")
+    z, t = normal(g, (3, 20)), torch.zeros(3, dtype=torch.int64, device="cuda")
+    norm = lambda v, q: F().Norm(v, q, 1e-5, "layer")                                                       # noqa: E731
+    return {
+        "x": (lambda v: F().residual_norm(v, y, pre=norm(w, b))[1], x),
+        "y": (lambda v: F().residual_norm(x, v), y),
+        "post.weight": (lambda v: F().residual_norm(x, y, post=norm(v, b)), w),
+        "post.bias": (lambda v: F().residual_norm(x, y, post=norm(w, v)), b),
+        "pre.weight": (lambda v: F().residual_norm(x, y, pre=norm(v, b))[1], w),
+        "pre.bias": (lambda v: F().residual_norm(x, y, pre=norm(w, v))[1], b),
+        "gate": (lambda v: F().residual_norm(x, y, gate=v), w),
+        "scale": (lambda v: F().residual_norm(x, y, scale=v), torch.ones(2, device="cuda")),
+        "rms_norm": (lambda v: F().rms_norm(v, w), x),
+        "rms_norm.weight": (lambda v: F().rms_norm(x, v), w),
+        "rotary": (lambda v: F().rotary(v, pos, freqs, axis, 1), qkv),
+        "rotary.inplace": (lambda v: F().rotary(v, pos, freqs, axis, 1, inplace=True), qkv.clone()),
+        "rotary.positions": (lambda v: F().rotary(qkv, v, freqs, axis, 1), pos.double()),
+        "rotary.freqs": (lambda v: F().rotary(qkv, pos, v, axis, 1), freqs),
+        "token_logprobs": (lambda v: F().token_logprobs(v, t, 3)[0], z),
+        "newton_schulz": (lambda v: F().newton_schulz(v), normal(g, (12, 20))),
+    }
+
+
+CALLS = ["x", "y", "post.weight", "post.bias", "pre.weight", "pre.bias", "gate", "scale", "rms_norm", "rms_norm.weight", "rotary",
+         "rotary.inplace", "rotary.positions", "rotary.freqs", "token_logprobs", "newton_schulz"]
 
 
 # ------------------------------------------------------------------------------------------ Newton-Schulz of bf16 updates
@@ -59,3 +92,20 @@ def test_newton_schulz_fast_is_for_bf16():
     for dtype in (torch.float32, torch.float16):
         with pytest.raises(ValueError, match="bfloat16"):
             F().newton_schulz(torch.ones(4, 8, dtype=dtype, device="cuda"), fast=True)
+
+
+# ------------------------------------------------------------------------------------------ tangents, traces, tensor subclasses
+@pytest.mark.parametrize("name", CALLS)
+def test_tangents_are_refused(name):
+    """A forward-mode derivative is refused, not left out, with and without requires_grad, and in-place data stays as it is."""
+    call, v = _calls()[name]
+    before = v.clone()
+    with fwd.dual_level():
+        dual = fwd.make_dual(v, torch.ones_like(v))
+        with pytest.raises((NotImplementedError, ValueError), match="forward-mode|no gradient"):
+            call(dual)
+    torch.cuda.synchronize()
+    assert torch.equal(v, before)
+    call(v)                                        # (and no tangent, no refusal)
+    with fwd.dual_level():
+        call(v)

@@ -1,6 +1,7 @@
 """The transformer operators' refusals, modules and optimizer at their edges, on the CPU backend."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from distributed_pytorch_amd.ops import functional as F
 
@@ -11,3 +12,42 @@ def test_newton_schulz_fast_is_for_bf16():
         with pytest.raises(ValueError, match="bfloat16"):
             F.newton_schulz(g.to(dtype), fast=True)
     assert torch.equal(F.newton_schulz(g.bfloat16(), fast=True), F.newton_schulz(g.bfloat16()))     # (32 bits here either way)
+
+
+def _native_calls():
+    """{name: (call of the native module with one floating-point argument, that argument)}: what it refuses, it refuses before it
+    looks at the device."""
+    from distributed_pytorch_amd.ops.transformer_ops import T
+
+    x, y, w = torch.randn(2, 3, 16), torch.randn(2, 3, 16), torch.randn(16)
+    qkv, pos, freqs, axis = torch.randn(1, 4, 48), torch.zeros(4, 2), torch.ones(8), torch.zeros(8, dtype=torch.int32)
+
+    def rn(**kw):
+        a = dict(x=x, y=y, post_w=None, post_b=None, post=0, post_eps=0.0, pre_w=None, pre_b=None, pre=0, pre_eps=0.0, gate=None,
+                 scale=None)
+        a.update(kw)
+        return T().residual_norm(*a.values(), False)
+
+    calls = {k: (lambda v, k=k: rn(**{k: v}), v) for k, v in (
+        ("x", x), ("y", y), ("post_w", w), ("post_b", w), ("pre_w", w), ("pre_b", w), ("gate", w), ("scale", torch.ones(2)))}
+    calls["qkv"] = (lambda v: T().rotary(v, pos, freqs, axis, 1, False, False), qkv)
+    calls["inplace"] = (lambda v: T().rotary(v, pos, freqs, axis, 1, False, True), qkv)
+    calls["positions"] = (lambda v: T().rotary(qkv, v, freqs, axis, 1, False, False), pos)
+    calls["freqs"] = (lambda v: T().rotary(qkv, pos, v, axis, 1, False, False), freqs)
+    calls["logits"] = (lambda v: T().token_logprobs(v, torch.zeros(2, dtype=torch.int64), 3), torch.randn(2, 9))
+    return calls
+
+
+def test_native_module_refuses_tangents():
+    for name, (call, v) in _native_calls().items():
+        assert call(v) is None, name                # (not a GPU tensor: not taken, and no error)
+        with fwd.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(fwd.make_dual(v, torch.ones_like(v)))
+
+
+def test_newton_schulz_refuses_tangents():
+    with fwd.dual_level():
+        F.newton_schulz(torch.ones(3, 4))
+        with pytest.raises(ValueError, match="no gradient"):
+            F.newton_schulz(fwd.make_dual(torch.ones(3, 4), torch.ones(3, 4)))
