@@ -8,10 +8,12 @@
 // Outputs and workspaces come from torch's allocator per call and launches go to torch's current stream of the tensors'
 // device: nothing is shared between two calls or two graphs, and nothing synchronises with the host.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <ATen/TracerMode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -65,6 +67,30 @@ template <typename... Ts> void no_tangents(const char* op, const Ts&... ts) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(ts) || ...), op, ": forward-mode derivatives are not implemented");
 }
 
+// Only the allocation of results goes through torch's dispatcher.  Who records a call there (torch.jit.trace, make_fx,
+// fake tensors) would hold buffers that nothing fills, and a tensor subclass or wrapper has no memory that a kernel could read.
+void not_recorded(const char* op) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::tracer::impl::is_dispatch_enabled(), op, ": cannot be traced");
+  if (Modes::any_modes_set())
+    TORCH_CHECK_NOT_IMPLEMENTED(!Modes::get_mode(Key::PROXY) && !Modes::get_mode(Key::FAKE) && !Modes::get_mode(Key::FUNCTIONAL),
+                                op, ": cannot be traced");
+}
+bool is_plain(const Tensor& t) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet wrapped({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
+                                         DispatchKey::FuncTorchGradWrapper});
+  return !t.defined() || !t.key_set().has_any(wrapped);
+}
+bool is_plain(const OptTensor& t) { return !t.has_value() || is_plain(*t); }
+// in front of everything else that an operator does
+template <typename... Ts> void check_call(const char* op, const Ts&... ts) {
+  not_recorded(op);
+  TORCH_CHECK_NOT_IMPLEMENTED((is_plain(ts) && ...), op, ": tensor subclasses and wrappers are not supported");
+  no_tangents(op, ts...);
+}
+
 // ---- what ops/functional.py checks, argument by argument
 bool float_type(const Tensor& t) {
   const auto d = t.scalar_type();
@@ -84,6 +110,7 @@ bool norm_taken(const OptTensor& w, const OptTensor& b, int64_t kind, double eps
 
 // a gradient of a gradient would silently be missing
 void once(const char* op) {
+  not_recorded(op);
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass is not differentiable (create_graph)");
 }
 
@@ -294,7 +321,7 @@ std::optional<std::pair<OptTensor, OptTensor>> residual_norm(const Tensor& x, co
                                               const OptTensor& post_b, int64_t post, double post_eps, const OptTensor& pre_w,
                                               const OptTensor& pre_b, int64_t pre, double pre_eps, const OptTensor& gate,
                                               const OptTensor& scale, bool sinks) {
-  no_tangents("residual_norm", x, y, post_w, post_b, pre_w, pre_b, gate, scale);
+  check_call("residual_norm", x, y, post_w, post_b, pre_w, pre_b, gate, scale);
   if (!x.is_cuda() || !rows_taken(x) || !norm_taken(post_w, post_b, post, post_eps, x) || !norm_taken(pre_w, pre_b, pre, pre_eps, x))
     return std::nullopt;
   if (y.has_value()) {
@@ -407,7 +434,7 @@ bool rotary_taken(const Tensor& qkv, const Tensor& pos, const Tensor& freqs, con
 // (`inplace`: its strides have been checked)
 OptTensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs, const Tensor& axis, int64_t heads,
                  bool interleaved, bool inplace) {
-  no_tangents("rotary", qkv, positions, freqs);
+  check_call("rotary", qkv, positions, freqs, axis);
   if (!rotary_taken(qkv, positions, freqs, axis, heads)) return std::nullopt;
   const Tensor pos = positions.contiguous(), f = freqs.contiguous(), a = axis.to(at::kInt).contiguous();
   if (inplace) {
@@ -494,7 +521,7 @@ struct TokenLogprobsBackward : Node {
 
 // logits [N, V]
 std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const Tensor& logits, const Tensor& target, int64_t k) {
-  no_tangents("token_logprobs", logits);
+  check_call("token_logprobs", logits, target);
   const auto type = target.scalar_type();
   if (!logits.is_cuda() || !float_type(logits) || logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > 1l << 30 ||
       target.dim() != 1 || target.size(0) != logits.size(0) || target.device() != logits.device() ||
@@ -525,6 +552,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const T
 // ------------------------------------------------------------------------------------------ Newton-Schulz and Muon
 // out may be g itself (contiguous then)
 Tensor newton_schulz(const Tensor& g0, const OptTensor& into, int64_t steps, double a, double b, double c, double eps, bool fast) {
+  check_call("newton_schulz", g0);
   const Tensor g = g0.contiguous();
   const c10::DeviceGuard guard(g.device());
   const Tensor out = into.has_value() ? *into : at::empty_like(g);

@@ -109,3 +109,45 @@ def test_tangents_are_refused(name):
     call(v)                                        # (and no tangent, no refusal)
     with fwd.dual_level():
         call(v)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tracing_is_refused(name):
+    """A trace would hold the allocation of the result and nothing that fills it."""
+    call, v = _calls()[name]
+    with pytest.raises((NotImplementedError, RuntimeError), match="trac"):
+        torch.jit.trace(call, (v,), check_trace=False)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_fake_tensors_and_graph_tracing_are_refused(name):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    call, v = _calls()[name]
+    mode = FakeTensorMode(allow_non_fake_inputs=True)
+    with pytest.raises(NotImplementedError, match="traced|subclasses"):
+        call(mode.from_tensor(v))
+    with mode, pytest.raises(NotImplementedError, match="traced|subclasses"):
+        call(v)
+    with pytest.raises(NotImplementedError, match="traced|subclasses"):
+        make_fx(call)(v)
+
+
+def test_backward_is_not_traced_either():
+    x = normal(gen(0), (2, 3, 16)).requires_grad_()
+    h = F().rms_norm(x, torch.ones(16, device="cuda"))
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    with pytest.raises(NotImplementedError, match="traced"):
+        make_fx(lambda v: torch.autograd.grad(h, x, v, retain_graph=True)[0])(torch.ones_like(h))
+
+
+def test_modes_that_watch_are_welcome():
+    """A mode that only watches what torch allocates changes nothing."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    x, w = normal(gen(0), (2, 3, 16)), torch.ones(16, device="cuda")
+    want = F().rms_norm(x, w)
+    with FlopCounterMode(display=False):
+        assert torch.equal(F().rms_norm(x, w), want)

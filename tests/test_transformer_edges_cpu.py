@@ -46,6 +46,38 @@ def test_native_module_refuses_tangents():
                 call(fwd.make_dual(v, torch.ones_like(v)))
 
 
+def test_native_module_refuses_what_records_it():
+    """Traces, fake tensors, functional wrappers, tensor subclasses: the results would be buffers that nothing fills, and the
+    arguments have no memory to read."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    class Watched(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return NotImplemented
+
+    for name, (call, v) in _native_calls().items():
+        with pytest.raises((NotImplementedError, RuntimeError), match="traced"):
+            torch.jit.trace(call, (v,), check_trace=False)
+        with pytest.raises(NotImplementedError, match="traced|subclasses"):
+            make_fx(lambda u: call(u))(v)
+        mode = FakeTensorMode(allow_non_fake_inputs=True)
+        fake = mode.from_tensor(v)
+        with pytest.raises(NotImplementedError, match="subclasses"):
+            call(fake)
+        with mode, pytest.raises(NotImplementedError, match="traced"):
+            call(v)
+        with pytest.raises(NotImplementedError, match="subclasses"):
+            call(torch._to_functional_tensor(v))
+        with pytest.raises(NotImplementedError, match="subclasses"):
+            call(torch.Tensor._make_subclass(Watched, v))
+        with pytest.raises(NotImplementedError, match="subclasses"):
+            torch.func.vmap(lambda u: call(u), in_dims=0)(torch.stack([v, v]))
+        assert call(v) is None and call(torch.nn.Parameter(v) if v.is_floating_point() and name not in ("scale", "positions", "freqs")
+                                        else v) is None
+
+
 def test_newton_schulz_refuses_tangents():
     with fwd.dual_level():
         F.newton_schulz(torch.ones(3, 4))
