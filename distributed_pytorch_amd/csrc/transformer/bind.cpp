@@ -140,7 +140,7 @@ RowShape row_shape(const Tensor& x) {
   RowShape r;
   r.C = (int)x.size(-1);
   r.rows = x.numel() / r.C;
-  r.per_sample = x.size(0) > 0 && r.rows > 0 ? r.rows / x.size(0) : 1;
+  r.per_sample = x.dim() > 1 && x.size(0) > 0 && r.rows > 0 ? r.rows / x.size(0) : 1;      // (a vector is one row, no samples)
   return r;
 }
 // fp32 copies of post_w, post_b, pre_w, pre_b, gate, scale

@@ -151,3 +151,21 @@ def test_modes_that_watch_are_welcome():
     want = F().rms_norm(x, w)
     with FlopCounterMode(display=False):
         assert torch.equal(F().rms_norm(x, w), want)
+
+
+# ------------------------------------------------------------------------------------------ residual norm
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [1, 8, 33, 768, 4099])
+def test_rms_norm_of_a_vector(C, dtype):
+    g = gen(C)
+    x, w, dh = normal(g, (C,), dtype, 2.0), normal(g, (C,), std=0.2, mean=1.0), normal(g, (C,), dtype)
+    want = ref.residual_norm(x[None], torch.zeros_like(x)[None], None, None, None, F().Norm(w, None, 1e-6, "rms"), None, dh[None])
+    x.requires_grad_()
+    w.requires_grad_()
+    h = F().rms_norm(x, w, 1e-6)
+    dx, dw = torch.autograd.grad(h, [x, w], dh)
+    for name, got in (("h", h), ("d_x", dx)):
+        ref.within(got, want[name][0][0], want[name][1][0], name)
+    ref.within(dw, *want["d_pre_w"], "dw")
+    with torch.no_grad():
+        assert torch.equal(h, F().rms_norm(x, w, 1e-6))
