@@ -470,11 +470,12 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogp
     for (int i = lo + tid; i < hi; i += 256) dz[i] = from_float<T>(0.f);
     return;
   }
-  // p (-gsum - ge (log p + H)) with log p = d - ls, d = z - m; where p is 0 d is kept finite
+  // p (-gsum - ge (log p + H)) with log p = d - ls, d = z - m.  Below -128 p is 0 (ls >= 0, and e^-104 is under the smallest
+  // float): d stops there, so that its product with ge does not overflow beside a p of 0
   const float c0 = -gsum - ge * H + ge * ls, shift = -ls * kLog2e;
   const auto grad = [&](float v) {
     const float d = v - m;
-    return __builtin_amdgcn_exp2f(fmaf(d, kLog2e, shift)) * fmaf(-ge, fmaxf(d, -1e30f), c0);
+    return __builtin_amdgcn_exp2f(fmaf(d, kLog2e, shift)) * fmaf(-ge, fmaxf(d, -128.f), c0);
   };
   const auto chunk = [&](const Vec16<T>& v) {
     Vec16<T> o;

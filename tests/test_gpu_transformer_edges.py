@@ -1,5 +1,7 @@
 """Calls at the edge of what the transformer operators take: who watches a call (tangents, traces, tensor subclasses), every
 size of workgroup, vectors, sinks of gates, extreme gradients.  Bounds are those of tests/_transformer_ref.py."""
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -169,3 +171,26 @@ def test_rms_norm_of_a_vector(C, dtype):
     ref.within(dw, *want["d_pre_w"], "dw")
     with torch.no_grad():
         assert torch.equal(h, F().rms_norm(x, w, 1e-6))
+
+
+# ------------------------------------------------------------------------------------------ log probabilities
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e9, 1e30])
+def test_token_logprobs_large_entropy_gradients_beside_masked_classes(size, dtype):
+    """A masked class has no gradient however large the entropy's is (a loss scale on top of a large weight)."""
+    g = gen(5)
+    z = normal(g, (3, 300))
+    z[0, ::3] = -math.inf
+    z[1, 1:] = torch.finfo(dtype).min
+    z[2] = z[2] * 10
+    z = z.to(dtype).requires_grad_()
+    t = torch.zeros(3, dtype=torch.int64, device="cuda") + 1
+    _, ent, _, _ = F().token_logprobs(z, t)
+    d_ent = normal(g, (3,)) * size
+    (d,) = torch.autograd.grad(ent, z, d_ent)
+    assert not d[0, ::3].any()
+    value, bound = ref.token_logprobs(z, t, 0, torch.zeros(3), d_ent)["d_logits"]
+    if dtype == torch.float16:                                # (values past its range are infinite)
+        assert not d.isnan().any()
+    else:
+        ref.within(d, value, bound, "d_logits")
