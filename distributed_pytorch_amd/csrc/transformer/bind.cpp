@@ -251,8 +251,9 @@ struct ResidualNormBackward : Node {
     if (any_leaf) {
       const py::gil_scoped_acquire gil;
       for (int i = 0; i < 5; ++i) {
-        if (!need[i] || (i == 4 && gate_kind == kGateSample)) continue;
+        if (!need[i]) continue;
         find_sink(params[i], sinks[i]);
+        if (i == 4 && gate_kind == kGateSample) sinks[i].sink = py::object();      // its sums have a buffer of their own
         for (int j = 0; j < i; ++j)             // a parameter used twice in this call: its second sum has a buffer of its own
           if (sinks[j].sink && sinks[i].sink && sinks[j].sink.is(sinks[i].sink)) sinks[i].sink = py::object();
       }

@@ -173,6 +173,29 @@ def test_rms_norm_of_a_vector(C, dtype):
         assert torch.equal(h, F().rms_norm(x, w, 1e-6))
 
 
+def test_gate_of_samples_with_a_sink():
+    """A per-sample gate that is a parameter of a gradient arena: delivered like any other, over two uses, and nothing is owed
+    to its sink afterwards."""
+    from distributed_pytorch_amd.parallel.distributed import GradArena
+
+    g = gen(3)
+    x, y, ds = normal(g, (4, 5, 24)), normal(g, (4, 5, 24)), normal(g, (4, 5, 24))
+    gate, flat = torch.nn.Parameter(normal(g, (4, 24))), torch.nn.Parameter(normal(g, (24,)))
+    ready = []
+    arena = GradArena([gate, flat], on_ready=lambda s: ready.append(s.param))
+    arena.begin_step()
+    total = 0.0
+    for _ in range(2):
+        total = total + (F().residual_norm(x, y, gate=gate) * ds).sum() + (F().residual_norm(x, y, gate=flat) * ds).sum()
+    total.backward()
+    assert [sum(p is q for q in ready) for p in (gate, flat)] == [1, 1]
+    arena.finish_step()
+    for p in (gate, flat):
+        assert p.grad is p._dpa_sink.view and p._dpa_sink.uses == 0
+        value, bound = ref.residual_norm(x, y, None, p, None, None, ds)["d_gate"]
+        ref.within(p.grad, 2 * value, 2 * bound + 8 * ref.E32 * value.abs(), "gate")
+
+
 # ------------------------------------------------------------------------------------------ log probabilities
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [1e9, 1e30])
