@@ -176,6 +176,20 @@ struct Sink {
   float beta = 0.f;
   bool late = false;         // the gradient goes through deliver() after the kernel
 };
+// The sinks of one backward pass, which runs without the GIL: an allocation or a launch that throws ends their life there, and
+// only a holder of the GIL may drop what they refer to.
+struct Sinks : std::array<Sink, 5> {
+  Sinks() = default;
+  Sinks(const Sinks&) = delete;
+  Sinks& operator=(const Sinks&) = delete;
+  ~Sinks() {
+    bool held = false;
+    for (const Sink& s : *this) held = held || s.sink;
+    if (!held) return;
+    const py::gil_scoped_acquire gil;
+    for (Sink& s : *this) s.sink = py::object();
+  }
+};
 // needs the GIL
 void find_sink(const Tensor& param, Sink& out) {
   if (!param.is_leaf()) return;
@@ -247,7 +261,7 @@ struct ResidualNormBackward : Node {
 
     ResidualNormBwd p;
     Tensor own[5];
-    std::array<Sink, 5> sinks;
+    Sinks sinks;
     if (any_leaf) {
       const py::gil_scoped_acquire gil;
       for (int i = 0; i < 5; ++i) {

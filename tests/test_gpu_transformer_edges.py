@@ -196,6 +196,37 @@ def test_gate_of_samples_with_a_sink():
         ref.within(p.grad, 2 * value, 2 * bound + 8 * ref.E32 * value.abs(), "gate")
 
 
+def test_an_error_on_delivery_is_the_callers():
+    """Who is told of a finished gradient may raise (a collective that failed): the call to backward raises it, and the process
+    goes on."""
+    from distributed_pytorch_amd.parallel.distributed import GradArena
+
+    g = gen(3)
+    x, y = normal(g, (4, 5, 24)), normal(g, (4, 5, 24))
+    w, gate = torch.nn.Parameter(normal(g, (24,))), torch.nn.Parameter(normal(g, (4, 24)))
+    fail = [True]
+
+    def ready(sink):
+        if fail[0]:
+            raise ValueError("not delivered")
+
+    arena = GradArena([w, gate], on_ready=ready)
+
+    def step():
+        arena.begin_step()
+        s, h = F().residual_norm(x, y, gate=gate, pre=F().Norm(w, None, 1e-5, "rms"))
+        (s.sum() + h.sum()).backward()
+
+    for _ in range(3):
+        with pytest.raises(Exception, match="not delivered"):
+            step()
+        arena.end_step()
+    fail[0] = False
+    step()
+    arena.finish_step()
+    assert w.grad.isfinite().all() and gate.grad.isfinite().all()
+
+
 # ------------------------------------------------------------------------------------------ log probabilities
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [1e9, 1e30])
