@@ -453,8 +453,8 @@ OptTensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs
   if (!rotary_taken(qkv, positions, freqs, axis, heads)) return std::nullopt;
   const Tensor pos = positions.contiguous(), f = freqs.contiguous(), a = axis.to(at::kInt).contiguous();
   if (inplace) {
+    qkv.unsafeGetTensorImpl()->bump_version();      // (raises for an inference tensor outside inference mode)
     rotary_run(qkv, qkv, pos, f, a, heads, interleaved, false);
-    qkv.unsafeGetTensorImpl()->bump_version();
     return qkv;
   }
   if (!tracked({qkv})) return rotary_new(qkv, pos, f, a, heads, interleaved, false);

@@ -248,3 +248,19 @@ def test_token_logprobs_large_entropy_gradients_beside_masked_classes(size, dtyp
         assert not d.isnan().any()
     else:
         ref.within(d, value, bound, "d_logits")
+
+
+# ------------------------------------------------------------------------------------------ rotary
+def test_rotary_in_place_of_an_inference_tensor():
+    """Refused outside inference mode before anything is written, taken inside."""
+    with torch.inference_mode():
+        qkv = normal(gen(0), (1, 4, 48))
+        kept = qkv.clone()
+    pos = torch.arange(4, device="cuda")[:, None]
+    freqs, axis = torch.ones(8, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    with torch.no_grad(), pytest.raises(RuntimeError, match="[Ii]nference"):
+        F().rotary(qkv, pos, freqs, axis, 1, inplace=True)
+    with torch.inference_mode():
+        assert torch.equal(qkv, kept)
+        want = F().rotary(qkv, pos, freqs, axis, 1)
+        assert torch.equal(F().rotary(qkv, pos, freqs, axis, 1, inplace=True), want)
