@@ -92,7 +92,7 @@ class EncoderBlock(nn.Module):
         return F.add(x, self.mlp(self.ln_2(x)))
 
     def _attend(self, h, rotary=None):
-        y = self.self_attention(h, rotary)
+        y = self.self_attention(h) if rotary is None else self.self_attention(h, rotary)
         return self.dropout(y) if self.dropout.p else y
 
     def fused(self, x, h, next_norm, rotary=None):
@@ -102,13 +102,22 @@ class EncoderBlock(nn.Module):
         return F.residual_norm(x, self.mlp(h), pre=next_norm.spec())
 
 
+class EncoderLayers(nn.Sequential):
+    """The blocks one behind the other, each with the rotary positions where there are any."""
+
+    def forward(self, x, rotary=None):
+        for block in self:
+            x = block(x) if rotary is None else block(x, rotary)
+        return x
+
+
 class Encoder(nn.Module):
     def __init__(self, seq_length: int, num_layers: int, num_heads: int, hidden_dim: int, mlp_dim: int, dropout: float,
                  attention_dropout: float):
         super().__init__()
         self.pos_embedding = nn.Parameter(torch.empty(1, seq_length, hidden_dim).normal_(std=0.02))
         self.dropout = Dropout(dropout)
-        self.layers = nn.Sequential(OrderedDict(
+        self.layers = EncoderLayers(OrderedDict(
             ("encoder_layer_%d" % i, EncoderBlock(num_heads, hidden_dim, mlp_dim, dropout, attention_dropout))
             for i in range(num_layers)))
         self.ln = LayerNorm(hidden_dim, eps=1e-6)
@@ -122,9 +131,7 @@ class Encoder(nn.Module):
             for i, block in enumerate(self.layers):
                 x, h = block.fused(x, h, self.layers[i + 1].ln_1 if i + 1 < len(self.layers) else self.ln, rotary)
             return h
-        for block in self.layers:
-            x = block(x, rotary)
-        return self.ln(x)
+        return self.ln(self.layers(x) if rotary is None else self.layers(x, rotary))
 
 
 class VisionTransformer(_ImageNetCNN):

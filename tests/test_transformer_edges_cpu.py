@@ -3,6 +3,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from distributed_pytorch_amd import models
 from distributed_pytorch_amd.ops import functional as F
 
 
@@ -83,3 +84,45 @@ def test_newton_schulz_refuses_tangents():
         F.newton_schulz(torch.ones(3, 4))
         with pytest.raises(ValueError, match="no gradient"):
             F.newton_schulz(fwd.make_dual(torch.ones(3, 4), torch.ones(3, 4)))
+
+
+def _tiny_vit(rotary=False):
+    torch.manual_seed(0)
+    m = models.vit.VisionTransformer(32, 8, 2, 2, 32, 64, num_classes=5, rotary=rotary)
+    torch.nn.init.normal_(m.heads.head.weight)
+    return m
+
+
+class _Renamed(torch.nn.Module):
+    """A module in place of another that takes one argument, as checkpointing wrappers are."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x):
+        return self.inner(x)
+
+
+@pytest.mark.parametrize("rotary", [False, True])
+def test_hooks_of_the_encoder(rotary):
+    """Hooks on the sequence of blocks, the blocks, their norms and attention fire, with the activations alone as arguments
+    where there are no rotary positions."""
+    m, x, seen = _tiny_vit(rotary), torch.randn(2, 3, 32, 32), []
+    want = m(x)
+    block = m.encoder.layers[1]
+    for name, mod in (("layers", m.encoder.layers), ("block", block), ("ln_1", block.ln_1), ("attention", block.self_attention),
+                      ("ln_2", block.ln_2), ("ln", m.encoder.ln)):
+        mod.register_forward_hook(lambda mod, args, out, name=name: seen.append((name, len(args))))
+    assert torch.equal(m(x), want)
+    more = 2 if rotary else 1
+    assert sorted(seen) == sorted([("layers", more), ("block", more), ("ln_1", 1), ("attention", more), ("ln_2", 1), ("ln", 1)])
+    assert isinstance(m.encoder.layers, torch.nn.Sequential) and len(m.encoder.layers[:1]) == 1
+
+
+def test_blocks_that_take_the_activations_alone():
+    m, x = _tiny_vit(), torch.randn(2, 3, 32, 32)
+    want = m(x)
+    m.encoder.layers[0] = _Renamed(m.encoder.layers[0])
+    m.encoder.layers[1].self_attention = _Renamed(m.encoder.layers[1].self_attention)
+    assert torch.equal(m(x), want)
