@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ..nn.modules import AdaptiveAvgPool2d, Conv2d, GELU, LayerNorm, Linear, StochasticDepth
+from ..nn.modules import AdaptiveAvgPool2d, Conv2d, GELU, LayerNorm, Linear, StochasticDepth, can_bypass
 from ..ops import functional as F
 from .alexnet_vgg import _ImageNetCNN
 
@@ -51,9 +51,9 @@ class CNBlock(nn.Module):
         b = self.block
         h = b[5](b[4](b[3](b[2](b[0](x)))))
         n, c = h.shape[0], h.shape[-1]
-        if F.fuse_residual_norm():
-            return F.residual_norm(x, h, gate=self.layer_scale.reshape(c),
-                                   scale=F.stochastic_depth_scale(h, self.stochastic_depth.p, self.training))
+        drop = self.stochastic_depth
+        if F.fuse_residual_norm() and can_bypass((StochasticDepth,), drop):
+            return F.residual_norm(x, h, gate=self.layer_scale.reshape(c), scale=F.stochastic_depth_scale(h, drop.p, drop.training))
         h = F.se_scale(h, self.layer_scale.reshape(1, c).float().expand(n, c))      # per-channel layer scale
         return F.add(self.stochastic_depth(h), x)
 

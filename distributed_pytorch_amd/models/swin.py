@@ -26,7 +26,7 @@ from typing import Dict, List, Optional
 import torch
 from torch import nn
 
-from ..nn.modules import GELU, Conv2d, Dropout, LayerNorm, Linear, ReLU, StochasticDepth
+from ..nn.modules import GELU, Conv2d, Dropout, LayerNorm, Linear, ReLU, RMSNorm, StochasticDepth, can_bypass
 from ..ops import functional as F
 from .alexnet_vgg import _ImageNetCNN
 
@@ -217,7 +217,8 @@ class SwinTransformerBlock(nn.Module):
 
     def _fused(self, x):
         """The residual sums with their norms and stochastic depth as ``F.residual_norm``."""
-        sd = lambda: F.stochastic_depth_scale(x, self.stochastic_depth.p, self.training)      # noqa: E731
+        drop = self.stochastic_depth
+        sd = lambda: F.stochastic_depth_scale(x, drop.p, drop.training)      # noqa: E731
         if self.v2:
             x = F.residual_norm(x, self.attn(x), post=self.norm1.spec(), scale=sd())
             return F.residual_norm(x, self.mlp(x), post=self.norm2.spec(), scale=sd())
@@ -225,7 +226,7 @@ class SwinTransformerBlock(nn.Module):
         return F.residual_norm(x, self.mlp(h), scale=sd())
 
     def forward(self, x):
-        if F.fuse_residual_norm():
+        if F.fuse_residual_norm() and can_bypass((LayerNorm, RMSNorm, StochasticDepth), self.norm1, self.norm2, self.stochastic_depth):
             return self._fused(x)
         if self.v2:
             x = F.add(x, self.stochastic_depth(self.norm1(self.attn(x))))

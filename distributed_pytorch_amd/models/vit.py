@@ -20,7 +20,7 @@ from collections import OrderedDict
 import torch
 from torch import nn
 
-from ..nn.modules import GELU, AxialRotary, Conv2d, Dropout, LayerNorm, Linear
+from ..nn.modules import GELU, AxialRotary, Conv2d, Dropout, LayerNorm, Linear, RMSNorm, can_bypass
 from ..ops import functional as F
 from .alexnet_vgg import _ImageNetCNN
 
@@ -122,11 +122,17 @@ class Encoder(nn.Module):
             for i in range(num_layers)))
         self.ln = LayerNorm(hidden_dim, eps=1e-6)
 
+    def _can_fuse(self) -> bool:
+        blocks = list(self.layers)
+        if not blocks or not can_bypass((EncoderLayers, EncoderBlock), self.layers, *blocks):
+            return False
+        return can_bypass((LayerNorm, RMSNorm), *(n for b in blocks for n in (b.ln_1, b.ln_2)), self.ln)
+
     def forward(self, x, rotary=None):
         x = x + self.pos_embedding.to(x.dtype)
         if self.dropout.p:
             x = self.dropout(x)
-        if F.fuse_residual_norm():
+        if F.fuse_residual_norm() and self._can_fuse():
             h = self.layers[0].ln_1(x)
             for i, block in enumerate(self.layers):
                 x, h = block.fused(x, h, self.layers[i + 1].ln_1 if i + 1 < len(self.layers) else self.ln, rotary)

@@ -239,6 +239,19 @@ class StochasticDepth(nn.Module):
         return F.stochastic_depth(x, self.p, self.training)
 
 
+def can_bypass(kinds, *modules) -> bool:
+    """Whether a fused pass may stand in for the calls of these modules: each is one of ``kinds``, nobody replaced its
+    ``forward``, and no hook waits for the call."""
+    if nn.modules.module._has_any_global_hook():
+        return False
+    for m in modules:
+        if "forward" in m.__dict__ or not any(isinstance(m, k) and type(m).forward is k.forward for k in kinds):
+            return False
+        if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
+            return False
+    return True
+
+
 class SqueezeExcitation(nn.Module):
     """torchvision ``SqueezeExcitation``: ``x * gate(fc2(act(fc1(mean_hw(x)))))`` with 1x1-conv shaped parameters
     (``fc1.weight [S, C, 1, 1]`` ...) so checkpoints interchange.

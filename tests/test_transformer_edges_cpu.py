@@ -126,3 +126,83 @@ def test_blocks_that_take_the_activations_alone():
     m.encoder.layers[0] = _Renamed(m.encoder.layers[0])
     m.encoder.layers[1].self_attention = _Renamed(m.encoder.layers[1].self_attention)
     assert torch.equal(m(x), want)
+
+
+def _block_of(arch, **kw):
+    """(model, input, a block of it, what the fused pass of that block stands in for)"""
+    from distributed_pytorch_amd.models import convnext, swin
+
+    torch.manual_seed(0)
+    if arch == "vit":
+        m = _tiny_vit()
+        b = m.encoder.layers[0]
+        return m, torch.randn(2, 3, 32, 32), [m.encoder.layers, b, b.ln_1, b.ln_2, m.encoder.ln]
+    if arch == "convnext":
+        b = convnext.CNBlock(16, 0.5, 0.5)
+        return b, torch.randn(2, 8, 8, 16), [b.stochastic_depth]
+    kind = swin.SwinTransformerBlock if arch == "swin" else swin.SwinTransformerBlockV2
+    b = kind(32, 2, [4, 4], [0, 0], stochastic_depth_prob=0.5)
+    return b, torch.randn(2, 8, 8, 32), [b.norm1, b.norm2, b.stochastic_depth]
+
+
+@pytest.mark.parametrize("arch", ["vit", "swin", "swin_v2", "convnext"])
+def test_fused_passes_step_aside_for_hooks(arch, monkeypatch):
+    """A hook on anything that the fused pass would stand in for is called, and may change what its module returns."""
+    monkeypatch.setattr(F, "_FUSE_RESIDUAL_NORM", True)
+    m, x, inside = _block_of(arch)
+    m.train()
+    for mod in inside:
+        seen = []
+        for hook in (mod.register_forward_hook(lambda *a: seen.append(0)), mod.register_forward_pre_hook(lambda *a: seen.append(0)),
+                     mod.register_full_backward_hook(lambda *a: seen.append(0))):
+            del seen[:]
+            m(x.clone().requires_grad_()).sum().backward()
+            assert seen, (mod, hook)
+            hook.remove()
+    seen = []
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda mod, *a: seen.append(mod))
+    try:
+        m(x)
+    finally:
+        hook.remove()
+    assert all(any(mod is s for s in seen) for mod in inside)
+
+
+@pytest.mark.parametrize("arch", ["vit", "swin", "swin_v2", "convnext"])
+def test_fused_passes_step_aside_for_other_modules(arch, monkeypatch):
+    """A norm or stochastic depth that is another module, or whose forward was replaced, is the one that runs."""
+    monkeypatch.setattr(F, "_FUSE_RESIDUAL_NORM", True)
+    m, x, inside = _block_of(arch)
+    m.eval()
+    mod = inside[-1]                     # the last norm, or stochastic depth
+    mod.forward = lambda v: torch.zeros_like(v)
+    out = m(x)
+    if arch == "vit":
+        assert torch.equal(out, m.heads.head.bias.expand_as(out))
+    else:
+        monkeypatch.setattr(F, "_FUSE_RESIDUAL_NORM", False)
+        assert torch.equal(m(x), out)
+    del mod.forward
+    if arch == "vit":
+        m.encoder.layers[0] = _Renamed(m.encoder.layers[0])
+        m(x)
+
+
+@pytest.mark.parametrize("arch", ["swin", "swin_v2", "convnext"])
+def test_fused_stochastic_depth_follows_its_own_mode(arch, monkeypatch):
+    """Stochastic depth in evaluation mode inside a block that trains drops nothing."""
+    m, x, inside = _block_of(arch)
+    m.train()
+    inside[-1].eval()
+    got = []
+    for fused in (False, True):
+        monkeypatch.setattr(F, "_FUSE_RESIDUAL_NORM", fused)
+        got.append(m(x))
+    # 32 bits either way, additions in another order: 2^-24 each, some hundreds deep at most
+    assert float((got[0] - got[1]).abs().max()) <= 1e-4 * float(got[0].abs().max())
+
+
+def test_fused_encoder_without_blocks(monkeypatch):
+    monkeypatch.setattr(F, "_FUSE_RESIDUAL_NORM", True)
+    m = models.vit.VisionTransformer(32, 8, 0, 2, 32, 64, num_classes=5)
+    assert m(torch.randn(1, 3, 32, 32)).shape == (1, 5)
