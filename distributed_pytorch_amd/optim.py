@@ -248,10 +248,10 @@ class FusedMuon(FusedSGD):
         if groups and not isinstance(groups[0], dict):
             groups = [g for g in (dict(params=[p for p in groups if p.dim() == 2], orthogonal=True),
                                   dict(params=[p for p in groups if p.dim() != 2], orthogonal=False)) if g["params"]]
+        self._nesterov = bool(nesterov)              # (add_param_group, which the base constructor calls, reads it)
         super().__init__(groups, lr=lr, momentum=momentum, weight_decay=weight_decay)
         self._matrix_defaults = dict(orthogonal=False, matrix_scale=float(matrix_scale), ns_steps=int(ns_steps),
                                      ns_coefficients=tuple(float(v) for v in ns_coefficients), ns_eps=float(ns_eps))
-        self._nesterov = bool(nesterov)
         self._muon = None
         self._fill_groups()
 
@@ -269,13 +269,14 @@ class FusedMuon(FusedSGD):
                 raise ValueError("ns_steps must be at least 1 and ns_eps positive")
             _check_schulz(tuple(float(v) for v in group["ns_coefficients"]), int(group["ns_steps"]))
             if group["orthogonal"]:
-                group["nesterov"] = self._nesterov
                 if group["dampening"] != 0:
                     raise ValueError("FusedMuon: no dampening in an orthogonal group")
                 if any(p.dim() < 2 for p in group["params"]):
                     raise ValueError("FusedMuon: an orthogonal group holds matrices (2 or more dimensions)")
 
     def add_param_group(self, group) -> None:
+        if isinstance(group, dict) and group.get("orthogonal"):
+            group.setdefault("nesterov", self._nesterov)
         super().add_param_group(group)
         if hasattr(self, "_matrix_defaults"):        # (the base constructor adds its groups through here)
             self._fill_groups()

@@ -206,3 +206,46 @@ def test_fused_encoder_without_blocks(monkeypatch):
     monkeypatch.setattr(F, "_FUSE_RESIDUAL_NORM", True)
     m = models.vit.VisionTransformer(32, 8, 0, 2, 32, 64, num_classes=5)
     assert m(torch.randn(1, 3, 32, 32)).shape == (1, 5)
+
+
+# ------------------------------------------------------------------------------------------ FusedMuon
+def _matrices(seed):
+    g = torch.Generator().manual_seed(seed)
+    ps = [torch.nn.Parameter(torch.randn(6, 10, generator=g)), torch.nn.Parameter(torch.randn(7, generator=g))]
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=g)
+    return ps
+
+
+def test_muon_nesterov_of_a_group():
+    """A group's own choice stands; the constructor's is for groups without one."""
+    from distributed_pytorch_amd.optim import FusedMuon
+
+    a, b = _matrices(0), _matrices(1)
+    for of_all in (True, False):
+        opt = FusedMuon([dict(params=a[:1], orthogonal=True, nesterov=not of_all), dict(params=b[:1], orthogonal=True),
+                         dict(params=a[1:])], nesterov=of_all)
+        assert [g["nesterov"] for g in opt.param_groups] == [not of_all, of_all, False]
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(3, 4))], orthogonal=True))
+        assert opt.param_groups[-1]["nesterov"] is of_all
+
+
+@pytest.mark.parametrize("saved", [True, False])
+def test_muon_resumes_with_the_checkpoints_nesterov(saved):
+    """Whatever the new optimizer was built with: the steps after a resume are those of the run that was saved."""
+    import copy
+
+    from distributed_pytorch_amd.optim import FusedMuon
+
+    a, b = _matrices(2), _matrices(2)
+    x, y = FusedMuon(a, lr=0.1, nesterov=saved), FusedMuon(b, lr=0.1, nesterov=not saved)
+    x.step()
+    y.load_state_dict(copy.deepcopy(x.state_dict()))
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    for _ in range(2):
+        x.step()
+        y.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
