@@ -3219,9 +3219,7 @@ class SgdPlan:
         chunk = C().sgd_chunk_elems()
         self.groups = []
         self.params_with_copies = []
-        for group in opt.param_groups:
-            if group.get("orthogonal"):         # updated by transformer_ops.MuonPlan
-                continue
+        for group in opt.sgd_groups():
             entries, keep, plist, nchunks = [], [], [], 0
             g_dtype = lp_dtype = None
             device = None

@@ -137,12 +137,16 @@ class FusedSGD(Optimizer):
             st["momentum_buffer"] = buf
         return buf
 
+    def sgd_groups(self) -> list:
+        """The groups that SGD updates."""
+        return self.param_groups
+
     def _step_reference(self, scaler) -> None:
         skip = scaler is not None and float(scaler.found_inf.item()) > 0
         if skip:
             return
         inv = None if scaler is None else scaler.inv_scale
-        for group in self.param_groups:
+        for group in self.sgd_groups():
             lr, mu, wd = group["lr"], group["momentum"], group["weight_decay"]
             damp, nesterov = group["dampening"], group["nesterov"]
             for p in group["params"]:
@@ -282,21 +286,19 @@ class FusedMuon(FusedSGD):
             self._fill_groups()
             self._plan = self._muon = None
 
+    def sgd_groups(self) -> list:
+        return [g for g in self.param_groups if not g["orthogonal"]]
+
     def _step_reference(self, scaler) -> None:
         from .ops import functional as F
 
         if scaler is not None and float(scaler.found_inf.item()) > 0:
             return
-        plain, mine = [], []
-        for g in self.param_groups:
-            (mine if g["orthogonal"] else plain).append(g)
-        every, self.param_groups = self.param_groups, plain
-        try:
-            super()._step_reference(scaler)
-        finally:
-            self.param_groups = every
+        super()._step_reference(scaler)
         inv = None if scaler is None else scaler.inv_scale
-        for group in mine:
+        for group in self.param_groups:
+            if not group["orthogonal"]:
+                continue
             lr, mu = group["lr"], group["momentum"]
             for p in group["params"]:
                 if p.grad is None:
@@ -336,6 +338,10 @@ class FusedMuon(FusedSGD):
             self._muon.sync_hyper(self)
 
     def load_state_dict(self, state_dict) -> None:
+        own = [{k: g[k] for k in ("nesterov", *self._matrix_defaults)} for g in self.param_groups]
         super().load_state_dict(state_dict)
+        for group, saved, mine in zip(self.param_groups, state_dict["param_groups"], own):
+            if "orthogonal" not in saved:            # SGD's: it has the momentum, which matrices take as it is, and no say in the rest
+                group.update(mine)
         self._muon = None
         self._fill_groups()

@@ -264,3 +264,34 @@ def test_rotary_in_place_of_an_inference_tensor():
         assert torch.equal(qkv, kept)
         want = F().rotary(qkv, pos, freqs, axis, 1)
         assert torch.equal(F().rotary(qkv, pos, freqs, axis, 1, inplace=True), want)
+
+
+# ------------------------------------------------------------------------------------------ FusedMuon
+def test_sgd_with_the_groups_of_a_muon_checkpoint():
+    """FusedSGD updates every parameter, also in groups that a checkpoint of FusedMuon marks as matrices; FusedMuon takes the
+    momentum of an SGD checkpoint and goes on with its matrices."""
+    import copy
+
+    from distributed_pytorch_amd.optim import FusedMuon, FusedSGD
+
+    def params():
+        ps = [torch.nn.Parameter(normal(gen(1), (24, 40)))]
+        ps[0].grad = normal(gen(2), (24, 40))
+        return ps
+
+    a, b, c = params(), params(), params()
+    muon = FusedMuon([dict(params=a, orthogonal=True)], lr=0.1, momentum=0.9)
+    muon.step()
+    sgd = FusedSGD(b, lr=0.1, momentum=0.9)
+    sgd.load_state_dict(copy.deepcopy(muon.state_dict()))
+    before, grad, buf = b[0].detach().clone(), b[0].grad.clone(), sgd.state[b[0]]["momentum_buffer"].clone()
+    sgd.step()
+    buf = 0.9 * buf + grad
+    step = grad + 0.9 * buf if sgd.param_groups[0]["nesterov"] else buf
+    assert torch.allclose(b[0], before - 0.1 * step, rtol=0, atol=1e-5)
+    again = FusedMuon([dict(params=c, orthogonal=True)], lr=0.1, momentum=0.9)
+    again.load_state_dict(copy.deepcopy(FusedSGD(params(), lr=0.1, momentum=0.9).state_dict()))
+    before = c[0].detach().clone()
+    again.step()
+    assert again.param_groups[0]["orthogonal"] is True and 0.0 < float((c[0] - before).norm()) < 0.1 * 0.2 * 1.3 * 24 ** 0.5
+

@@ -249,3 +249,30 @@ def test_muon_resumes_with_the_checkpoints_nesterov(saved):
         y.step()
     for p, q in zip(a, b):
         assert torch.equal(p, q)
+
+
+def test_muon_from_a_checkpoint_of_sgd_and_back():
+    """The momentum goes over; which groups are orthogonalised stays the optimizer's own, and SGD updates every group."""
+    import copy
+
+    from distributed_pytorch_amd.optim import FusedMuon, FusedSGD
+
+    a, b, c, d = (_matrices(4) for _ in range(4))
+    sgd, muon = FusedSGD(a[:1], lr=0.1, momentum=0.9), FusedMuon([dict(params=b[:1], orthogonal=True)], lr=0.2, matrix_scale=0.5)
+    sgd.step()
+    muon.load_state_dict(copy.deepcopy(sgd.state_dict()))
+    group = muon.param_groups[0]
+    assert group["orthogonal"] is True and group["nesterov"] is True and group["matrix_scale"] == 0.5 and group["lr"] == 0.1
+    with torch.no_grad():
+        b[0].copy_(c[0])
+    muon.step()
+    buf = 0.9 * a[0].grad + a[0].grad
+    want = c[0] - 0.1 * 0.5 * F.newton_schulz((a[0].grad + 0.9 * buf).detach())
+    assert torch.allclose(b[0], want, rtol=0, atol=1e-5)
+
+    back = FusedSGD(d[:1], lr=0.1, momentum=0.9)
+    back.load_state_dict(copy.deepcopy(muon.state_dict()))
+    before = d[0].detach().clone()
+    assert back.sgd_groups() == back.param_groups and len(back.param_groups) == 1
+    back.step()
+    assert not torch.equal(before, d[0])
