@@ -228,6 +228,70 @@ def test_an_error_on_delivery_is_the_callers():
 
 
 # ------------------------------------------------------------------------------------------ log probabilities
+# rows that select 64, 128 and 256 lanes a row where rows are long
+ROWS = [520, 2100, 4200]
+
+
+def _lanes(rows):
+    return 64 if rows >= 4096 else 128 if rows >= 2048 else 256
+
+
+def _check_rows(z, t, k, rows, seed=0):
+    """Every row's results and gradients are computed, `rows` of them are compared."""
+    g = gen(seed)
+    N = z.shape[0]
+    d_lp, d_ent, d_top = normal(g, (N,)), normal(g, (N,)), normal(g, (N, k))
+    z = z.detach().requires_grad_()
+    out = F().token_logprobs(z, t, k)
+    (d,) = torch.autograd.grad(out[:3], [z], [d_lp, d_ent, d_top])
+    at = torch.tensor(rows, device="cuda")
+    want = ref.token_logprobs(z[at], t[at], k, d_lp[at], d_ent[at], d_top[at])
+    assert torch.equal(out[3][at].cpu(), want["index"][0]), "indices"
+    # (the reference's bounds count V / 256 additions in a row for a lane; fewer lanes add more of them)
+    V = z.shape[1]
+    more = (V / _lanes(N) + 24) / (V / 256 + 24)
+    for name, got in zip(("logprob", "entropy", "top"), out):
+        ref.within(got[at], want[name][0], more * want[name][1], name)
+    value, bound = want["d_logits"]
+    rounding = ref.U[z.dtype] * value.abs()
+    ref.within(d[at], value, rounding + more * (bound - rounding), "d_logits")
+
+
+@pytest.mark.parametrize("N", ROWS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("few,k", [(1, 40), (12, 64), (64, 64)])
+def test_token_logprobs_crowded_lanes_of_every_workgroup(few, k, dtype, N):
+    """Long rows whose largest values lie in the chunks of a few lanes, several chunks each, for each size of workgroup."""
+    V, g = 9001, gen(few)
+    lanes, step = _lanes(N), 16 // (torch.finfo(dtype).bits // 8)
+    assert -(-V // step) > 256
+    lane = torch.arange(V, device="cuda") // step % lanes
+    z = normal(g, (N, V))
+    crowd = (lane >= 5) & (lane < 5 + few)
+    z[1] += torch.where(crowd, 9.0, 0.0)
+    z[N - 1] += torch.where(crowd, 3.0, 0.0)
+    z[N // 2] = torch.where(crowd, 2.0, 0.0)                  # equal values alone: more than the list holds
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    _check_rows(z.to(dtype), t, k, [0, 1, N // 2, N - 1])
+
+
+@pytest.mark.parametrize("N", ROWS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_token_logprobs_ties_and_masks_of_every_workgroup(dtype, N):
+    V, k, g = 9001, 64, gen(N)
+    base = torch.arange(V, device="cuda")
+    z = normal(g, (N, V), dtype, 2.0)
+    z[0] = 0.0                                                # every class the same: looked at again and again
+    z[1] = (base % 3).to(dtype)
+    z[2] = (base / V).to(dtype)
+    z[3] = (-base / V).to(dtype)
+    z[4] = torch.finfo(dtype).min
+    z[5, 70:] = -math.inf
+    z[6, ::2] = -math.inf
+    t = torch.randint(0, 64, (N,), generator=g, device="cuda") | 1
+    _check_rows(z, t, k, [0, 1, 2, 3, 4, 5, 6, 7, N - 1])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [1e9, 1e30])
 def test_token_logprobs_large_entropy_gradients_beside_masked_classes(size, dtype):
