@@ -4,7 +4,7 @@
 hipcc (cross-compiles without a GPU), the C++ runtime / bindings, and links two pybind11 modules that
 sit next to the package so they travel to the GPU box with the tree: ``_C``, and ``_T`` (``csrc/transformer``:
 operators with autograd nodes in C++, the only part built against torch's headers).  Objects are cached under
-``build/`` and rebuilt only when a source (or a header that it includes) is newer.
+``build/`` and rebuilt only when a source (or a header that it includes) is newer or the command that makes them changed.
 """
 from __future__ import annotations
 
@@ -64,6 +64,26 @@ def _torch_flags():
     return ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"] + inc, libs
 
 
+def _stale(out: str, stamp: str, cmd, newest: float) -> bool:
+    """Whether ``out`` has to be made again: it is not there, older than what it is made of, or made by another command."""
+    if not os.path.exists(out) or os.path.getmtime(out) < newest or not os.path.exists(stamp):
+        return True
+    with open(stamp) as f:
+        return f.read() != " ".join(cmd)
+
+
+def _make(out: str, stamp: str, cmd, verbose: bool, what: str) -> None:
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    if os.path.exists(stamp):
+        os.remove(stamp)                  # (what an interrupted command leaves is made again)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("%s\n%s" % (what, r.stderr[-4000:]))
+    with open(stamp, "w") as f:
+        f.write(" ".join(cmd))
+
+
 def build(verbose: bool = False, force: bool = False, jobs: int = 0) -> str:
     import pybind11
 
@@ -81,34 +101,24 @@ def build(verbose: bool = False, force: bool = False, jobs: int = 0) -> str:
         for src in sources:
             obj = os.path.join(objdir, os.path.relpath(src, CSRC).replace(os.sep, "_") + ".o")
             objs[module].append(obj)
-            if force or not os.path.exists(obj) or os.path.getmtime(obj) < _mtime_with_headers(src):
-                todo.append((module, src, obj))
+            cmd = (host if module == "_T" and src.endswith(".cpp") else common) + ["-c", src, "-o", obj]
+            if force or _stale(obj, obj + ".cmd", cmd, _mtime_with_headers(src)):
+                todo.append((src, obj, cmd))
 
     def compile_one(job):
-        module, src, obj = job
-        cmd = (host if module == "_T" and src.endswith(".cpp") else common) + ["-c", src, "-o", obj]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("compile failed: %s\n%s" % (src, r.stderr[-4000:]))
-        return obj
+        src, obj, cmd = job
+        _make(obj, obj + ".cmd", cmd, verbose, "compile failed: " + src)
 
     jobs = jobs or min(8, int(os.environ.get("MAX_JOBS", "8")), max(1, len(todo)))
     if todo:
         with ThreadPoolExecutor(max_workers=jobs) as ex:
             list(ex.map(compile_one, todo))
-    changed = {module for module, _, _ in todo}
     for module, files in objs.items():
-        tgt = target_path(module)
-        if module in changed or not os.path.exists(tgt):
-            # no rpath: at run time libamdhip64.so.7 (and torch's libraries) resolve to the copies torch loaded first
-            cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", tgt] + files + ["-ldl"] + (torch_ld if module == "_T" else [])
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            r = subprocess.run(cmd, capture_output=True, text=True)
-            if r.returncode != 0:
-                raise RuntimeError("link failed:\n%s" % r.stderr[-4000:])
+        tgt, stamp = target_path(module), os.path.join(objdir, module + ".cmd")
+        # no rpath: at run time libamdhip64.so.7 (and torch's libraries) resolve to the copies torch loaded first
+        cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", tgt] + files + ["-ldl"] + (torch_ld if module == "_T" else [])
+        if _stale(tgt, stamp, cmd, max(os.path.getmtime(f) for f in files)):
+            _make(tgt, stamp, cmd, verbose, "link failed:")
     return target_path()
 
 
