@@ -121,6 +121,20 @@ template <typename N, typename... Inputs> std::shared_ptr<N> make_node(const Inp
   node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
   return node;
 }
+// A saved value comes back through the hooks that were set when it was saved (torch.autograd.graph.saved_tensors_hooks), which
+// may return anything: what a kernel would read past the end of is refused.
+void check_kept(const char* op, const Tensor& t, at::ScalarType type, at::IntArrayRef size, const at::Device& device) {
+  TORCH_CHECK(t.defined() && is_plain(t) && t.scalar_type() == type && t.sizes() == size && t.device() == device, op,
+              ": a saved tensor came back with another type, shape or device");
+}
+Tensor kept(const char* op, const Tensor& t, at::ScalarType type, at::IntArrayRef size, const at::Device& device) {
+  check_kept(op, t, type, size, device);
+  return t.contiguous();
+}
+// gradients of subclasses and wrappers have no memory to read either
+template <typename... Ts> void check_grads(const char* op, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED((is_plain(ts) && ...), op, ": gradients that are tensor subclasses or wrappers are not supported");
+}
 SavedVariable saved(const Tensor& t, bool is_output = false) { return t.defined() ? SavedVariable(t, is_output) : SavedVariable(); }
 void has_history(const Tensor& t, const std::shared_ptr<Node>& node) {
   if (t.defined()) torch::autograd::set_history(t, node);
@@ -225,16 +239,31 @@ struct ResidualNormBackward : Node {
   variable_list apply(variable_list&& grads) override {
     once("residual_norm");
     const std::lock_guard<std::mutex> lock(mutex_);
-    const std::array<Tensor, 10> sv{x_.unpack(), y_.unpack(), post_stat_.unpack(), pre_stat_.unpack(), post_w_.unpack(),
+    std::array<Tensor, 10> sv{x_.unpack(), y_.unpack(), post_stat_.unpack(), pre_stat_.unpack(), post_w_.unpack(),
                                     post_b_.unpack(), pre_w_.unpack(), pre_b_.unpack(), gate_.unpack(), scale_.unpack()};
     const int64_t cfg[4] = {post, pre, has_y, may_sink};
     variable_list got(7);
     Tensor ds = has_y ? grads[0] : Tensor(), dh = has_y ? (grads.size() > 1 ? grads[1] : Tensor()) : grads[0];
     if (!ds.defined() && !dh.defined()) return got;
+    check_grads("residual_norm", ds, dh);
     ds = dense(ds);
     dh = dense(dh);
     const Tensor& ref = ds.defined() ? ds : dh;
     const c10::DeviceGuard guard(ref.device());
+    {
+      const int64_t C = ref.size(-1), stat[2] = {2, ref.numel() / C};
+      for (int i = 0; i < 2; ++i)
+        if (sv[i].defined()) sv[i] = kept("residual_norm", sv[i], ref.scalar_type(), ref.sizes(), ref.device());
+      for (int i = 2; i < 4; ++i)
+        if (sv[i].defined()) sv[i] = kept("residual_norm", sv[i], at::kFloat, stat, ref.device());
+      const int64_t gate[2] = {ref.size(0), C};
+      for (int i = 4; i < 9; ++i) {                 // (vectors of any type, converted below; leaves stay themselves for their sinks)
+        if (!sv[i].defined()) continue;
+        const bool of_samples = i == 8 && sv[i].dim() == 2;
+        check_kept("residual_norm", sv[i], sv[i].scalar_type(), of_samples ? at::IntArrayRef(gate) : at::IntArrayRef(C), ref.device());
+      }
+      if (sv[9].defined()) sv[9] = kept("residual_norm", sv[9], at::kFloat, ref.size(0), ref.device());
+    }
     const Tensor &x = sv[0], &y = sv[1];
     // the caller's parameters in the order of the kernel's sums, and where their gradients go
     const std::array<Tensor, 5> params{sv[6], sv[7], sv[4], sv[5], sv[8]};
@@ -414,8 +443,10 @@ Tensor rotary_new(const Tensor& t, const Tensor& pos, const Tensor& freqs, const
 
 struct RotaryBackward : Node {
   SavedVariable pos_, freqs_, axis_;
-  int64_t heads = 0;
+  int64_t heads = 0, pairs = 0;
   bool interleaved = false;
+  at::ScalarType pos_type = at::kLong, freqs_type = at::kDouble;
+  c10::SmallVector<int64_t, 3> pos_size;
 
   std::string name() const override { return "RotaryBackward"; }
   void release_variables() override {
@@ -426,8 +457,13 @@ struct RotaryBackward : Node {
     once("rotary");
     const std::lock_guard<std::mutex> lock(mutex_);
     variable_list got(1);
-    const Tensor pos = pos_.unpack(), freqs = freqs_.unpack(), axis = axis_.unpack();
-    if (grads[0].defined()) got[0] = rotary_new(grads[0], pos, freqs, axis, heads, interleaved, true);
+    if (!grads[0].defined()) return got;
+    check_grads("rotary", grads[0]);
+    Tensor pos = pos_.unpack(), freqs = freqs_.unpack(), axis = axis_.unpack();
+    pos = kept("rotary", pos, pos_type, pos_size, grads[0].device());
+    freqs = kept("rotary", freqs, freqs_type, pairs, grads[0].device());
+    axis = kept("rotary", axis, at::kInt, pairs, grads[0].device());
+    got[0] = rotary_new(grads[0], pos, freqs, axis, heads, interleaved, true);
     return got;
   }
 };
@@ -468,6 +504,10 @@ OptTensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs
     node->axis_ = saved(a);
     node->heads = heads;
     node->interleaved = interleaved;
+    node->pairs = f.numel();
+    node->pos_type = pos.scalar_type();
+    node->freqs_type = f.scalar_type();
+    node->pos_size.assign(pos.sizes().begin(), pos.sizes().end());
   }
   has_history(out, node);
   return out;
@@ -499,7 +539,9 @@ LpOut lp_forward(const Tensor& z, const Tensor& t, int64_t k) {
 
 struct TokenLogprobsBackward : Node {
   SavedVariable logits_, target_, norm_, entropy_, index_;
-  int64_t k = 0;
+  int64_t k = 0, rows = 0, classes = 0;
+  at::ScalarType type = at::kFloat;
+  at::Device device = at::kCPU;
 
   std::string name() const override { return "TokenLogprobsBackward"; }
   void release_variables() override {
@@ -510,7 +552,7 @@ struct TokenLogprobsBackward : Node {
     once("token_logprobs");
     const std::lock_guard<std::mutex> lock(mutex_);
     variable_list got(1);
-    const std::array<Tensor, 5> sv{logits_.unpack(), target_.unpack(), norm_.unpack(), entropy_.unpack(shared_from_this()),
+    std::array<Tensor, 5> sv{logits_.unpack(), target_.unpack(), norm_.unpack(), entropy_.unpack(shared_from_this()),
                                    index_.unpack()};
     Tensor g[3];
     bool any = false;
@@ -519,8 +561,15 @@ struct TokenLogprobsBackward : Node {
       any = any || g[i].defined();
     }
     if (!any) return got;
+    check_grads("token_logprobs", grads[0], grads[1], grads[2]);
+    const c10::DeviceGuard guard(device);
+    check_kept("token_logprobs", sv[0], type, {rows, classes}, device);
+    if (sv[0].stride(1) != 1) sv[0] = sv[0].contiguous();
+    sv[1] = kept("token_logprobs", sv[1], at::kLong, rows, device);
+    sv[2] = kept("token_logprobs", sv[2], at::kFloat, {rows, 2}, device);
+    sv[3] = kept("token_logprobs", sv[3], at::kFloat, rows, device);
+    sv[4] = kept("token_logprobs", sv[4], at::kLong, {rows, k}, device);
     const Tensor& z = sv[0];
-    const c10::DeviceGuard guard(z.device());
     const Tensor dz = at::empty(z.sizes(), z.options());
     TokenLogprobsBwd p;
     p.logits = z.data_ptr(); p.target = sv[1].data_ptr<int64_t>(); p.norm = sv[2].data_ptr<float>();
@@ -558,6 +607,10 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const T
     node->norm_ = saved(o.norm);
     node->index_ = saved(o.idx);
     node->k = k;
+    node->rows = z.size(0);
+    node->classes = z.size(1);
+    node->type = z.scalar_type();
+    node->device = z.device();
   }
   for (const Tensor& out : {o.lp, o.ent, o.top}) has_history(out, node);
   node->entropy_ = saved(o.ent, true);

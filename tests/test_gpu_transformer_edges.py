@@ -155,6 +155,70 @@ def test_modes_that_watch_are_welcome():
         assert torch.equal(F().rms_norm(x, w), want)
 
 
+# ------------------------------------------------------------------------------------------ saved tensors
+def _with_gradients(seed=0):
+    """[(results, leaves, gradients)] of every operator that has a backward pass."""
+    g = gen(seed)
+    leaf = lambda *shape, dtype=torch.float32: normal(g, shape, dtype).requires_grad_()                        # noqa: E731
+    x, y, w, b, v, gate = leaf(3, 5, 24), leaf(3, 5, 24), leaf(24), leaf(24), leaf(24), leaf(3, 24)
+    scale = torch.tensor([0.0, 1.0, 2.0], device="cuda")
+    s, h = F().residual_norm(x, y, post=F().Norm(w, b, 1e-5, "layer"), gate=gate, scale=scale, pre=F().Norm(v, None, 1e-5, "rms"))
+    qkv, z = leaf(2, 4, 48, dtype=torch.bfloat16), leaf(3, 20)
+    wide = normal(g, (3, 30)).requires_grad_()
+    pos = torch.arange(8, device="cuda").view(2, 4, 1)
+    r = F().rotary(qkv, pos, torch.ones(8, device="cuda"), torch.zeros(8, dtype=torch.int64, device="cuda"), 1)
+    t = torch.tensor([1, 5, -1], device="cuda")
+    lp = F().token_logprobs(z, t, 4)[:3] + F().token_logprobs(wide[:, 3:23], t, 4)[:3]
+    return [([s, h], [x, y, w, b, v, gate], None), ([r], [qkv], None), (list(lp), [z, wide], None)]
+
+
+def _gradients(cases):
+    return [torch.autograd.grad(outs, leaves, [torch.ones_like(o) for o in outs]) for outs, leaves, _ in cases]
+
+
+def test_saved_tensors_may_go_elsewhere_and_come_back():
+    want = _gradients(_with_gradients())
+    with torch.autograd.graph.save_on_cpu():
+        cases = _with_gradients()
+    for a, b in zip(_gradients(cases), want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_recomputed_calls_give_the_same_gradients():
+    from torch.utils.checkpoint import checkpoint
+
+    x, y, w = (normal(gen(i), s).requires_grad_() for i, s in enumerate([(3, 5, 24), (3, 5, 24), (24,)]))
+    call = lambda x, y, w: F().residual_norm(x, y * 2.0, pre=F().Norm(w, None, 1e-5, "rms"))[1]              # noqa: E731
+    want = torch.autograd.grad(call(x, y, w).sum(), [x, y, w])
+    for reentrant in (False, True):
+        got = torch.autograd.grad(checkpoint(call, x, y, w, use_reentrant=False).sum(), [x, y, w]) if not reentrant else None
+        if reentrant:
+            checkpoint(call, x, y, w, use_reentrant=True).sum().backward()
+            got = [t.grad for t in (x, y, w)]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("unpack", ["shorter", "narrower", "elsewhere", "fake"])
+def test_saved_tensors_that_come_back_changed_are_refused(unpack):
+    """... before a kernel reads past their ends."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    changed = {"shorter": lambda v: v.flatten()[:1], "narrower": lambda v: v.to(torch.float16 if v.is_floating_point() else torch.int32), "elsewhere": lambda v: v.cpu(),
+               "fake": lambda v: FakeTensorMode(allow_non_fake_inputs=True).from_tensor(v)}[unpack]
+    for which in range(3):
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: changed(v.detach())):
+            case = _with_gradients()[which]
+        with pytest.raises(RuntimeError, match="saved tensor came back|subclass|Type"):
+            _gradients([case])
+
+
+def test_gradients_that_are_wrappers_are_refused():
+    for outs, leaves, _ in _with_gradients():
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(outs[:1], leaves[:1], [torch.stack([torch.ones_like(outs[0])] * 2)], is_grads_batched=True)
+
+
 # ------------------------------------------------------------------------------------------ residual norm
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("C", [1, 8, 33, 768, 4099])
