@@ -487,7 +487,9 @@ OptTensor rotary(const Tensor& qkv, const Tensor& positions, const Tensor& freqs
                  bool interleaved, bool inplace) {
   check_call("rotary", qkv, positions, freqs, axis);
   if (!rotary_taken(qkv, positions, freqs, axis, heads)) return std::nullopt;
-  const Tensor pos = positions.contiguous(), f = freqs.contiguous(), a = axis.to(at::kInt).contiguous();
+  const Tensor pos = positions.contiguous(), f = freqs.contiguous();
+  // (clamped first: an entry of 2^32 would become 0)
+  const Tensor a = (axis.scalar_type() == at::kLong ? axis.clamp(-1, positions.size(-1)) : axis).to(at::kInt).contiguous();
   if (inplace) {
     qkv.unsafeGetTensorImpl()->bump_version();      // (raises for an inference tensor outside inference mode)
     rotary_run(qkv, qkv, pos, f, a, heads, interleaved, false);

@@ -379,6 +379,15 @@ def test_token_logprobs_large_entropy_gradients_beside_masked_classes(size, dtyp
 
 
 # ------------------------------------------------------------------------------------------ rotary
+def test_rotary_axis_far_outside():
+    """An entry that does not fit 32 bits is outside like any other."""
+    qkv, pos = normal(gen(0), (1, 4, 48)), torch.arange(8, device="cuda").view(4, 2)
+    freqs, axis = torch.ones(8, device="cuda"), torch.tensor([0, 1, 2 ** 32, 0, -2 ** 32 + 1, 1, 2 ** 33 + 1, 0], device="cuda")
+    out = F().rotary(qkv, pos, freqs, axis, 1).view(4, 3, 2, 8)
+    outside = torch.tensor([False, False, True, False, True, False, True, False], device="cuda")
+    assert out[:, :2][..., outside].isnan().all() and out[..., ~outside].isfinite().all() and out[:, 2].isfinite().all()
+
+
 def test_rotary_in_place_of_an_inference_tensor():
     """Refused outside inference mode before anything is written, taken inside."""
     with torch.inference_mode():
