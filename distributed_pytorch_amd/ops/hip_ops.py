@@ -3226,6 +3226,8 @@ class SgdPlan:
             for p in group["params"]:
                 if p.grad is None:
                     continue
+                if not p.is_cuda:
+                    raise ValueError("FusedSGD: parameters on the CPU beside others on the GPU")
                 if p.dtype != torch.float32:
                     raise TypeError("FusedSGD HIP path needs fp32 parameters, got %s" % p.dtype)
                 if not _dense(p):

@@ -81,6 +81,8 @@ class MuonPlan:
                 continue
             shapes = {}
             for p in members:
+                if not p.is_cuda:
+                    raise ValueError("FusedMuon: parameters on the CPU beside others on the GPU")
                 if p.dtype != torch.float32:
                     raise TypeError("FusedMuon HIP path needs fp32 parameters, got %s" % p.dtype)
                 if not _dense(p):

@@ -169,10 +169,16 @@ class FusedSGD(Optimizer):
                 p.add_(g.to(p.dtype), alpha=-lr)
 
     def _step_hip(self, scaler) -> None:
+        self._prepare_hip()                          # (what it refuses, it refuses before anything is updated)
+        self._launch_hip(scaler)
+
+    def _prepare_hip(self) -> None:
         from .ops import hip_ops
 
         if self._plan is None or not self._plan.matches(self):
             self._plan = hip_ops.SgdPlan(self)
+
+    def _launch_hip(self, scaler) -> None:
         self._plan.launch(self, scaler)
         _amp.mark_copies_written(self._plan.params_with_copies)
 
@@ -314,13 +320,16 @@ class FusedMuon(FusedSGD):
                 p.mul_(1.0 - lr * group["weight_decay"])
                 p.add_(o.reshape(p.shape), alpha=-lr * group["matrix_scale"] * max(1.0, rows / cols) ** 0.5)
 
-    def _step_hip(self, scaler) -> None:
+    def _prepare_hip(self) -> None:
         from .ops.transformer_ops import MuonPlan
 
         if self._muon is None or not self._muon.matches(self):
             self._muon = MuonPlan(self)
+        super()._prepare_hip()
+
+    def _launch_hip(self, scaler) -> None:
         self._muon.launch(self, scaler)
-        super()._step_hip(scaler)                    # the other groups; then every derived copy is stale ...
+        super()._launch_hip(scaler)                  # the other groups; then every derived copy is stale ...
         self._muon.stamp_copies()                    # ... but those that this step wrote
         _amp.mark_copies_written([p for gt in self._muon.groups for p, lp in gt["plist"] if lp is not None])
 

@@ -432,3 +432,22 @@ def test_sgd_with_the_groups_of_a_muon_checkpoint():
     again.step()
     assert again.param_groups[0]["orthogonal"] is True and 0.0 < float((c[0] - before).norm()) < 0.1 * 0.2 * 1.3 * 24 ** 0.5
 
+
+@pytest.mark.parametrize("cpu", ["matrix", "vector"])
+def test_optimizers_refuse_parameters_of_the_cpu_beside_the_gpus(cpu):
+    """... whose addresses no kernel may read."""
+    from distributed_pytorch_amd.optim import FusedMuon, FusedSGD
+
+    def params():
+        ps = [torch.nn.Parameter(torch.ones(s, device="cpu" if (len(s) == 2) == (cpu == "matrix") else "cuda")) for s in ((4, 6), (5,))]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        return ps
+
+    a, b = params(), params()
+    for opt in (FusedMuon([dict(params=a[:1], orthogonal=True), dict(params=a[1:])], lr=0.1),
+                FusedSGD([dict(params=b[:1]), dict(params=b[1:])], lr=0.1)):
+        with pytest.raises(ValueError, match="CPU"):
+            opt.step()
+    for p in a + b:
+        assert bool((p == 1.0).all())
