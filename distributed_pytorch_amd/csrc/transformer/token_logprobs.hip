@@ -12,9 +12,9 @@
 // (order-preserving value bits, then the lower index), so ties go to the lowest index and the result does not depend on the
 // order of collection.  If more than the list's capacity reach the bound (many large elements with one lane), the k-th
 // largest collected becomes the new bound and the row is looked at again.  Few long rows are split over workgroups and
-// joined.  Bound by memory bandwidth and the exponentials' issue rate together: 2048 x 50257 bf16 with k = 20 48 us from the
-// last-level cache, 83 behind a backward pass's writes; backward 80 us (5.2 TB/s); 1024 x 1000 fp32 8 + 6 us; one row of 128000
-// fp32 9 us and 5 to join, bound by latency.
+// joined.  Bound by memory bandwidth and the exponentials' issue rate together: 2048 x 50257 bf16 with k = 20 63 us with inputs
+// from memory (3.3 TB/s), 84 behind a backward pass's writes; backward 80 us (5.2 TB/s); 1024 x 1000 fp32 9 + 6 us; one row of
+// 128000 fp32 10 us and 5 to join, bound by latency.
 #include "../common.h"
 #include "transformer.h"
 
@@ -89,11 +89,9 @@ template <typename T> __device__ __forceinline__ Vec16<T> load_any(const T* p) {
   return v;
 }
 typedef uint32_t any128 __attribute__((ext_vector_type(4), aligned(2)));
-// `stream`: not kept in the caches (the gradient of a vocabulary is larger than they are: 117 -> 103 us for 2048 x 50257)
-template <typename T> __device__ __forceinline__ void store_any(const Vec16<T>& v, T* p, bool stream) {
+template <typename T> __device__ __forceinline__ void store_any(const Vec16<T>& v, T* p) {
   const any128 x = {v.raw.x, v.raw.y, v.raw.z, v.raw.w};
-  if (stream) __builtin_nontemporal_store(x, reinterpret_cast<any128*>(p));
-  else *reinterpret_cast<any128*>(p) = x;
+  *reinterpret_cast<any128*>(p) = x;
 }
 
 template <typename T> __device__ __forceinline__ float chunk_max(const Vec16<T>& v) {
@@ -436,9 +434,9 @@ __global__ __launch_bounds__(kJoin) void token_logprobs_join_kernel(const TokenL
 
 // One part of a row.  The elements that carry a gradient of their own (the target and the k listed ones) are few: the pass
 // writes all elements without them, and a lane each then writes those again.  (Looking for them in the pass, by a bit per 8
-// columns, took 26 of 124 us of 2048 x 50257 bf16 with k = 20: nearly every row has waves that stop for them.)
+// columns, made it a fifth longer for 2048 x 50257 bf16 with k = 20: nearly every row has waves that stop for them.)
 template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogprobsBwd p, const int splits, const bool stream) {
+__global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogprobsBwd p, const int splits) {
   constexpr int V = 16 / (int)sizeof(T);
   __shared__ long idx[kTokenTopMax + 1];
   __shared__ float gx[kTokenTopMax + 1];
@@ -490,12 +488,12 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogp
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = load_any(z + c + u * kStep);
 #pragma unroll
-    for (int u = 0; u < U; ++u) store_any(chunk(v[u]), dz + c + u * kStep, stream);
+    for (int u = 0; u < U; ++u) store_any(chunk(v[u]), dz + c + u * kStep);
   }
   for (; c < hi; c += kStep) {
     const Vec16<T> o = chunk(load_chunk(z, c, hi));
     if (c + V <= hi) {
-      store_any(o, dz + c, stream);
+      store_any(o, dz + c);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j)
@@ -509,7 +507,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const TokenLogp
       g += gx[j];
       if (j < tid) at = -2;                        // (an element listed twice is written by the first lane that has it)
     }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the pass has written, streaming stores too
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the pass has written
   __syncthreads();
   if (at >= 0) dz[at] = from_float<T>(g);
 }
@@ -559,7 +557,7 @@ void token_logprobs_bwd_launch(const TokenLogprobsBwd& p, int dtype, hipStream_t
   if (splits < 1) splits = 1;
   if (p.N * splits >= (1l << 31)) throw std::invalid_argument("token_logprobs: too many rows");
   DPA_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(token_logprobs_bwd_kernel<T>, dim3((unsigned)(p.N * splits)), dim3(256), 0, s, p,
-                                               (int)splits, p.N * p.C * (long)sizeof(T) >= (32l << 20)));
+                                               (int)splits));
   DPA_CHECK_HIP(hipGetLastError());
 }
 
