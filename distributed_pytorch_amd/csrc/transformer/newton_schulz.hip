@@ -22,10 +22,11 @@
 //
 // Two product kernels (ns_use_large has the rule and its measurements):
 //  * 256 x 256 tiles, 8 waves: the half-tile ring of the framework's large GEMM (gemm8.hip has the ordering argument),
-//    bound by the matrix cores; the epilogue moves whole 128-byte row pieces through the free ring.  24 x 1024 x 4096 bf16, a
-//    step: A 126 us (0.82 PFLOP/s), B 47 us, X 370 us (0.56 PFLOP/s beside 1.2 GB of planes).
+//    bound by the matrix cores; the epilogue moves whole 128-byte row pieces through the free ring.  24 x 1024 x 4096, a
+//    step: A 322 us (0.96 PFLOP/s of fp16 products), B 105 us, X 681 us (0.91 PFLOP/s beside 1.6 GB of planes); `fast`:
+//    A 120 us (0.86 PFLOP/s), B 47 us, X 360 us (0.57 PFLOP/s beside 1.2 GB).
 //  * 64 x 64 and 128 x 128 tiles: for matrices too small or too few to fill the card with the large ones; bound by latency
-//    and by the L2's rate.  6 x 256 x 2304 fp32, a step: A 10 + 5 us (parts and their join), B 9 us, X 17 us.
+//    and by the L2's rate.  6 x 256 x 2304 fp32, a step: A 10 + 5 us (parts and their join), B 8 us, X 18 us.
 #include "../common.h"
 #include "transformer.h"
 #include <type_traits>

@@ -5,7 +5,7 @@
 //     dy = dz, or the same formula of `post` applied to it;  dw_post = sum dz * yh,  db_post = sum dz
 //
 // One pass: ds, dh, x, y are read once, dx and dy written once (64 x 197 x 1024 bf16 with `pre` 24 us, 5.3 TB/s; 64 x 3136 x
-// 96 bf16 with `post` 28 us, 4.1 TB/s; 24 x 257 x 1280 fp32 with both and a per-sample gate 42 us, 4.5 TB/s; the fold 4 us, a
+// 96 bf16 with `post` 28 us, 4.1 TB/s, with `pre` and a scale 51; 24 x 257 x 1280 fp32 with both and a per-sample gate 42 us, 4.5 TB/s; the fold 4 us, a
 // launch and a wait for memory).  s is formed again from x and y in 32 bits: the s of
 // the forward pass is rounded to T, and 1 / deviation and the sums over rows magnify that (dw_pre of bf16 rows is off by
 // 2e-3 from it, by 2e-7 from this), for one more tensor to read where there is no `post` (5 in place of 4).  The per-channel sums stay with the lane across all rows
@@ -363,8 +363,8 @@ struct Units {
   int splits;
   unsigned blocks;
 };
-// `parts`: how many workgroups the card holds at once (64 x 197 x 1024 bf16 with its fold: 31 us with the 512 that fit, 32 with
-// 256, 35 with 768, which take two turns)
+// `parts`: how many workgroups the card holds at once.  With that many, 256 and 768, the pass with its fold, us: 64 x 197 x 1024
+// bf16 (512 fit) 27 : 28 : 32, 64 x 3136 x 96 bf16 29 : 52 : 30, 24 x 257 x 1280 fp32 47 : 75 : 47
 Units units_of(long rows, long per_sample, const Plan& pl, long parts, int gate_kind) {
   Units u;
   const long trip = pl.rows_per_trip;

@@ -656,7 +656,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750
     updates: ``X = g / (|g|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` (on the
     transposed matrix where ``m > n``).  With the default ``coefficients`` ``(a, b, c)`` five steps move the singular
     values into about [0.7, 1.2].  Products have about 22 significant bits and are summed in 32, whatever ``g``'s type; the
-    result is rounded to that type once.  No gradient.  A matrix with an infinity or a NaN gives NaN.
+    result is rounded to that type once.  No gradient.  A matrix with an infinity or a NaN gives NaN.  The GPU takes up to
+    65535 matrices a call.
 
     ``fast``, for bfloat16 alone: the GPU's products take operands of 11 significant bits, at a third of the matrix work.  The
     result is then off by 2e-4 to 7e-4 of its norm before it is rounded to bfloat16 (1.7e-3), 2e-3 where a few directions
